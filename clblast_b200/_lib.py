@@ -2,7 +2,7 @@
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_int, c_size_t, c_uint64, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_int, c_size_t, c_uint64, c_void_p, POINTER
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libclblast.so"
@@ -58,6 +58,26 @@ def lib() -> ctypes.CDLL:
         f = getattr(L, name)
         f.restype = i
         f.argtypes = [i, i] + [sz] * 11 + [vp, sz, vp, sz, vp, i]
+    d = c_double
+    L.b200blas_gemm_epilogue.restype = i
+    L.b200blas_gemm_epilogue.argtypes = [i, i, i, i, i, sz, sz, sz, d, vp, sz, sz, vp, sz, sz, vp, sz, i, vp, sz, sz, d,
+                                         vp, sz, sz, vp, sz, sz, vp, i]
+    L.b200blas_gemm_epilogue_grad.restype = i
+    L.b200blas_gemm_epilogue_grad.argtypes = [i, i, i, i, sz, sz, sz, d, vp, sz, sz, vp, sz, sz, d, vp, sz, sz, i, vp, sz,
+                                              sz, vp, sz, sz, vp, sz, vp, i]
+    L.b200blas_activation_grad.restype = i
+    L.b200blas_activation_grad.argtypes = [i, sz, sz, i, vp, sz, sz, vp, sz, sz, vp, sz, sz, vp, sz, sz, vp, sz, vp, i]
+    L.b200blas_gemm_grouped.restype = i
+    L.b200blas_gemm_grouped.argtypes = [i, i, i, sz, sz, sz, sz, d, vp, sz, sz, vp, sz, sz, sz, vp, vp, sz, sz, i, vp, sz,
+                                        sz, d, vp, sz, sz, vp, sz, sz, vp, i]
+    L.b200blas_gemm_grouped_grad.restype = i
+    L.b200blas_gemm_grouped_grad.argtypes = [i, i, sz, sz, sz, sz, d, vp, sz, sz, vp, sz, sz, sz, vp, d, vp, sz, sz, i,
+                                             vp, sz, sz, vp, sz, sz, vp, sz, sz, vp, i]
+    L.b200blas_gemm_grouped_weight.restype = i
+    L.b200blas_gemm_grouped_weight.argtypes = [i, i, sz, sz, sz, sz, d, vp, sz, sz, vp, sz, sz, vp, d, vp, sz, sz, sz, vp,
+                                               i]
+    L.b200blas_newton_schulz.restype = i
+    L.b200blas_newton_schulz.argtypes = [i, i, sz, sz, d, vp, sz, sz, sz, vp, sz, sz, sz, sz, sz, POINTER(d), sz, d, vp, i]
     L.b200blas_gemm_temp_buffer_size.restype = i
     L.b200blas_gemm_temp_buffer_size.argtypes = [i, i, i, i] + [sz] * 9 + [POINTER(sz)]
     L.b200blas_clear_cache.restype = i
@@ -100,6 +120,8 @@ C_ABI_SYMBOLS = [
     "b200blas_gemm", "b200blas_gemm_strided_batched", "b200blas_gemm_batched", "b200blas_gemm_batched_static",
     "b200blas_convgemm", "b200blas_symm", "b200blas_hemm", "b200blas_syrk", "b200blas_herk", "b200blas_syr2k",
     "b200blas_her2k", "b200blas_trmm", "b200blas_trsm", "b200blas_omatcopy", "b200blas_im2col", "b200blas_col2im",
+    "b200blas_gemm_epilogue", "b200blas_gemm_epilogue_grad", "b200blas_activation_grad", "b200blas_gemm_grouped",
+    "b200blas_gemm_grouped_grad", "b200blas_gemm_grouped_weight", "b200blas_newton_schulz",
     "b200blas_gemm_temp_buffer_size", "b200blas_clear_cache", "b200blas_fill_cache", "b200blas_override_parameters",
     "b200blas_retrieve_parameters", "b200blas_set_sm_budget", "b200blas_tensor_core_status", "b200blas_ipc_export", "b200blas_ipc_open",
     "b200blas_ipc_close", "b200blas_stream_copy", "b200blas_stream_wait_flag", "b200blas_stream_write_flag", "b200blas_last_kernel", "b200blas_launch_count", "b200blas_version",

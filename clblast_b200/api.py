@@ -34,6 +34,10 @@ class StatusCode(enum.IntEnum):
     kInsufficientMemoryA = -1011
     kInsufficientMemoryB = -1010
     kInsufficientMemoryC = -1009
+    kInvalidVectorX = -1019
+    kInvalidVectorY = -1018
+    kInsufficientMemoryX = -1008
+    kInsufficientMemoryY = -1007
     kInsufficientMemoryTemp = -2050
     kInvalidBatchCount = -2049
     kInvalidOverrideKernel = -2048
@@ -76,8 +80,18 @@ class KernelMode(enum.IntEnum):
     kConvolution = 152
 
 
+class Activation(enum.IntEnum):
+    """Activations of the products with an epilogue (no counterpart in the reference)."""
+    kIdentity = 161
+    kRelu = 162
+    kGelu = 163
+    kGeluTanh = 164
+    kSilu = 165
+
+
 class Precision(enum.IntEnum):
     kHalf = 16
+    kBFloat16 = 1016  # only in the products around a transformer block
     kSingle = 32
     kDouble = 64
     kComplexSingle = 3232
@@ -331,6 +345,138 @@ def Col2im(kernel_mode, channels, height, width, kernel_h, kernel_w, pad_h, pad_
     return _status(lib().b200blas_col2im(p, int(kernel_mode), channels, height, width, kernel_h, kernel_w, pad_h, pad_w,
                                          stride_h, stride_w, dilation_h, dilation_w, _ptr(col_buffer), col_offset,
                                          _ptr(im_buffer), im_offset, sp, is_async))
+
+
+# ---- products around a transformer block (no counterpart in the reference) -------------------------------------------
+
+_TORCH_CODE = {}
+
+
+def _code(dtype) -> int:
+    """Precision code of a torch dtype, 0 for one that the library does not know."""
+    if not _TORCH_CODE:
+        import torch
+        _TORCH_CODE.update({torch.float16: 16, torch.bfloat16: 1016, torch.float32: 32, torch.float64: 64,
+                            torch.complex64: 3232, torch.complex128: 6464})
+    return _TORCH_CODE.get(dtype, 0)
+
+
+def _types(operand, result, others, precision, c_precision):
+    """(dtype, c_dtype) of a call, from the arguments or from the tensors; tensors of another type are refused."""
+    p = int(precision) if precision is not None else _code(getattr(operand, "dtype", None))
+    if p == 0:
+        raise TypeError("pass precision= for raw pointers or unsupported tensor dtypes")
+    c = int(c_precision) if c_precision is not None else (_code(getattr(result, "dtype", None)) or p)
+    for buf, want in others:
+        if buf is not None and hasattr(buf, "dtype") and _code(buf.dtype) != (c if want == "c" else p):
+            raise TypeError(f"a tensor of {buf.dtype} where the call needs precision {c if want == 'c' else p}")
+    return p, c
+
+
+def _offsets(buf) -> int:
+    if hasattr(buf, "dtype"):
+        import torch
+        if buf.dtype != torch.int64 or not buf.is_contiguous():
+            raise TypeError("group offsets are contiguous 64-bit integers")
+    return _ptr(buf)
+
+
+def GemmEpilogue(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer, a_offset, a_ld, b_buffer, b_offset, b_ld,
+                 bias_buffer, bias_offset, activation, z_buffer, z_offset, z_ld, beta, d_buffer, d_offset, d_ld, c_buffer,
+                 c_offset, c_ld, *, precision=None, c_precision=None, stream=None):
+    """Z = alpha*op(A)*op(B) + bias, C = activation(Z) + beta*D; bias runs along C's unit-stride extent.
+
+    ``bias_buffer``, ``z_buffer`` (stores Z for the backward pass) and ``d_buffer`` may be None. Half, bfloat16 or
+    single; C and D may be single with 16-bit operands (``c_precision``)."""
+    p, c = _types(a_buffer, c_buffer, ((b_buffer, "a"), (bias_buffer, "a"), (z_buffer, "a"), (d_buffer, "c"), (c_buffer, "c")),
+                  precision, c_precision)
+    sp, is_async = _stream_arg(stream)
+    return _status(lib().b200blas_gemm_epilogue(
+        p, c, layout, a_transpose, b_transpose, m, n, k, alpha, _ptr(a_buffer), a_offset, a_ld,
+        _ptr(b_buffer), b_offset, b_ld, _ptr(bias_buffer), bias_offset, activation, _ptr(z_buffer), z_offset, z_ld,
+        beta, _ptr(d_buffer), d_offset, d_ld, _ptr(c_buffer), c_offset, c_ld, sp, is_async))
+
+
+def GemmEpilogueGrad(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer, a_offset, a_ld, b_buffer, b_offset, b_ld,
+                     beta, d_buffer, d_offset, d_ld, activation, z_buffer, z_offset, z_ld, c_buffer, c_offset, c_ld,
+                     bias_grad_buffer, bias_grad_offset, *, precision=None, stream=None):
+    """C = (alpha*op(A)*op(B) + beta*D) * activation'(Z), bias_grad = sums of C along its bias extent.
+
+    The backward pass through the activation of :func:`GemmEpilogue`: A is the gradient behind the next product, op(B)
+    that product's weights the other way round. ``d_buffer`` and ``bias_grad_buffer`` may be None."""
+    p, _ = _types(a_buffer, c_buffer, ((b_buffer, "a"), (d_buffer, "a"), (z_buffer, "a"), (c_buffer, "a"), (bias_grad_buffer, "a")),
+                  precision, precision)
+    sp, is_async = _stream_arg(stream)
+    return _status(lib().b200blas_gemm_epilogue_grad(
+        p, layout, a_transpose, b_transpose, m, n, k, alpha, _ptr(a_buffer), a_offset, a_ld,
+        _ptr(b_buffer), b_offset, b_ld, beta, _ptr(d_buffer), d_offset, d_ld, activation, _ptr(z_buffer), z_offset,
+        z_ld, _ptr(c_buffer), c_offset, c_ld, _ptr(bias_grad_buffer), bias_grad_offset, sp, is_async))
+
+
+def ActivationGrad(rows, n, activation, dy_buffer, dy_offset, dy_ld, z_buffer, z_offset, z_ld, dz_buffer, dz_offset, dz_ld,
+                   bias_grad_buffer, bias_grad_offset, *, groups=0, group_offsets=None, bias_grad_ld=0, precision=None,
+                   stream=None):
+    """DZ = DY * activation'(Z) for ``rows`` contiguous vectors of n elements, bias_grad = sums of DZ over the rows (of
+    each group, when ``groups`` > 0). DZ or bias_grad may be None."""
+    p, _ = _types(dy_buffer, dz_buffer, ((z_buffer, "a"), (dz_buffer, "a"), (bias_grad_buffer, "a")), precision, precision)
+    sp, is_async = _stream_arg(stream)
+    return _status(lib().b200blas_activation_grad(
+        p, rows, n, activation, _ptr(dy_buffer), dy_offset, dy_ld, _ptr(z_buffer), z_offset, z_ld, _ptr(dz_buffer),
+        dz_offset, dz_ld, _ptr(bias_grad_buffer), bias_grad_offset, groups, _offsets(group_offsets), bias_grad_ld, sp,
+        is_async))
+
+
+def GemmGrouped(w_transpose, groups, rows, n, k, alpha, x_buffer, x_offset, x_ld, w_buffer, w_offset, w_ld, w_stride,
+                group_offsets, bias_buffer, bias_offset, bias_ld, activation, z_buffer, z_offset, z_ld, beta, d_buffer,
+                d_offset, d_ld, c_buffer, c_offset, c_ld, *, precision=None, c_precision=None, stream=None):
+    """Rows sorted by group, each group with weights of its own: C = activation(alpha*X*op(W_g) + bias_g) + beta*D.
+
+    ``group_offsets``: device array of groups + 1 ascending 64-bit row numbers, read when the work runs. Rows of no
+    group are left as they were. Half or bfloat16; C and D may be single."""
+    p, c = _types(x_buffer, c_buffer, ((w_buffer, "a"), (bias_buffer, "a"), (z_buffer, "a"), (d_buffer, "c"), (c_buffer, "c")),
+                  precision, c_precision)
+    sp, is_async = _stream_arg(stream)
+    return _status(lib().b200blas_gemm_grouped(
+        p, c, w_transpose, groups, rows, n, k, alpha, _ptr(x_buffer), x_offset, x_ld, _ptr(w_buffer), w_offset, w_ld,
+        w_stride, _offsets(group_offsets), _ptr(bias_buffer), bias_offset, bias_ld, activation, _ptr(z_buffer),
+        z_offset, z_ld, beta, _ptr(d_buffer), d_offset, d_ld, _ptr(c_buffer), c_offset, c_ld, sp, is_async))
+
+
+def GemmGroupedGrad(w_transpose, groups, rows, n, k, alpha, x_buffer, x_offset, x_ld, w_buffer, w_offset, w_ld, w_stride,
+                    group_offsets, beta, d_buffer, d_offset, d_ld, activation, z_buffer, z_offset, z_ld, c_buffer,
+                    c_offset, c_ld, bias_grad_buffer, bias_grad_offset, bias_grad_ld, *, precision=None, stream=None):
+    """C = (alpha*X*op(W_g) + beta*D) * activation'(Z) row by row, bias_grad_g = sums of C over the rows of group g."""
+    p, _ = _types(x_buffer, c_buffer, ((w_buffer, "a"), (d_buffer, "a"), (z_buffer, "a"), (c_buffer, "a"), (bias_grad_buffer, "a")),
+                  precision, precision)
+    sp, is_async = _stream_arg(stream)
+    return _status(lib().b200blas_gemm_grouped_grad(
+        p, w_transpose, groups, rows, n, k, alpha, _ptr(x_buffer), x_offset, x_ld, _ptr(w_buffer), w_offset, w_ld,
+        w_stride, _offsets(group_offsets), beta, _ptr(d_buffer), d_offset, d_ld, activation, _ptr(z_buffer), z_offset,
+        z_ld, _ptr(c_buffer), c_offset, c_ld, _ptr(bias_grad_buffer), bias_grad_offset, bias_grad_ld, sp, is_async))
+
+
+def GemmGroupedWeight(groups, rows, m, n, alpha, x_buffer, x_offset, x_ld, y_buffer, y_offset, y_ld, group_offsets, beta,
+                      c_buffer, c_offset, c_ld, c_stride, *, precision=None, c_precision=None, stream=None):
+    """C_g = alpha*X_g^T*Y_g + beta*C_g over the rows of group g: the weight gradients of :func:`GemmGrouped`."""
+    p, c = _types(x_buffer, c_buffer, ((y_buffer, "a"), (c_buffer, "c")), precision, c_precision)
+    sp, is_async = _stream_arg(stream)
+    return _status(lib().b200blas_gemm_grouped_weight(
+        p, c, groups, rows, m, n, alpha, _ptr(x_buffer), x_offset, x_ld, _ptr(y_buffer), y_offset, y_ld,
+        _offsets(group_offsets), beta, _ptr(c_buffer), c_offset, c_ld, c_stride, sp, is_async))
+
+
+def NewtonSchulz(layout, m, n, alpha, a_buffer, a_offset, a_ld, a_stride, b_buffer, b_offset, b_ld, b_stride, batch_count, *,
+                 steps=5, coefficients=(3.4445, -4.7750, 2.0315), epsilon=1e-7, precision=None, stream=None):
+    """B = alpha * orthogonalised A for ``batch_count`` m x n matrices: X = A / (|A|_F + epsilon), then ``steps`` times
+    X <- a*X + (b*G + c*G*G)*X with G = X*X^T on the shorter side.
+
+    ``coefficients``: one triple (a, b, c), or a sequence of at least ``steps`` triples. B may be A."""
+    p, _ = _types(a_buffer, b_buffer, ((b_buffer, "a"),), precision, precision)
+    flat = np.ascontiguousarray(np.asarray(coefficients, dtype=np.float64)).reshape(-1, 3)
+    sp, is_async = _stream_arg(stream)
+    return _status(lib().b200blas_newton_schulz(
+        p, layout, m, n, alpha, _ptr(a_buffer), a_offset, a_ld, a_stride, _ptr(b_buffer), b_offset, b_ld, b_stride,
+        batch_count, steps, flat.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), len(flat), epsilon, sp, is_async))
 
 
 def GemmTempBufferSize(layout, a_transpose, b_transpose, m, n, k, a_offset, a_ld, b_offset, b_ld, c_offset, c_ld, *,

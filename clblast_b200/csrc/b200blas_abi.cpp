@@ -26,6 +26,7 @@
 #include "noalloc_bridge.h"
 #include "params_store.h"
 #include "runtime_state.h"
+#include "scratch.h"
 #include "host_common.h"
 
 namespace b200 {
@@ -264,6 +265,14 @@ cudaError_t dispatch(const GemmDesc& d, cudaStream_t stream) {
   if (err == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
   if (verbose_level() > 0) log_launch(d, name, err, stream);
   return err;
+}
+
+// Bookkeeping of a call that did not go through dispatch().
+void note_launch(const char* name, cudaError_t err) {
+  t_last_kernel = name;
+  if (err == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
+  if (verbose_level() > 0)
+    std::fprintf(stderr, "[b200blas] %s -> %s\n", name, err == cudaSuccess ? "enqueued" : cudaGetErrorString(err));
 }
 
 // Runs `d` either synchronously on the private stream or asynchronously on the caller's stream.
@@ -663,7 +672,10 @@ extern "C" int b200blas_gemm_temp_buffer_size(int dtype, int layout, int ta, int
 
 extern "C" void b200blas_set_sm_budget(int sms) { g_sm_budget.store(sms > 0 ? sms : 0, std::memory_order_relaxed); }
 
-extern "C" int b200blas_clear_cache(void) { return kSuccess; }
+extern "C" int b200blas_clear_cache(void) {
+  scratch_trim();
+  return kSuccess;
+}
 extern "C" int b200blas_fill_cache(int) { return kSuccess; }
 
 extern "C" int b200blas_tensor_core_status(unsigned int out[4], int clear) {

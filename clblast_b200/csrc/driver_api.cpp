@@ -16,6 +16,7 @@ DriverApi bind() {
   api.CtxPopCurrent = reinterpret_cast<decltype(api.CtxPopCurrent)>(sym("cuCtxPopCurrent_v2"));
   api.CtxGetId = reinterpret_cast<decltype(api.CtxGetId)>(sym("cuCtxGetId"));
   api.MemGetAddressRange = reinterpret_cast<decltype(api.MemGetAddressRange)>(sym("cuMemGetAddressRange_v2"));
+  api.PointerGetAttribute = reinterpret_cast<decltype(api.PointerGetAttribute)>(sym("cuPointerGetAttribute"));
   api.TensorMapEncodeTiled = reinterpret_cast<decltype(api.TensorMapEncodeTiled)>(sym("cuTensorMapEncodeTiled"));
   api.StreamWaitValue32 = reinterpret_cast<decltype(api.StreamWaitValue32)>(sym("cuStreamWaitValue32_v2"));
   api.StreamWriteValue32 = reinterpret_cast<decltype(api.StreamWriteValue32)>(sym("cuStreamWriteValue32_v2"));

@@ -18,6 +18,7 @@ struct DriverApi {
   CUresult (*TensorMapEncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  CUresult (*PointerGetAttribute)(void*, CUpointer_attribute, CUdeviceptr);  // may be null on old drivers
   // Stream memory operations (used by the multi-GPU helpers only; may be null on old drivers).
   CUresult (*StreamWaitValue32)(CUstream, CUdeviceptr, cuuint32_t, unsigned int);
   CUresult (*StreamWriteValue32)(CUstream, CUdeviceptr, cuuint32_t, unsigned int);

@@ -1,0 +1,272 @@
+#include "fused_host.h"
+
+#include <cuda.h>
+
+#include <cstdint>
+#include <cstdio>
+#include <cstdlib>
+#include <cstring>
+
+#include "driver_api.h"
+#include "kernels/fused_aux.h"
+#include "kernels/launchers.h"
+#include "runtime_state.h"
+#include "scratch.h"
+#include "tc_host.h"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kMaxSmem = 232448;  // 227 KB
+constexpr int kBarBytes = 512, kSlot = 4096, kRing = 4, kAlign = 1024;
+
+int elem_size(int type) { return type == 32 ? 4 : 2; }
+
+// Tensor map of an epilogue matrix (m contiguous): boxes of 128 rows and 32 bytes' worth of columns, no swizzle.
+bool encode_block_map(CUtensorMap* map, int type, int cols, const void* base, long long m, long long n, long long ld,
+                      long long planes, long long stride) {
+  const DriverApi& drv = driver_api();
+  if (!drv.ok || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
+  const long long elem = elem_size(type);
+  const cuuint64_t row_bytes = static_cast<cuuint64_t>(ld * elem);
+  const cuuint64_t plane_bytes = planes > 1 ? static_cast<cuuint64_t>(stride * elem) : row_bytes;
+  if ((row_bytes & 15) || (plane_bytes & 15) || row_bytes >= (1ULL << 40) || plane_bytes >= (1ULL << 40)) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(m), static_cast<cuuint64_t>(n),
+                              static_cast<cuuint64_t>(planes > 1 ? planes : 1)};
+  const cuuint64_t strides[2] = {row_bytes, plane_bytes};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(cols), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType dt = elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  return drv.TensorMapEncodeTiled(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Choice {
+  int variant, split;
+};
+
+constexpr const char* kNames[kFusedVariants] = {"fused_pair_256x256x64", "fused_128x256x64", "fused_128x128x64",
+                                                "fused_128x64x64", "fused_128x32x64"};
+
+// Upper bound of the column tiles of a call (exact for the plain kinds).
+long long column_tiles(const FusedDesc& d, int bn) {
+  const long long whole = (d.n + bn - 1) / bn;
+  return d.kind == kFusedRaggedCols ? whole + d.problems : whole;
+}
+
+bool variant_fits(const FusedDesc& d, int v, int split) {
+  const FusedVariant& t = kFusedTable[v];
+  if (t.ctas == 2 && (d.kind == kFusedRaggedInner || split > 1)) return false;  // its peer cannot clear the inner tail
+  if (d.b_mn && t.bn / t.ctas < 64) return false;                               // a 128-byte row is 64 columns
+  if (d.tri && !(t.ctas * 128 == t.bn)) return false;                           // square tiles meet their mirror image
+  if (split > 1 && (t.bn / split) % 4 != 0) return false;
+  if (split > 1 && d.tri) return false;
+  return true;
+}
+
+// Teams of `team` CTAs that run at once, within the caller's limit on SMs.
+int resident_teams(int team) {
+  int n = fused_resident_clusters(team);
+  if (sm_budget() > 0 && sm_budget() / team < n) n = sm_budget() / team;
+  return n > 0 ? n : 1;
+}
+
+// Time in SM cycles by a small model: waves of tiles x (inner blocks x the slower of the MMAs and the operand loads of a
+// block) + the drain of the last tile, against the memory traffic of the whole call.
+double estimate(const FusedDesc& d, int v, int split) {
+  const FusedVariant& t = kFusedTable[v];
+  const double tm = static_cast<double>((d.m + 128 * t.ctas - 1) / (128 * t.ctas));
+  double tn, problems = 1, k = static_cast<double>(d.k);
+  if (d.kind == kFusedRaggedCols) {
+    const double active = static_cast<double>(d.problems < d.n ? d.problems : d.n);
+    const double each = static_cast<double>(d.n) / active;
+    tn = active * static_cast<double>(static_cast<long long>((each + t.bn - 1) / t.bn));
+  } else {
+    tn = static_cast<double>((d.n + t.bn - 1) / t.bn);
+    problems = static_cast<double>(d.problems);
+    if (d.kind == kFusedRaggedInner) k = k / problems;
+  }
+  double tiles = tm * tn * problems;
+  if (d.tri) tiles = tm * (tm + 1) / 2 * problems;
+  const double blocks = static_cast<double>(static_cast<long long>((k + 63) / 64));
+  const double per_block_mma = t.ctas == 2 ? 530.0 : (t.bn == 256 ? 530.0 : (t.bn == 128 ? 270.0 : (t.bn == 64 ? 150.0 : 110.0)));
+  const double per_block_load = t.stage_bytes / 60.0;
+  const double per_block = per_block_mma > per_block_load ? per_block_mma : per_block_load;
+  const double teams = static_cast<double>(resident_teams(t.ctas * split));
+  const double waves = static_cast<double>(static_cast<long long>((tiles + teams - 1) / teams));
+  const double inner = static_cast<double>(static_cast<long long>((blocks + split - 1) / split));
+  const double drain = 1500.0 + 12.0 * t.bn + (split > 1 ? 1500.0 : 0.0);
+  return waves * (inner * per_block + 400.0) + drain + 1500.0;
+}
+
+Choice choose(const FusedDesc& d) {
+  Choice best = {2, 1};
+  double best_time = 1e300;
+  for (int v = 0; v < kFusedVariants; ++v) {
+    for (int split = 1; split <= 8; split *= 2) {
+      if (!variant_fits(d, v, split)) continue;
+      const double time = estimate(d, v, split);
+      if (time < best_time * 0.999) {
+        best_time = time;
+        best = {v, split};
+      }
+    }
+  }
+  // B200BLAS_FUSED=<variant>[,<split>] forces one for measurements and tests where it can serve the call.
+  if (const char* env = std::getenv("B200BLAS_FUSED")) {
+    int v = -1, split = 1;
+    if (std::sscanf(env, "%d,%d", &v, &split) >= 1 && v >= 0 && v < kFusedVariants && split >= 1 && split <= 8 &&
+        (split & (split - 1)) == 0 && variant_fits(d, v, split))
+      best = {v, split};
+  }
+  return best;
+}
+
+bool unaddressable(const void* base, long long ld, long long planes, long long stride) {
+  return (reinterpret_cast<uintptr_t>(base) & 15) != 0 || (ld % 8) != 0 || (planes > 1 && (stride % 8) != 0);
+}
+
+}  // namespace
+
+cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** name) {
+  // an operand with stride 0 is shared by all problems
+  const long long a_planes = d.kind == kFusedRaggedInner || d.a_stride == 0 ? 1 : d.problems;
+  const long long b_planes = d.kind == kFusedPlain && d.b_stride != 0 ? d.problems : 1;
+  // Operands that TMA cannot address are copied once to an aligned pitch.
+  PoolScratch a_copy, b_copy, partial;
+  FusedDesc r = d;
+  auto pack = [&](PoolScratch& to, const void*& base, long long& ld, long long& stride, bool mn, long long rows,
+                  long long planes) -> cudaError_t {
+    if (!unaddressable(base, ld, planes, stride)) return cudaSuccess;
+    PackJob job;
+    job.one = mn ? rows : d.k;
+    job.two = mn ? d.k : rows;
+    job.planes = planes;
+    job.src = base;
+    job.src_ld = ld;
+    job.src_stride = planes > 1 ? stride : 0;
+    job.pitch = (job.one + 7) / 8 * 8;
+    const cudaError_t e = to.get(static_cast<size_t>(job.pitch) * job.two * planes * 2, stream);
+    if (e != cudaSuccess) return e;
+    job.dst = to.ptr();
+    base = to.ptr();
+    ld = job.pitch;
+    stride = job.pitch * job.two;
+    return launch_pack(job, stream);
+  };
+  cudaError_t e = pack(a_copy, r.a, r.lda, r.a_stride, d.a_mn != 0, d.m, a_planes);
+  if (e == cudaSuccess) e = pack(b_copy, r.b, r.ldb, r.b_stride, d.b_mn != 0, d.n, b_planes);
+  if (e != cudaSuccess) return e;
+
+  const Choice choice = choose(d);
+  const FusedVariant& t = kFusedTable[choice.variant];
+  FusedParams p = {};
+  p.status = tc_status_device();
+  p.m = static_cast<int>(d.m);
+  p.n = static_cast<int>(d.n);
+  p.k = static_cast<int>(d.k);
+  p.kind = d.kind;
+  p.problems = static_cast<int>(d.problems);
+  p.offsets = d.offsets;
+  p.tiles_m = static_cast<int>((d.m + 128 * t.ctas - 1) / (128 * t.ctas));
+  p.tiles_n = static_cast<int>((d.n + t.bn - 1) / t.bn);
+  p.raster = t.ctas == 2 ? 8 : 16;
+  p.tri = d.tri;
+  p.a_mn = d.a_mn;
+  p.b_mn = d.b_mn;
+  const unsigned format = d.type == 16 ? 0u : 1u;  // fp32 accumulator; f16 or bf16 operands
+  p.idesc = (1u << 4) | (format << 7) | (format << 10) | (static_cast<unsigned>(d.a_mn != 0) << 15) |
+            (static_cast<unsigned>(d.b_mn != 0) << 16) | (static_cast<unsigned>(t.bn >> 3) << 17) |
+            (static_cast<unsigned>((128 * t.ctas) >> 4) << 24);
+  p.a_batched = a_planes > 1;
+  p.b_batched = b_planes > 1;
+  p.split = choice.split;
+  p.alpha = static_cast<float>(d.alpha);
+  p.beta = static_cast<float>(d.beta);
+  p.bias = d.bias;
+  p.bias_stride = d.bias_stride;
+  p.act = d.act;
+  p.grad = d.grad;
+  p.c = d.c; p.ldc = d.ldc; p.c_stride = d.c_stride;
+  p.d = d.beta != 0.0 ? d.d : nullptr; p.ldd = d.ldd; p.d_stride = d.d_stride;
+  p.z = d.z; p.ldz = d.ldz; p.z_stride = d.z_stride;
+  p.hint_a = p.hint_b = 2;
+
+  CUtensorMap maps[5];
+  std::memset(maps, 0, sizeof(maps));
+  if (!encode_operand_map(&maps[0], 2, r.a, d.m, d.k, r.lda, d.a_mn != 0, 128, a_planes, r.a_stride) ||
+      !encode_operand_map(&maps[1], 2, r.b, d.n, d.k, r.ldb, d.b_mn != 0, t.bn / t.ctas, b_planes, r.b_stride))
+    return cudaErrorInvalidValue;
+  const int cols = 32 / elem_size(d.c_type);
+  const long long c_planes = d.kind == kFusedRaggedCols ? 1 : d.problems;
+  // Columns of a group are cut off by 16-byte copies: m has to be a multiple of 16 bytes there.
+  bool tma = d.kind != kFusedRaggedCols || d.m % 8 == 0;
+  tma = tma && encode_block_map(&maps[2], d.c_type, cols, d.c, d.m, d.n, d.ldc, c_planes, d.c_stride);
+  if (tma && p.d) tma = encode_block_map(&maps[3], d.d_type, cols, p.d, d.m, d.n, d.ldd, c_planes, d.d_stride);
+  if (tma && p.z) tma = encode_block_map(&maps[4], d.type, cols, p.z, d.m, d.n, d.ldz, c_planes, d.z_stride);
+  p.tma = tma ? 1 : 0;
+
+  const long long col_tiles = column_tiles(d, t.bn);
+  long long tiles = col_tiles * p.tiles_m;
+  if (d.kind != kFusedRaggedCols) tiles *= d.problems;
+  if (d.tri) tiles = static_cast<long long>(p.tiles_m) * (p.tiles_m + 1) / 2 * d.problems;
+  if (tiles > 0x3FFFFFFF) return cudaErrorInvalidValue;
+  const int lines_per_tile = t.epi_groups * choice.split;
+  if (d.bias_grad != nullptr) {
+    e = partial.get(static_cast<size_t>(col_tiles) * lines_per_tile * d.m * sizeof(float), stream);
+    if (e != cudaSuccess) return e;
+    p.partial = reinterpret_cast<float*>(partial.ptr());
+  }
+
+  // shared memory: the ring takes what staging, barriers and the group table leave
+  const int staging = t.epi_groups * kRing * kSlot * (p.z ? 2 : 1);
+  const int sums = choice.split > 1 ? t.bn * 128 * 4 : 0;
+  const int table = d.kind == kFusedRaggedCols ? 8 * (p.problems + 1) : 0;
+  const int fixed = kAlign + (staging > sums ? staging : sums) + kBarBytes + table;
+  int stages = (kMaxSmem - fixed) / t.stage_bytes;
+  if (stages > 12) stages = 12;
+  if (stages < 2) return cudaErrorInvalidValue;
+  p.stages = stages;
+  const int smem = fixed + stages * t.stage_bytes;
+
+  const int team = t.ctas * choice.split;
+  long long teams = resident_teams(team);
+  if (tiles < teams) teams = tiles;
+  e = launch_fused_variant(choice.variant, d.type, d.d_type, d.c_type, maps, p, static_cast<int>(teams) * team, smem, stream);
+  static thread_local char label[64];
+  if (choice.split > 1) std::snprintf(label, sizeof(label), "%s_split%d", kNames[choice.variant], choice.split);
+  else std::snprintf(label, sizeof(label), "%s", kNames[choice.variant]);
+  *name = label;
+  if (e == cudaSuccess && d.bias_grad != nullptr) {
+    SumJob job = {};
+    job.partial = p.partial;
+    job.m = d.m;
+    job.type = d.type;
+    job.out = d.bias_grad;
+    job.out_stride = d.bias_grad_stride;
+    job.offsets = d.kind == kFusedRaggedCols ? d.offsets : nullptr;
+    job.groups = p.problems;
+    job.bound = d.n;
+    job.per_tile = t.bn;
+    job.lines_per_tile = lines_per_tile;
+    job.tiles = col_tiles;
+    e = launch_sum_partials(job, stream);
+  }
+  return e;
+}
+
+cudaError_t launch_fused_variant(int v, int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p,
+                                 int grid, int smem, cudaStream_t stream) {
+  switch (v) {
+    case 0: return launch_fused_pair(type, d_type, c_type, maps, p, grid, smem, stream);
+    case 1: return launch_fused_256(type, d_type, c_type, maps, p, grid, smem, stream);
+    case 2: return launch_fused_128(type, d_type, c_type, maps, p, grid, smem, stream);
+    case 3: return launch_fused_64(type, d_type, c_type, maps, p, grid, smem, stream);
+    case 4: return launch_fused_32(type, d_type, c_type, maps, p, grid, smem, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace b200

@@ -1,0 +1,78 @@
+// Launch interface of the fused 16-bit products: bias, activation, residual and their gradients in the epilogue, and
+// ragged groups of rows (csrc/fused_abi.cpp holds the entry points, csrc/fused_host.cpp the selection).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime_api.h>
+
+namespace b200 {
+
+constexpr int kBFloat16 = 1016;  // precision code of bfloat16, known to the fused routines only
+
+// What the ragged extent of a grouped call is.
+enum FusedKind : int {
+  kFusedPlain = 0,        // one problem, or `problems` of equal size at constant strides
+  kFusedRaggedCols = 1,   // group g owns the columns [offsets[g], offsets[g + 1]) of C and of op(B), and its own op(A)
+  kFusedRaggedInner = 2,  // group g sums over the inner indices [offsets[g], offsets[g + 1]) and has its own C
+};
+
+// Most groups of a call: the table of the groups' tiles lives in shared memory.
+constexpr int kFusedMaxGroups = 1024;
+
+// Kernel arguments. C is m x n with m contiguous: rows are the features of a caller's contiguous vectors, columns the
+// vectors (tokens).
+struct FusedParams {
+  unsigned int* status;
+  int m, n, k;                // kFusedRaggedCols: n is the bound on the offsets; kFusedRaggedInner: k is
+  int kind, problems;
+  const long long* offsets;   // problems + 1 entries in device memory (ragged kinds)
+  int tiles_m, tiles_n;       // per problem (tiles_n unused for kFusedRaggedCols)
+  int raster;                 // tile rows walked together
+  int tri;                    // C is symmetric: tiles on and below the diagonal are computed, the others mirrored
+  int a_mn, b_mn;             // operand is contiguous along m / n (else along k)
+  unsigned int idesc;
+  int a_batched, b_batched;
+  int stages;                 // depth of the operand ring
+  int split;                  // CTAs of a cluster that share one tile's inner extent (kernels of one CTA per tile)
+  float alpha, beta;
+  const void* bias;           // one value per row of C, or null
+  long long bias_stride;      // between problems
+  int act, grad;              // grad: C = (alpha AB + beta D) * slope(Z); else Z = alpha AB + bias, C = act(Z) + beta D
+  void* c;
+  const void* d;              // null without residual
+  void* z;                    // written (grad == 0) or read; null without
+  long long ldc, ldd, ldz, c_stride, d_stride, z_stride;
+  int tma;                    // C, D and Z travel by TMA
+  float* partial;             // row sums of C per column tile (bias gradient), or null
+  int hint_a, hint_b;
+};
+
+// Sizes of one kernel variant as the selection sees it.
+struct FusedVariant {
+  int ctas;           // CTAs per tile: 2 for the pair kernel
+  int bn;             // columns per tile; rows are 128 * ctas
+  int stage_bytes;
+  int epi_groups;     // epilogue groups of four warps
+};
+constexpr int kFusedVariants = 5;
+constexpr FusedVariant kFusedTable[kFusedVariants] = {
+    {2, 256, 32768, 2}, {1, 256, 49152, 2}, {1, 128, 32768, 2}, {1, 64, 24576, 1}, {1, 32, 20480, 1}};
+
+// Enqueues variant `v` with operand type / D type / C type. `grid` counts CTAs, `smem` bytes of dynamic shared memory.
+cudaError_t launch_fused_variant(int v, int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p,
+                                 int grid, int smem, cudaStream_t stream);
+// Clusters of `cluster` (1, 2, 4 or 8) CTAs with nearly all of an SM's shared memory each that the current device
+// holds at once.
+int fused_resident_clusters(int cluster);
+cudaError_t launch_fused_pair(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,
+                              int smem, cudaStream_t stream);
+cudaError_t launch_fused_256(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,
+                             int smem, cudaStream_t stream);
+cudaError_t launch_fused_128(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,
+                             int smem, cudaStream_t stream);
+cudaError_t launch_fused_64(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,
+                            int smem, cudaStream_t stream);
+cudaError_t launch_fused_32(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,
+                            int smem, cudaStream_t stream);
+
+}  // namespace b200

@@ -146,13 +146,102 @@ int b200blas_col2im(int dtype, int kernel_mode, size_t channels, size_t height, 
                     size_t dilation_w, const void* col, size_t col_offset, void* im, size_t im_offset, void* stream,
                     int async);
 
+/* ---- products around a transformer block (no counterpart in the reference) ---------------------------------------
+ * Matrix products whose epilogue adds a bias, applies an activation and adds a residual, products grouped by expert
+ * over ragged groups of rows, the backward forms of both, and the orthogonalisation of an update.
+ *   - `dtype` is 16 (half) or B200BLAS_BFLOAT16; where said also 32. `c_dtype` is `dtype` or, for 16-bit operands, 32:
+ *     the type of C and of the residual D. Every other matrix and vector has `dtype`. Other precisions of the library
+ *     return kNotImplemented.
+ *   - scalars are passed by value in double precision. Sums run in fp32; a stored value is rounded once.
+ *   - `activation`: 161 identity, 162 relu, 163 gelu (z times the normal distribution function), 164 gelu in its tanh
+ *     form, 165 silu. act' below is its derivative.
+ *   - optional buffers are absent when NULL; D is not read when beta == 0, Z is not read when the activation is the
+ *     identity. D may be C itself, a Z that is read may be C too; any other overlap with C is refused
+ *     (kInvalidMatrixC). C must not overlap A or B.
+ *   - Z and D have C's extents and are reported with C's status codes; a bad bias is kInvalidVectorX (-1019) or
+ *     kInsufficientMemoryX (-1008), a bad bias gradient kInvalidVectorY (-1018) or kInsufficientMemoryY (-1007).
+ *     Extents above 2^31 - 4097 are kInvalidDimension. Buffers that do not lie on the current device are invalid.
+ *   - any alignment, leading dimension and offset is served. Operands whose base, leading dimension or stride is not a
+ *     multiple of 16 bytes are first copied to scratch; outputs that are not are written with narrow stores.
+ *   - scratch (those copies, partial bias gradients, Newton-Schulz intermediates) comes from a stream-ordered pool of
+ *     the library that keeps up to 1 GB per device until b200blas_clear_cache; a captured call owns its scratch through
+ *     its graph. Results do not depend on timing: no atomics are used. */
+#define B200BLAS_BFLOAT16 1016
+#define B200BLAS_MAX_GROUPS 1024
+
+/* Z = alpha * op(A) * op(B) + bias, C = act(Z) + beta * D. `bias` has one entry per element of C's unit-stride extent
+ * (n for row-major, m for column-major layouts). Z, when given, is stored for the backward pass. dtype 16, bf16, 32. */
+int b200blas_gemm_epilogue(int dtype, int c_dtype, int layout, int a_transpose, int b_transpose, size_t m, size_t n,
+                           size_t k, double alpha, const void* a, size_t a_offset, size_t a_ld, const void* b,
+                           size_t b_offset, size_t b_ld, const void* bias, size_t bias_offset, int activation, void* z,
+                           size_t z_offset, size_t z_ld, double beta, const void* d, size_t d_offset, size_t d_ld,
+                           void* c, size_t c_offset, size_t c_ld, void* stream, int async);
+
+/* C = (alpha * op(A) * op(B) + beta * D) * act'(Z): the gradient in front of an activation whose input was Z.
+ * `bias_grad`, when given, receives the sums of C over the extent that is not unit-stride. dtype 16, bf16, 32. */
+int b200blas_gemm_epilogue_grad(int dtype, int layout, int a_transpose, int b_transpose, size_t m, size_t n, size_t k,
+                                double alpha, const void* a, size_t a_offset, size_t a_ld, const void* b,
+                                size_t b_offset, size_t b_ld, double beta, const void* d, size_t d_offset, size_t d_ld,
+                                int activation, const void* z, size_t z_offset, size_t z_ld, void* c, size_t c_offset,
+                                size_t c_ld, void* bias_grad, size_t bias_grad_offset, void* stream, int async);
+
+/* DZ = DY * act'(Z) for `rows` contiguous vectors of n elements, and the sums of DZ over the rows: the same for a
+ * gradient that no product of this library produced. DZ or bias_grad may be absent; DZ may be DY or Z. With `groups`
+ * > 0 there is one bias gradient per group (lines of bias_grad_ld elements) and only the rows of groups are touched
+ * (see b200blas_gemm_grouped); group_offsets is NULL exactly when groups == 0. dtype 16, bf16, 32. */
+int b200blas_activation_grad(int dtype, size_t rows, size_t n, int activation, const void* dy, size_t dy_offset,
+                             size_t dy_ld, const void* z, size_t z_offset, size_t z_ld, void* dz, size_t dz_offset,
+                             size_t dz_ld, void* bias_grad, size_t bias_grad_offset, size_t groups,
+                             const long long* group_offsets, size_t bias_grad_ld, void* stream, int async);
+
+/* Row i of group g: C_i = act(alpha * X_i * op(W_g) + bias_g) + beta * D_i. Rows are contiguous vectors (X: k elements,
+ * C, D, Z: n); group g owns the rows [group_offsets[g], group_offsets[g + 1]). `group_offsets` is a DEVICE array of
+ * groups + 1 ascending 64-bit row numbers up to `rows`, read when the work runs; offsets outside [0, rows] are clamped
+ * and descending ones leave their group empty. Rows of no group are neither read for a result nor written. op(W_g) is
+ * k x n: W_g has k rows of n elements (111) or n rows of k elements (112), w_stride elements apart. `bias`: groups
+ * lines of bias_ld elements. groups may not exceed B200BLAS_MAX_GROUPS (kInvalidBatchCount). dtype 16, bf16. */
+int b200blas_gemm_grouped(int dtype, int c_dtype, int w_transpose, size_t groups, size_t rows, size_t n, size_t k,
+                          double alpha, const void* x, size_t x_offset, size_t x_ld, const void* w, size_t w_offset,
+                          size_t w_ld, size_t w_stride, const long long* group_offsets, const void* bias,
+                          size_t bias_offset, size_t bias_ld, int activation, void* z, size_t z_offset, size_t z_ld,
+                          double beta, const void* d, size_t d_offset, size_t d_ld, void* c, size_t c_offset,
+                          size_t c_ld, void* stream, int async);
+
+/* C_i = (alpha * X_i * op(W_g) + beta * D_i) * act'(Z_i), bias_grad_g = the sum of C_i over the group's rows (zero for
+ * an empty group). dtype 16, bf16. */
+int b200blas_gemm_grouped_grad(int dtype, int w_transpose, size_t groups, size_t rows, size_t n, size_t k, double alpha,
+                               const void* x, size_t x_offset, size_t x_ld, const void* w, size_t w_offset, size_t w_ld,
+                               size_t w_stride, const long long* group_offsets, double beta, const void* d,
+                               size_t d_offset, size_t d_ld, int activation, const void* z, size_t z_offset, size_t z_ld,
+                               void* c, size_t c_offset, size_t c_ld, void* bias_grad, size_t bias_grad_offset,
+                               size_t bias_grad_ld, void* stream, int async);
+
+/* C_g = alpha * X_g^T * Y_g + beta * C_g, m x n with n contiguous, over the rows of group g (X: m elements, Y: n); an
+ * empty group gets beta * C_g. The weight gradient of the grouped product. c_stride must keep the groups' results
+ * apart (kInvalidDimension). dtype 16, bf16. */
+int b200blas_gemm_grouped_weight(int dtype, int c_dtype, size_t groups, size_t rows, size_t m, size_t n, double alpha,
+                                 const void* x, size_t x_offset, size_t x_ld, const void* y, size_t y_offset, size_t y_ld,
+                                 const long long* group_offsets, double beta, void* c, size_t c_offset, size_t c_ld,
+                                 size_t c_stride, void* stream, int async);
+
+/* Orthogonalises batch_count m x n matrices by Newton-Schulz products: X = A / (|A|_F + epsilon), then `steps` times
+ * X <- a X + (b G + c G G) X with G = X X^T (on the shorter side), B = alpha * X. `coefficients` (HOST) holds one triple
+ * (a, b, c) for all steps, or, with coefficient_count >= steps, one per step. B may be A. 16-bit types keep X, G and the
+ * bracket in half precision between the products; 32 runs on the single-precision kernels throughout.
+ * dtype 16, bf16, 32. steps 1 to 1000, at most 65535 matrices. */
+int b200blas_newton_schulz(int dtype, int layout, size_t m, size_t n, double alpha, const void* a, size_t a_offset,
+                           size_t a_ld, size_t a_stride, void* b, size_t b_offset, size_t b_ld, size_t b_stride,
+                           size_t batch_count, size_t steps, const double* coefficients, size_t coefficient_count,
+                           double epsilon, void* stream, int async);
+
 /* Replaces clblast::GemmTempBufferSize<T> (include/clblast_cuda.h:523-527, src/clblast_cuda.cpp:1818-1843).
  * Validates the dimensions and writes 0: no kernel of this library needs caller scratch. */
 int b200blas_gemm_temp_buffer_size(int dtype, int layout, int a_transpose, int b_transpose, size_t m, size_t n,
                                    size_t k, size_t a_offset, size_t a_ld, size_t b_offset, size_t b_ld,
                                    size_t c_offset, size_t c_ld, size_t* temp_buffer_size);
 
-/* Replace clblast::ClearCache / FillCache (include/clblast_cuda.h:533-537, src/api_common.cpp:25-33,120-135). */
+/* Replace clblast::ClearCache / FillCache (include/clblast_cuda.h:533-537, src/api_common.cpp:25-33,120-135).
+ * ClearCache also gives back the scratch memory that the products around a transformer block keep. */
 int b200blas_clear_cache(void);
 int b200blas_fill_cache(int device);
 
