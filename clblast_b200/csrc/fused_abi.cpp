@@ -504,10 +504,11 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
                                long long a_stride, void* b, long long b_ld, long long b_stride, long long batch, int steps,
                                const double* coefficients, bool per_step, double eps, cudaStream_t s, const char** name) {
   const bool gram_of_lines = one > two;  // the shorter side is the number of lines
-  const long long side = gram_of_lines ? two : one;
-  const long long pitch = (one + 7) / 8 * 8, gram_pitch = (side + 7) / 8 * 8;
+  // extents inside are multiples of 8, the rest zero: the symmetric products store 16 bytes at a time
+  const long long pitch = (one + 7) / 8 * 8, lines = (two + 7) / 8 * 8;
+  const long long side = gram_of_lines ? lines : pitch, gram_pitch = side;
   const auto round = [](size_t x) { return (x + 255) / 256 * 256; };
-  const size_t x_bytes = round(static_cast<size_t>(batch) * two * pitch * 2);
+  const size_t x_bytes = round(static_cast<size_t>(batch) * lines * pitch * 2);
   const size_t g_bytes = round(static_cast<size_t>(batch) * side * gram_pitch * 2);
   const size_t s_bytes = round(static_cast<size_t>(batch) * kNormBlocks * sizeof(double));
   PoolScratch scratch;
@@ -523,7 +524,7 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
   const double scale0 = std::ldexp(1.0, shift);
   NormaliseJob norm = {};
   norm.type = dtype; norm.x_type = 16; norm.g = a; norm.one = one; norm.two = two; norm.ld = a_ld; norm.stride = a_stride;
-  norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.eps = eps; norm.scale = scale0;
+  norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.lines = lines; norm.eps = eps; norm.scale = scale0;
   norm.sums = reinterpret_cast<double*>(base + 2 * x_bytes + 2 * g_bytes);
   e = launch_normalise(norm, s);
   for (int i = 0; i < steps && e == cudaSuccess; ++i) {
@@ -535,8 +536,8 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
     f.type = f.c_type = f.d_type = 16;
     f.kind = kFusedPlain; f.problems = batch; f.act = kActIdentityCode;
     // A = X X^T
-    f.m = f.n = side; f.k = gram_of_lines ? one : two;
-    f.a = f.b = from; f.lda = f.ldb = pitch; f.a_stride = f.b_stride = two * pitch;
+    f.m = f.n = side; f.k = gram_of_lines ? pitch : lines;
+    f.a = f.b = from; f.lda = f.ldb = pitch; f.a_stride = f.b_stride = lines * pitch;
     f.a_mn = f.b_mn = gram_of_lines ? 0 : 1;
     f.alpha = undo * undo; f.tri = 1;
     f.c = gram; f.ldc = gram_pitch; f.c_stride = side * gram_pitch;
@@ -553,19 +554,19 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
     // a X + (.) X, on the last step straight into the caller's matrix
     const double out = undo * (last ? alpha : 1.0);
     f.tri = 0;
-    f.m = one; f.n = two; f.k = side;
+    f.m = last ? one : pitch; f.n = last ? two : lines; f.k = side;
     if (gram_of_lines) {
-      f.a = from; f.lda = pitch; f.a_stride = two * pitch; f.a_mn = 1;
+      f.a = from; f.lda = pitch; f.a_stride = lines * pitch; f.a_mn = 1;
       f.b = poly; f.ldb = gram_pitch; f.b_stride = side * gram_pitch; f.b_mn = 0;
     } else {
       f.a = poly; f.lda = gram_pitch; f.a_stride = side * gram_pitch; f.a_mn = 0;
-      f.b = from; f.ldb = pitch; f.b_stride = two * pitch; f.b_mn = 0;
+      f.b = from; f.ldb = pitch; f.b_stride = lines * pitch; f.b_mn = 0;
     }
-    f.alpha = out; f.beta = q[0] * out; f.d = from; f.ldd = pitch; f.d_stride = two * pitch;
+    f.alpha = out; f.beta = q[0] * out; f.d = from; f.ldd = pitch; f.d_stride = lines * pitch;
     if (last) {
       f.c_type = dtype; f.c = b; f.ldc = b_ld; f.c_stride = b_stride;
     } else {
-      f.c = x[(i + 1) & 1]; f.ldc = pitch; f.c_stride = two * pitch;
+      f.c = x[(i + 1) & 1]; f.ldc = pitch; f.c_stride = lines * pitch;
     }
     e = launch_fused(f, s, name);
   }
@@ -592,7 +593,7 @@ cudaError_t newton_schulz_single(long long one, long long two, double alpha, con
   void* const poly = base + 2 * x_bytes + g_bytes;
   NormaliseJob norm = {};
   norm.type = 32; norm.x_type = 32; norm.g = a; norm.one = one; norm.two = two; norm.ld = a_ld; norm.stride = a_stride;
-  norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.eps = eps; norm.scale = 1.0;
+  norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.lines = two; norm.eps = eps; norm.scale = 1.0;
   norm.sums = reinterpret_cast<double*>(base + 2 * x_bytes + 2 * g_bytes);
   e = launch_normalise(norm, s);
   for (int i = 0; i < steps && e == cudaSuccess; ++i) {

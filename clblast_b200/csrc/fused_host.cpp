@@ -19,28 +19,27 @@ namespace b200 {
 namespace {
 
 constexpr int kMaxSmem = 232448;  // 227 KB
-constexpr int kBarBytes = 512, kSlot = 4096, kRing = 4, kAlign = 1024;
+constexpr int kAlign = 1024;
 
 int elem_size(int type) { return type == 32 ? 4 : 2; }
 
-// Tensor map of an epilogue matrix (m contiguous): boxes of 128 rows and 32 bytes' worth of columns, no swizzle.
-bool encode_block_map(CUtensorMap* map, int type, int cols, const void* base, long long m, long long n, long long ld,
-                      long long planes, long long stride) {
+bool aligned16(const void* base, long long ld, long long planes, long long stride, int elem) {
+  return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && (ld * elem) % 16 == 0 && (planes <= 1 || (stride * elem) % 16 == 0);
+}
+
+// Tensor map of an epilogue matrix (m contiguous), used to bring tiles of 128 rows x 32 columns into L2.
+bool encode_prefetch_map(CUtensorMap* map, int elem, const void* base, long long m, long long n, long long ld, long long planes,
+                         long long stride) {
   const DriverApi& drv = driver_api();
-  if (!drv.ok || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
-  const long long elem = elem_size(type);
-  const cuuint64_t row_bytes = static_cast<cuuint64_t>(ld * elem);
-  const cuuint64_t plane_bytes = planes > 1 ? static_cast<cuuint64_t>(stride * elem) : row_bytes;
-  if ((row_bytes & 15) || (plane_bytes & 15) || row_bytes >= (1ULL << 40) || plane_bytes >= (1ULL << 40)) return false;
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(m), static_cast<cuuint64_t>(n),
-                              static_cast<cuuint64_t>(planes > 1 ? planes : 1)};
-  const cuuint64_t strides[2] = {row_bytes, plane_bytes};
-  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(cols), 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
+  if (!drv.ok) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(m), static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(planes > 1 ? planes : 1)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * elem), static_cast<cuuint64_t>((planes > 1 ? stride : ld) * elem)};
+  if (strides[0] >= (1ULL << 40) || strides[1] >= (1ULL << 40)) return false;
+  const cuuint32_t box[3] = {128, 32, 1}, estr[3] = {1, 1, 1};
   const CUtensorMapDataType dt = elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  return drv.TensorMapEncodeTiled(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
-                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return drv.TensorMapEncodeTiled(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 struct Choice {
@@ -48,7 +47,7 @@ struct Choice {
 };
 
 constexpr const char* kNames[kFusedVariants] = {"fused_pair_256x256x64", "fused_128x256x64", "fused_128x128x64",
-                                                "fused_128x64x64", "fused_128x32x64"};
+                                                "fused_128x64x64", "fused_128x32x64", "fused_pair_256x128x64"};
 
 // Upper bound of the column tiles of a call (exact for the plain kinds).
 long long column_tiles(const FusedDesc& d, int bn) {
@@ -58,9 +57,10 @@ long long column_tiles(const FusedDesc& d, int bn) {
 
 bool variant_fits(const FusedDesc& d, int v, int split) {
   const FusedVariant& t = kFusedTable[v];
-  if (t.ctas == 2 && (d.kind == kFusedRaggedInner || split > 1)) return false;  // its peer cannot clear the inner tail
+  if (t.ctas == 2 && split > 1) return false;
   if (d.b_mn && t.bn / t.ctas < 64) return false;                               // a 128-byte row is 64 columns
-  if (d.tri && !(t.ctas * 128 == t.bn)) return false;                           // square tiles meet their mirror image
+  if (d.c_type == 32 && t.bn > 128) return false;                               // the epilogue's sums fill the registers
+  if (d.tri && t.ctas * 128 != t.bn) return false;                               // square tiles meet their mirror image
   if (split > 1 && (t.bn / split) % 4 != 0) return false;
   if (split > 1 && d.tri) return false;
   return true;
@@ -91,7 +91,7 @@ double estimate(const FusedDesc& d, int v, int split) {
   double tiles = tm * tn * problems;
   if (d.tri) tiles = tm * (tm + 1) / 2 * problems;
   const double blocks = static_cast<double>(static_cast<long long>((k + 63) / 64));
-  const double per_block_mma = t.ctas == 2 ? 530.0 : (t.bn == 256 ? 530.0 : (t.bn == 128 ? 270.0 : (t.bn == 64 ? 150.0 : 110.0)));
+  const double per_block_mma = t.ctas == 2 ? (t.bn == 256 ? 530.0 : 270.0) : (t.bn == 256 ? 530.0 : (t.bn == 128 ? 270.0 : (t.bn == 64 ? 150.0 : 110.0)));
   const double per_block_load = t.stage_bytes / 60.0;
   const double per_block = per_block_mma > per_block_load ? per_block_mma : per_block_load;
   const double teams = static_cast<double>(resident_teams(t.ctas * split));
@@ -194,26 +194,29 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   p.z = d.z; p.ldz = d.ldz; p.z_stride = d.z_stride;
   p.hint_a = p.hint_b = 2;
 
-  CUtensorMap maps[5];
-  std::memset(maps, 0, sizeof(maps));
+  CUtensorMap maps[4];
+  std::memset(maps + 2, 0, 2 * sizeof(CUtensorMap));
   if (!encode_operand_map(&maps[0], 2, r.a, d.m, d.k, r.lda, d.a_mn != 0, 128, a_planes, r.a_stride) ||
       !encode_operand_map(&maps[1], 2, r.b, d.n, d.k, r.ldb, d.b_mn != 0, t.bn / t.ctas, b_planes, r.b_stride))
     return cudaErrorInvalidValue;
-  const int cols = 32 / elem_size(d.c_type);
   const long long c_planes = d.kind == kFusedRaggedCols ? 1 : d.problems;
-  // Columns of a group are cut off by 16-byte copies: m has to be a multiple of 16 bytes there.
-  bool tma = d.kind != kFusedRaggedCols || d.m % 8 == 0;
-  tma = tma && encode_block_map(&maps[2], d.c_type, cols, d.c, d.m, d.n, d.ldc, c_planes, d.c_stride);
-  if (tma && p.d) tma = encode_block_map(&maps[3], d.d_type, cols, p.d, d.m, d.n, d.ldd, c_planes, d.d_stride);
-  if (tma && p.z) tma = encode_block_map(&maps[4], d.type, cols, p.z, d.m, d.n, d.ldz, c_planes, d.z_stride);
-  p.tma = tma ? 1 : 0;
+  p.vec = d.m % 8 == 0 && aligned16(d.c, d.ldc, c_planes, d.c_stride, elem_size(d.c_type)) &&
+          (!p.d || aligned16(p.d, d.ldd, c_planes, d.d_stride, elem_size(d.d_type))) &&
+          (!p.z || aligned16(p.z, d.ldz, c_planes, d.z_stride, 2));
+
+  const bool reads_z = p.z && d.grad;
+  if (p.vec && choice.split == 1 && (p.d || reads_z))
+    p.prefetch = (!p.d || encode_prefetch_map(&maps[2], elem_size(d.d_type), p.d, d.m, d.n, d.ldd, c_planes, d.d_stride)) &&
+                 (!reads_z || encode_prefetch_map(&maps[3], 2, p.z, d.m, d.n, d.ldz, c_planes, d.z_stride));
+  if (d.tri && (!p.vec || p.z || d.n != d.m)) return cudaErrorInvalidValue;  // mirrored with 16-byte stores only
 
   const long long col_tiles = column_tiles(d, t.bn);
   long long tiles = col_tiles * p.tiles_m;
   if (d.kind != kFusedRaggedCols) tiles *= d.problems;
   if (d.tri) tiles = static_cast<long long>(p.tiles_m) * (p.tiles_m + 1) / 2 * d.problems;
   if (tiles > 0x3FFFFFFF) return cudaErrorInvalidValue;
-  const int lines_per_tile = t.epi_groups * choice.split;
+  const bool single = d.c_type == 32;
+  const int lines_per_tile = fused_groups(t.bn) * choice.split;
   if (d.bias_grad != nullptr) {
     e = partial.get(static_cast<size_t>(col_tiles) * lines_per_tile * d.m * sizeof(float), stream);
     if (e != cudaSuccess) return e;
@@ -221,10 +224,8 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   }
 
   // shared memory: the ring takes what staging, barriers and the group table leave
-  const int staging = t.epi_groups * kRing * kSlot * (p.z ? 2 : 1);
-  const int sums = choice.split > 1 ? t.bn * 128 * 4 : 0;
   const int table = d.kind == kFusedRaggedCols ? 8 * (p.problems + 1) : 0;
-  const int fixed = kAlign + (staging > sums ? staging : sums) + kBarBytes + table;
+  const int fixed = kAlign + fused_staging_bytes(t.bn, single, p.z != nullptr, choice.split) + kFusedBarBytes + table;
   int stages = (kMaxSmem - fixed) / t.stage_bytes;
   if (stages > 12) stages = 12;
   if (stages < 2) return cudaErrorInvalidValue;
@@ -264,6 +265,7 @@ cudaError_t launch_fused_variant(int v, int type, int d_type, int c_type, const 
     case 1: return launch_fused_256(type, d_type, c_type, maps, p, grid, smem, stream);
     case 2: return launch_fused_128(type, d_type, c_type, maps, p, grid, smem, stream);
     case 3: return launch_fused_64(type, d_type, c_type, maps, p, grid, smem, stream);
+    case 5: return launch_fused_pair128(type, d_type, c_type, maps, p, grid, smem, stream);
     case 4: return launch_fused_32(type, d_type, c_type, maps, p, grid, smem, stream);
     default: return cudaErrorInvalidValue;
   }

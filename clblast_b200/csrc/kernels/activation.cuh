@@ -17,57 +17,110 @@ namespace b200 {
 
 enum Act : int { kActIdentity = 161, kActRelu = 162, kActGelu = 163, kActGeluTanh = 164, kActSilu = 165 };
 
+// FAST: for results in 16 bits. The hardware's base-2 exponential and reciprocal, a relative error of about 2^-21 in all,
+// far below the 2^-12 of half a step of half precision; without it the full-precision functions, for results in single
+// precision. A gelu in the epilogue of 8192 x 8192 x 512 costs 195 us more than the identity with erfcf.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+
 // s(x) = 1 / (1 + exp(-x)) and, for slopes, 1 - s(x) = exp(-x) s(x), which the subtraction would leave with an absolute
-// error of s's last place. FAST: the hardware exponential and reciprocal, a relative error of about 2^-21, far below the
-// 2^-11 of a half result; without it the full-precision functions, for results in single precision. x is held above
-// -80, so that the exponential stays finite (a NaN passes).
+// error of s's last place. x is held above -80, so that the exponential stays finite (a NaN passes).
 template <bool FAST>
 __device__ __forceinline__ float logistic(float x, float* complement = nullptr) {
   const float xc = x < -80.f ? -80.f : x;
-  const float e = FAST ? __expf(-xc) : expf(-xc);
-  const float s = FAST ? __fdividef(1.f, 1.f + e) : 1.f / (1.f + e);
+  const float e = FAST ? exp2_fast(-kLog2E * xc) : expf(-xc);
+  const float s = FAST ? rcp_fast(1.f + e) : 1.f / (1.f + e);
   if (complement) *complement = e * s;
   return s;
 }
 
+// P(z), the normal distribution function, and exp(-z^2 / 2). With t = 1 / (1 + q |z|) the tail P(-|z|) is
+// exp(-z^2 / 2) t c(t); c is a polynomial of degree six fitted here to the smallest relative error over |z| < 13.4 (6.4e-7;
+// beyond, the exponential has left the range), so that a vanishing P keeps its relative precision.
 template <bool FAST>
-__device__ __forceinline__ float gelu_tanh_arg(float z) {  // 2u
-  constexpr float k2 = 1.5957691216057308f;  // 2 sqrt(2/pi)
-  return k2 * z * (1.f + 0.044715f * z * z);
+__device__ __forceinline__ float normal_cdf(float z, float* bell = nullptr) {
+  if (FAST) {
+    const float e = exp2_fast(z * z * (-0.5f * kLog2E));
+    const float t = rcp_fast(fmaf(0.26516504294495533f, fabsf(z), 1.f));
+    float c = -0.06754792165618550f;
+    c = fmaf(c, t, 0.19396880130252385f);
+    c = fmaf(c, t, -0.06479847023409181f);
+    c = fmaf(c, t, 0.14153061996590430f);
+    c = fmaf(c, t, 0.08333235214270828f);
+    c = fmaf(c, t, 0.10784457380456717f);
+    c = fmaf(c, t, 0.10566972585255615f);
+    const float tail = e * (t * c);
+    if (bell) *bell = e;
+    return z < 0.f ? tail : 1.f - tail;
+  }
+  if (bell) *bell = expf(-0.5f * z * z);
+  return 0.5f * erfcf(z * -0.70710678118654752f);
 }
 
-template <bool FAST>
-__device__ __forceinline__ float act_value(int act, float z) {
-  switch (act) {
+__device__ __forceinline__ float gelu_tanh_arg(float z) {  // 2u
+  constexpr float k2 = 1.5957691216057308f;  // 2 sqrt(2/pi)
+  return k2 * z * fmaf(0.044715f * z, z, 1.f);
+}
+
+template <bool FAST, int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  switch (ACT) {
     case kActRelu: return z < 0.f ? 0.f : z;
-    case kActGelu: return fmaxf(z, -60.f) * (0.5f * erfcf(z * -0.70710678118654752f));
-    case kActGeluTanh: return fmaxf(z, -60.f) * logistic<FAST>(gelu_tanh_arg<FAST>(z));
+    case kActGelu: return fmaxf(z, -60.f) * normal_cdf<FAST>(z);
+    case kActGeluTanh: return fmaxf(z, -60.f) * logistic<FAST>(gelu_tanh_arg(z));
     case kActSilu: return fmaxf(z, -80.f) * logistic<FAST>(z);
     default: return z;
   }
 }
 
-template <bool FAST>
-__device__ __forceinline__ float act_slope(int act, float z) {
+template <bool FAST, int ACT>
+__device__ __forceinline__ float act_slope(float z) {
   const float zc = fminf(fmaxf(z, -60.f), 60.f);
-  switch (act) {
+  switch (ACT) {
     case kActRelu: return z > 0.f ? 1.f : (z != z ? z : 0.f);
     case kActGelu: {
-      const float e = FAST ? __expf(-0.5f * zc * zc) : expf(-0.5f * zc * zc);
-      return 0.5f * erfcf(z * -0.70710678118654752f) + zc * (0.3989422804014327f * e);
+      float e;
+      const float cdf = normal_cdf<FAST>(z, &e);
+      return fmaf(zc * 0.3989422804014327f, e, cdf);
     }
     case kActGeluTanh: {
       float rest;
-      const float s = logistic<FAST>(gelu_tanh_arg<FAST>(z), &rest);
+      const float s = logistic<FAST>(gelu_tanh_arg(z), &rest);
       constexpr float k2 = 1.5957691216057308f;
-      return s + zc * s * rest * k2 * (1.f + 3.f * 0.044715f * zc * zc);
+      return fmaf(zc * s * rest, fmaf(k2 * 3.f * 0.044715f * zc, zc, k2), s);
     }
     case kActSilu: {
       float rest;
       const float s = logistic<FAST>(z, &rest);
-      return s * (1.f + fminf(fmaxf(z, -80.f), 200.f) * rest);
+      return s * fmaf(fminf(fmaxf(z, -80.f), 200.f), rest, 1.f);
     }
     default: return 1.f;
+  }
+}
+
+// Calls f with the activation as a compile-time constant. The choice is made once per block of values: taken per value
+// it keeps the compiler from interleaving the values' chains (8192 x 8192 x 512 with relu: 299 us against 110 without).
+template <int ACT>
+struct ActTag {
+  static constexpr int value = ACT;
+};
+template <class F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  switch (act) {
+    case kActRelu: f(ActTag<kActRelu>()); break;
+    case kActGelu: f(ActTag<kActGelu>()); break;
+    case kActGeluTanh: f(ActTag<kActGeluTanh>()); break;
+    case kActSilu: f(ActTag<kActSilu>()); break;
+    default: f(ActTag<kActIdentity>());
   }
 }
 

@@ -88,20 +88,22 @@ __global__ void __launch_bounds__(kPwLanes * kPwRows) pointwise_kernel(const Poi
       P d = {}, z = {}, c;
       if (job.d != nullptr) d = *reinterpret_cast<const P*>(static_cast<const T*>(job.d) + t * job.ldd + f0);
       if (job.grad && job.z != nullptr) z = *reinterpret_cast<const P*>(static_cast<const T*>(job.z) + t * job.ldz + f0);
+      with_act(job.grad && job.z == nullptr ? static_cast<int>(kActIdentity) : job.act, [&](auto tag) {
+        constexpr int ACT = decltype(tag)::value;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float add = job.d != nullptr ? job.beta * to_float(d.v[j]) : 0.f;
-        float y = to_float(p.v[j]) + bias[j];
-        if (job.grad) {
-          y += add;
-          if (job.z != nullptr) y *= act_slope<FAST>(job.act, to_float(z.v[j]));
-          total[j] += y;
-        } else {
-          z.v[j] = from_float<T>(y);
-          y = act_value<FAST>(job.act, y) + add;
+        for (int j = 0; j < VEC; ++j) {
+          const float add = job.d != nullptr ? job.beta * to_float(d.v[j]) : 0.f;
+          float y = to_float(p.v[j]) + bias[j];
+          if (job.grad) {
+            y = (y + add) * act_slope<FAST, ACT>(to_float(z.v[j]));
+            total[j] += y;
+          } else {
+            z.v[j] = from_float<T>(y);
+            y = act_value<FAST, ACT>(y) + add;
+          }
+          c.v[j] = from_float<T>(y);
         }
-        c.v[j] = from_float<T>(y);
-      }
+      });
       if (!job.grad && job.z != nullptr) *reinterpret_cast<P*>(static_cast<T*>(job.z) + t * job.ldz + f0) = z;
       if (job.c != nullptr) *reinterpret_cast<P*>(static_cast<T*>(job.c) + t * job.ldc + f0) = c;
     }
@@ -195,12 +197,12 @@ __global__ void __launch_bounds__(256) scale_kernel(const NormaliseJob job, int 
   __syncthreads();
   const double f = factor;
   const T* const g = static_cast<const T*>(job.g) + static_cast<long long>(blockIdx.y) * job.stride;
-  X* const x = static_cast<X*>(job.x) + static_cast<long long>(blockIdx.y) * job.two * job.pitch;
-  for (long long line = blockIdx.x; line < job.two; line += gridDim.x) {
+  X* const x = static_cast<X*>(job.x) + static_cast<long long>(blockIdx.y) * job.lines * job.pitch;
+  for (long long line = blockIdx.x; line < job.lines; line += gridDim.x) {
     const T* const row = g + line * job.ld;
 #pragma unroll 4
     for (long long i = threadIdx.x; i < job.pitch; i += 256)
-      x[line * job.pitch + i] = from_float<X>(i < job.one ? static_cast<float>(static_cast<double>(to_float(row[i])) * f) : 0.f);
+      x[line * job.pitch + i] = from_float<X>(i < job.one && line < job.two ? static_cast<float>(static_cast<double>(to_float(row[i])) * f) : 0.f);
   }
 }
 
@@ -290,7 +292,7 @@ cudaError_t launch_normalise(const NormaliseJob& job, cudaStream_t stream) {
   if (job.batch > 65535) return cudaErrorInvalidValue;
   const int blocks = static_cast<int>(job.two < kNormBlocks ? job.two : kNormBlocks);
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(job.batch));
-  const long long wide = job.two < 4096 ? job.two : 4096;
+  const long long wide = job.lines < 4096 ? job.lines : 4096;
   const dim3 scale_grid(static_cast<unsigned>(wide), static_cast<unsigned>(job.batch));
   return by_type(job.type, [&](auto* tag) {
     using T = typename std::remove_pointer<decltype(tag)>::type;

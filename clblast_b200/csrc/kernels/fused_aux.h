@@ -51,7 +51,7 @@ struct SumJob {
 cudaError_t launch_sum_partials(const SumJob& job, cudaStream_t stream);
 
 // Newton-Schulz input: X = scale * G / (|G|_F + eps) for `batch` matrices (lines of `one` contiguous elements, `two`
-// lines), X dense with line pitch `pitch` (padding zeroed) and planes two * pitch apart, in half (x_type 16) or single
+// lines), X dense with `lines` lines of `pitch` elements (what G does not have is zero), planes lines * pitch apart, in half (x_type 16) or single
 // (32) precision. `sums` is scratch of norm_scratch_doubles(batch) doubles.
 constexpr int kNormBlocks = 256;  // blocks per matrix
 struct NormaliseJob {
@@ -59,7 +59,7 @@ struct NormaliseJob {
   const void* g;
   long long one, two, ld, stride, batch;
   void* x;
-  long long pitch;
+  long long pitch, lines;
   double eps, scale;
   double* sums;
 };

@@ -8,16 +8,23 @@
 // bias gradient a running sum, and a 32-lane store covers consecutive addresses.
 //
 // Warp roles: warp 0 lane 0 issues the TMA loads of the operand ring, warp 1 the MMAs (and clears what a ragged inner
-// extent leaves behind its end), warps 2.. drain the accumulators in groups of four warps, each group its own range
+// extent leaves behind its end), warp 2 builds the group table, warps 4.. drain the accumulators in groups of four warps, each group its own range
 // of the tile's columns. Two accumulators alternate, so a tile is drained under the next one's MMAs.
 //   CTAS == 2: a cluster of two CTAs works on 256 x BN tiles with cta_group::2, each CTA staging half of op(B).
 //   CTAS == 1: tiles of 128 x BN; a cluster of p.split CTAs may share a tile's inner extent. Each CTA then leaves its
 //   fp32 sums in its own shared memory and the CTAs add them up for a range of columns each, in the order of the ranks
 //   (the result does not depend on which CTA came first).
 //
-// The epilogue goes by blocks of 32 bytes of columns x 128 rows (4 KB). D and Z come in and C and Z go out by TMA
-// through rings of four buffers per group; see write_block's counterpart in hgemm_epilogue.cuh for why one named barrier
-// per block orders everything. Columns behind a group's last one are cut off by storing column by column with bulk copies.
+// The epilogue goes by blocks of 16 columns x 32 rows, each warp by itself. A lane holds one row of a block while memory
+// runs along the rows, so blocks are turned round in 1 to 2 KB of the warp's own shared memory and leave as 16-byte
+// stores, four lanes to a column (C in half precision); D and Z come in the same way, two blocks ahead in registers.
+// Columns and rows that end inside a block are cut off lane by lane. (Staging through TMA with a barrier among the warps
+// per block, the form of the half-precision GEMM kernels, took 115 us for 8192 x 8192 x 512 and could not cut a group's
+// columns.)
+//
+// Sums for results in single precision: the tensor cores cut off instead of rounding when they add to an accumulator, an
+// error of about 4e-8 of the result per 16 inner elements that all points towards zero. Results in 16 bits do not see it.
+// For the others an accumulator takes kChunk blocks at most and is then added, rounded, to fp32 registers.
 //
 // All waits are bounded; on expiry a code is left in the status word and every role leaves its loop.
 #pragma once
@@ -41,48 +48,164 @@ using namespace tc;
 
 constexpr int BM = 128;   // rows of op(A) per CTA
 constexpr int BK = 64;    // inner elements per stage: 128-byte swizzle rows
-constexpr int SLOT = 4096;
-constexpr int RING = 4;   // staging buffers per epilogue group and matrix
-constexpr int BAR_BYTES = 512;
+constexpr int kChunk = 4; // operand stages (64 inner elements each) per accumulator for results in single precision
 
-// Shared memory behind the operand ring: staging (or the fp32 sums of a split tile), barriers, group table.
-__host__ __device__ constexpr int staging_bytes(int groups, bool aux) { return groups * RING * SLOT * (aux ? 2 : 1); }
-__host__ __device__ constexpr int sums_bytes(int bn) { return bn * BM * 4; }
-__host__ __device__ inline int table_bytes(int kind, int problems) {
-  return kind == kFusedRaggedCols ? 8 * (problems + 1) : 0;
+// Two values rounded to 16 bits in one word (the packed conversion runs on the full-rate pipe, the single one does not).
+template <class E>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void group_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool group_all(int id, bool mine) {
-  uint32_t out;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %1, 0;\n\t"
-      "bar.red.and.pred p, %2, 128, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(out)
-      : "r"(static_cast<uint32_t>(mine)), "r"(id)
-      : "memory");
-  return out != 0;
-}
+// A block of 32 rows x COLS (16 or 32) columns of a 16-bit matrix between memory and the lanes. In memory order lane l has
+// the rows 8 (l % 4) .. + 7 of the columns 2 (l / 4) and 2 (l / 4) + 1 of each 16; in row order it has row l of all
+// columns. Between the two the block lies in shared memory as [column pair][row] words of two columns.
+template <class E, int COLS>
+struct Block16 {
+  static constexpr int HALVES = COLS / 16;
+  static constexpr int WORDS = COLS * 16;  // shared memory
+  uint4 v[2 * HALVES];
 
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
-  static_assert(N == 8 || N == 16, "block width");
-  if constexpr (N == 16) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-  } else {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(taddr)
-                 : "memory");
+  // base: the block's first element; rows_left (a multiple of 8) and cols_left: how many of its rows and columns exist.
+  __device__ __forceinline__ void load(const E* base, long long ld, int rows_left, int cols_left, int lane) {
+    const int c0 = 2 * (lane >> 2), r0 = 8 * (lane & 3);
+    const bool in = r0 < rows_left;
+    const E* at = base + static_cast<long long>(c0) * ld + r0;
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h, at += 16 * ld) {
+      v[2 * h] = v[2 * h + 1] = make_uint4(0, 0, 0, 0);
+      if (in && c0 + 16 * h < cols_left) v[2 * h] = *reinterpret_cast<const uint4*>(at);
+      if (in && c0 + 16 * h + 1 < cols_left) v[2 * h + 1] = *reinterpret_cast<const uint4*>(at + ld);
+    }
   }
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // memory order -> row order: f[j] is column j of this lane's row. The buffer is free before and after.
+  __device__ __forceinline__ void to_rows(uint32_t* smem, float (&f)[COLS], int lane) const {
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+      const uint4 a = v[2 * h], b = v[2 * h + 1];
+      uint4* const at = reinterpret_cast<uint4*>(smem + h * 256 + (lane >> 2) * 32 + (lane & 3) * 8);
+      at[0] = make_uint4(__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
+                         __byte_perm(a.y, b.y, 0x7632));
+      at[1] = make_uint4(__byte_perm(a.z, b.z, 0x5410), __byte_perm(a.z, b.z, 0x7632), __byte_perm(a.w, b.w, 0x5410),
+                         __byte_perm(a.w, b.w, 0x7632));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < COLS / 2; ++q) {
+      const uint32_t w = smem[q * 32 + lane];
+      const unsigned short lo = static_cast<unsigned short>(w), hi = static_cast<unsigned short>(w >> 16);
+      f[2 * q] = to_float(*reinterpret_cast<const E*>(&lo));
+      f[2 * q + 1] = to_float(*reinterpret_cast<const E*>(&hi));
+    }
+    __syncwarp();
+  }
+  // row order -> memory
+  static __device__ __forceinline__ void store(E* base, long long ld, int rows_left, int cols_left, uint32_t* smem,
+                                               const float (&f)[COLS], int lane) {
+#pragma unroll
+    for (int q = 0; q < COLS / 2; ++q) smem[q * 32 + lane] = pack2<E>(f[2 * q], f[2 * q + 1]);
+    __syncwarp();
+    const int c0 = 2 * (lane >> 2), r0 = 8 * (lane & 3);
+    const bool in = r0 < rows_left;
+    E* at = base + static_cast<long long>(c0) * ld + r0;
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h, at += 16 * ld) {
+      const uint4* const from = reinterpret_cast<const uint4*>(smem + h * 256 + (lane >> 2) * 32 + r0);
+      const uint4 w0 = from[0], w1 = from[1];
+      if (in && c0 + 16 * h < cols_left)
+        *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(w0.x, w0.y, 0x5410), __byte_perm(w0.z, w0.w, 0x5410),
+                                                   __byte_perm(w1.x, w1.y, 0x5410), __byte_perm(w1.z, w1.w, 0x5410));
+      if (in && c0 + 16 * h + 1 < cols_left)
+        *reinterpret_cast<uint4*>(at + ld) = make_uint4(__byte_perm(w0.x, w0.y, 0x7632), __byte_perm(w0.z, w0.w, 0x7632),
+                                                        __byte_perm(w1.x, w1.y, 0x7632), __byte_perm(w1.z, w1.w, 0x7632));
+    }
+    __syncwarp();
+  }
+};
+
+// The same for single precision: in memory order lane l has the rows 4 (l % 8) .. + 3 of the columns l / 8 + 4 h.
+template <int COLS>
+struct Block32 {
+  static constexpr int WORDS = COLS * 32;
+  uint4 v[COLS / 4];
+
+  __device__ __forceinline__ void load(const float* base, long long ld, int rows_left, int cols_left, int lane) {
+    const int r0 = 4 * (lane & 7), c0 = lane >> 3;
+    const float* at = base + static_cast<long long>(c0) * ld + r0;
+#pragma unroll
+    for (int h = 0; h < COLS / 4; ++h, at += 4 * ld) {
+      v[h] = make_uint4(0, 0, 0, 0);
+      if (r0 < rows_left && c0 + 4 * h < cols_left) v[h] = *reinterpret_cast<const uint4*>(at);
+    }
+  }
+  __device__ __forceinline__ void to_rows(uint32_t* smem, float (&f)[COLS], int lane) const {
+#pragma unroll
+    for (int h = 0; h < COLS / 4; ++h) *reinterpret_cast<uint4*>(smem + ((lane >> 3) + 4 * h) * 32 + 4 * (lane & 7)) = v[h];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) f[j] = __uint_as_float(smem[j * 32 + lane]);
+    __syncwarp();
+  }
+  static __device__ __forceinline__ void store(float* base, long long ld, int rows_left, int cols_left, uint32_t* smem,
+                                               const float (&f)[COLS], int lane) {
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) smem[j * 32 + lane] = __float_as_uint(f[j]);
+    __syncwarp();
+    const int r0 = 4 * (lane & 7), c0 = lane >> 3;
+    float* at = base + static_cast<long long>(c0) * ld + r0;
+#pragma unroll
+    for (int h = 0; h < COLS / 4; ++h, at += 4 * ld) {
+      const uint4 w = *reinterpret_cast<const uint4*>(smem + (c0 + 4 * h) * 32 + r0);
+      if (r0 < rows_left && c0 + 4 * h < cols_left) *reinterpret_cast<uint4*>(at) = w;
+    }
+    __syncwarp();
+  }
+};
+template <class E, int COLS>
+struct BlockOf { using type = Block16<E, COLS>; };
+template <int COLS>
+struct BlockOf<float, COLS> { using type = Block32<COLS>; };
+
+// Starts the load of 32 or 16 accumulator columns; the values may be used after tmem_wait.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// The registers are operands, so that no use of them moves above the wait.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 
 __device__ __forceinline__ void tma_load_3d_hint(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z,
@@ -93,18 +216,47 @@ __device__ __forceinline__ void tma_load_3d_hint(uint32_t dst, const CUtensorMap
       : "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy)
       : "memory");
 }
-__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+// Arrival on a barrier of another CTA that orders this CTA's own accesses only: what it announces are tensor-memory
+// reads, ordered by their own wait and fence. A release at cluster scope would first wait for the epilogue's global
+// stores (1500 cycles per tile).
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Asks L2 for a tile of an epilogue matrix.
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+               "r"(y), "r"(z)
+               : "memory");
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t n;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
-  return n;
+// True in one lane of a converged warp. Instructions of the tensor and TMA units take their operands from uniform
+// registers; behind this predicate the compiler knows that one lane is active, behind `lane == 0` it does not and walks
+// through the lanes (measured: 550 cycles for the four MMAs of a stage, whatever their width).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one)::"memory");
+  return one != 0;
+}
+// Bounded wait of a whole converged warp: one lane polls (32 lanes polling cost the MMA issuer 150 us of 920 at 8192^3).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned code,
+                                          unsigned int* status) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, code, status) ? 1 : 0;
+  return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned code,
+                                                  unsigned int* status) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait_cluster(bar, parity, abort_flag, code, status) ? 1 : 0;
+  return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
 }
 
 // One tile of the walk.
@@ -122,12 +274,22 @@ __device__ __forceinline__ int total_tiles(const FusedParams& p, const int* tile
   return p.tiles_m * p.tiles_n * p.problems;
 }
 
+// a / b for 0 <= a < 2^30 and b > 0 by a float quotient and a correction; exact.
+__device__ __forceinline__ int divide(int a, int b) {
+  if (a < b) return 0;
+  if (a >= (1 << 22)) return a / b;  // the quotient's error stays below one for smaller numerators
+  int q = __float2int_rz(__fdividef(__int2float_rn(a), __int2float_rn(b)));
+  const int r = a - q * b;
+  q += (r >= b) - (r < 0);
+  return q;
+}
+
 template <int BN>
 __device__ __forceinline__ Tile locate(const FusedParams& p, int tile, const int* start, const int* tiles) {
   Tile t;
   int in_problem, cols;
   if (p.kind == kFusedRaggedCols) {
-    const int want = tile / p.tiles_m;  // the group with tiles[g] <= want < tiles[g + 1]
+    const int want = divide(tile, p.tiles_m);  // the group with tiles[g] <= want < tiles[g + 1]
     int lo = 0, hi = p.problems;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -138,12 +300,12 @@ __device__ __forceinline__ Tile locate(const FusedParams& p, int tile, const int
     cols = tiles[lo + 1] - tiles[lo];
   } else if (p.tri) {
     const int per = p.tiles_m * (p.tiles_m + 1) / 2;
-    t.z = tile / per;
+    t.z = divide(tile, per);
     in_problem = tile - t.z * per;
     cols = p.tiles_n;
   } else {
     const int per = p.tiles_m * p.tiles_n;
-    t.z = tile / per;
+    t.z = divide(tile, per);
     in_problem = tile - t.z * per;
     cols = p.tiles_n;
   }
@@ -155,11 +317,11 @@ __device__ __forceinline__ Tile locate(const FusedParams& p, int tile, const int
     t.tn = in_problem - r * (r + 1) / 2;
   } else {
     const int per_group = p.raster * cols;
-    const int group = in_problem / per_group;
+    const int group = divide(in_problem, per_group);
     const int first = group * p.raster;
     const int rows = min(p.raster, p.tiles_m - first);
     const int in_group = in_problem - group * per_group;
-    t.tn = in_group / rows;
+    t.tn = divide(in_group, rows);
     t.tm = first + in_group - t.tn * rows;
   }
   t.k0 = 0;
@@ -183,21 +345,19 @@ __device__ __forceinline__ Tile locate(const FusedParams& p, int tile, const int
   return t;
 }
 
-template <class T, class DT, class OT>
-struct Types {
-  static constexpr int CB = 32 / static_cast<int>(sizeof(OT));  // columns per block: 32 bytes of a column-of-columns
-  static constexpr int C_BYTES = CB * BM * static_cast<int>(sizeof(OT));
-  static constexpr int Z_BYTES = CB * BM * 2;
-};
+// What the epilogue is compiled for. The first two need 16-byte accesses to C, D and Z; the third takes everything else,
+// tiles shared by a cluster included.
+enum FusedMode : int { kModeForward = 0, kModeGrad = 1, kModeGeneral = 2 };
 
-template <int CTAS, int BN, class T, class DT, class OT>
-__global__ void __launch_bounds__(64 + 128 * (BN >= 128 ? 2 : 1), 1)
+template <int CTAS, int BN, class T, class DT, class OT, int MODE>
+__global__ void __launch_bounds__(fused_threads(BN), 1)
 fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                  const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_d,
-                  const __grid_constant__ CUtensorMap map_z, const FusedParams p) {
+                  const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_z,
+                  const FusedParams p) {
   static_assert(sizeof(DT) == sizeof(OT), "D and C share the staging buffers");
-  constexpr int EG = BN >= 128 ? 2 : 1;
-  constexpr int CB = Types<T, DT, OT>::CB;
+  constexpr bool CHUNKED = sizeof(OT) == 4;
+  constexpr int EG = fused_groups(BN);
+  constexpr int CB = fused_block_cols(CHUNKED);  // columns per epilogue block
   constexpr int B_ROWS = BN / CTAS;
   constexpr int A_BYTES = BM * BK * 2;
   constexpr int STAGE_BYTES = A_BYTES + B_ROWS * BK * 2;
@@ -211,25 +371,30 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   uint8_t* const base_ptr = smem_raw + (tiles_base - raw);
   const bool aux = p.z != nullptr;
   const int stages = p.stages;
+  const int split = (CTAS == 1 && MODE == kModeGeneral) ? p.split : 1;
   uint8_t* const staging = base_ptr + stages * STAGE_BYTES;
-  const int sb = staging_bytes(EG, aux);
-  uint8_t* const behind = staging + (p.split > 1 && sums_bytes(BN) > sb ? sums_bytes(BN) : sb);
+  uint8_t* const behind = staging + fused_staging_bytes(BN, CHUNKED, aux, split);
   const uint32_t bar_base = smem_u32(behind);
-  // full [0, 16), empty [16, 32), accumulator full / empty [32, 36), sums ready / free [36, 38), loads [40, 40 + 8)
+  // full [0, 16), empty [16, 32), accumulator full / empty [32, 36), sums ready / free [36, 38), tail [40, 56)
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (16 + s); };
   auto acc_full_bar = [&](int a) { return bar_base + 8u * (32 + a); };
   auto acc_empty_bar = [&](int a) { return bar_base + 8u * (34 + a); };
   const uint32_t sums_ready = bar_base + 8u * 36, sums_free = bar_base + 8u * 37;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(behind + 8 * 48);
+  // Pairs with a ragged inner extent: the second CTA has cleared the end of the block in this stage. (That the block has
+  // landed there it learns from its own full barrier.) One barrier per stage: of groups shorter than the ring several
+  // last blocks are under way at once.
+  auto tail_bar = [&](int s) { return bar_base + 8u * (40 + s); };
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(behind + 8 * 56);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* const start = reinterpret_cast<int*>(behind + BAR_BYTES);
+  volatile int* const progress = abort_flag + 1;  // tiles that the epilogue has begun
+  int* const start = reinterpret_cast<int*>(behind + kFusedBarBytes);
   int* const tiles = start + p.problems + 1;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = (CTAS == 2 || p.split > 1) ? cluster_ctarank() : 0u;
-  const int team = CTAS == 2 ? 2 : p.split;          // CTAs that work on one tile
+  const uint32_t rank = (CTAS == 2 || split > 1) ? cluster_ctarank() : 0u;
+  const int team = CTAS == 2 ? 2 : split;          // CTAs that work on one tile
   const int first_tile = static_cast<int>(blockIdx.x) / team;
   const int tile_step = static_cast<int>(gridDim.x) / team;
 
@@ -242,10 +407,11 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       mbar_init(acc_full_bar(a), 1);
       mbar_init(acc_empty_bar(a), 4 * EG * CTAS);
     }
-    mbar_init(sums_ready, 4 * EG * p.split);
-    mbar_init(sums_free, 4 * EG * p.split);
-    for (int b = 0; b < EG * RING; ++b) mbar_init(bar_base + 8u * (40 + b), 1);
+    mbar_init(sums_ready, 4 * EG * split);
+    mbar_init(sums_free, 4 * EG * split);
+    for (int s = 0; s < stages; ++s) mbar_init(tail_bar(s), 1);
     *abort_flag = 0;
+    *progress = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -255,7 +421,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   if (warp == 2 && p.kind == kFusedRaggedCols) build_table(p.offsets, p.problems, p.n, BN, start, tiles);
   tcgen05_fence_before();
   __syncthreads();
-  if (CTAS == 2 || p.split > 1) cluster_sync_all();  // all barriers exist before anyone signals across CTAs
+  if (CTAS == 2 || split > 1) cluster_sync_all();  // all barriers exist before anyone signals across CTAs
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int num_tiles = total_tiles(p, tiles);
@@ -263,9 +429,9 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   // this CTA's share of a tile's inner blocks
   auto k_range = [&](const Tile& t, int& kb0, int& kb1) {
     const int blocks = (t.k_len + BK - 1) / BK;
-    if (CTAS == 1 && p.split > 1) {
-      kb0 = blocks * static_cast<int>(rank) / p.split;
-      kb1 = blocks * (static_cast<int>(rank) + 1) / p.split;
+    if (split > 1) {
+      kb0 = blocks * static_cast<int>(rank) / split;
+      kb1 = blocks * (static_cast<int>(rank) + 1) / split;
     } else {
       kb0 = 0;
       kb1 = blocks;
@@ -273,8 +439,8 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   };
 
   if (warp == 0) {
-    // ---- TMA producer ----
-    if (lane == 0) {
+    // ---- TMA producer: the warp walks along, one lane issues ----
+    {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -287,34 +453,47 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         int kb0, kb1;
         k_range(t, kb0, kb1);
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, 1u, p.status)) { ok = false; break; }
-          const uint32_t a_dst = tiles_base + stage * STAGE_BYTES;
-          const uint32_t b_dst = a_dst + A_BYTES;
-          const int x = t.k0 + kb * BK;
-          uint32_t bar;
-          if constexpr (CTAS == 2) {
-            bar = map_to_cta(full_bar(stage), 0);
-            if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * STAGE_BYTES);  // the bytes of both CTAs
-          } else {
-            bar = full_bar(stage);
-            mbar_arrive_expect_tx(bar, STAGE_BYTES);
-          }
-          auto load = [&](uint32_t dst, const CUtensorMap* map, int cx, int cy, int cz, uint64_t pol) {
-            if constexpr (CTAS == 2) tma_load_3d_pair_hint(dst, map, bar, cx, cy, cz, pol);
-            else tma_load_3d_hint(dst, map, bar, cx, cy, cz, pol);
-          };
-          if (p.a_mn) {
+          ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, 1u, p.status);
+          if (!ok) break;
+          if (elect_one()) {
+            const uint32_t a_dst = tiles_base + stage * STAGE_BYTES;
+            const uint32_t b_dst = a_dst + A_BYTES;
+            const int x = t.k0 + kb * BK;
+            uint32_t bar;
+            if constexpr (CTAS == 2) {
+              // a block whose end has to be cleared is counted by each CTA for itself
+              const bool tail = p.kind == kFusedRaggedInner && t.k_len - kb * BK < BK;
+              if (rank == 0) {
+                bar = map_to_cta(full_bar(stage), 0);
+                mbar_arrive_expect_tx(full_bar(stage), (tail ? 1 : 2) * STAGE_BYTES);  // otherwise the bytes of both CTAs
+              } else if (tail) {
+                bar = map_to_cta(full_bar(stage), 1);
+                mbar_arrive_expect_tx(full_bar(stage), STAGE_BYTES);
+              } else {
+                bar = map_to_cta(full_bar(stage), 0);
+              }
+            } else {
+              bar = full_bar(stage);
+              mbar_arrive_expect_tx(bar, STAGE_BYTES);
+            }
+            auto load = [&](uint32_t dst, const CUtensorMap* map, int cx, int cy, int cz, uint64_t pol) {
+              if constexpr (CTAS == 2) tma_load_3d_pair_hint(dst, map, bar, cx, cy, cz, pol);
+              else tma_load_3d_hint(dst, map, bar, cx, cy, cz, pol);
+            };
+            if (p.a_mn) {
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) load(a_dst + j * 8192, &map_a, a_row0 + j * 64, x, az, pol_a);
-          } else {
-            load(a_dst, &map_a, x, a_row0, az, pol_a);
-          }
-          if (p.b_mn) {
+              for (int j = 0; j < BM / 64; ++j) load(a_dst + j * 8192, &map_a, a_row0 + j * 64, x, az, pol_a);
+            } else {
+              load(a_dst, &map_a, x, a_row0, az, pol_a);
+            }
+            if (p.b_mn) {
 #pragma unroll
-            for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * 8192, &map_b, b_row0 + j * 64, x, bz, pol_b);
-          } else {
-            load(b_dst, &map_b, x, b_row0, bz, pol_b);
+              for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * 8192, &map_b, b_row0 + j * 64, x, bz, pol_b);
+            } else {
+              load(b_dst, &map_b, x, b_row0, bz, pol_b);
+            }
           }
+          __syncwarp();
           if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
       }
@@ -325,326 +504,467 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       }
     }
   } else if (warp == 1) {
-    // ---- MMA issuer (of a pair: the leader, for both SMs). The whole warp walks along; lane 0 issues. ----
+    // Of a ragged inner extent the last block holds inner indices of the next group (or whatever lies behind the matrix).
+    // Both operands have one 128-byte row per inner index and 64 elements of m / n; rows up to the next multiple of an
+    // MMA's 16 are cleared in both (0 * NaN would not be 0), the MMAs behind that are left out. Called by the whole warp.
+    auto clear_tail = [&](int stage, int valid) {
+      const int steps = (valid + 15) / 16, rows = steps * 16 - valid;
+      uint8_t* const s = base_ptr + stage * STAGE_BYTES;
+      constexpr int TILES = BM / 64 + B_ROWS / 64;
+      for (int i = lane; i < rows * TILES * 8; i += 32) {
+        const int chunk = i & 7, r = (i >> 3) % rows, j = (i >> 3) / rows;
+        *reinterpret_cast<uint4*>(s + j * 8192 + (valid + r) * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      return steps;
+    };
+    if (CTAS == 2 && rank == 1 && p.kind == kFusedRaggedInner) {
+      // ---- second CTA of a pair: clears the end of its own operands and tells the leader ----
+      int blocks_before = 0;
+      uint32_t phases = 0;  // of the full barriers, one bit per stage
+      for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
+        const Tile t = locate<BN>(p, tile, start, tiles);
+        blocks_before += (t.k_len + BK - 1) / BK;
+        if (t.k_len % BK == 0) continue;
+        const int stage = (blocks_before - 1) % stages;
+        if (!warp_wait(full_bar(stage), (phases >> stage) & 1u, abort_flag, 10u, p.status)) break;
+        phases ^= 1u << stage;
+        clear_tail(stage, t.k_len % BK);
+        if (lane == 0) mbar_arrive_remote(map_to_cta(tail_bar(stage), 0));
+      }
+    }
+    // ---- MMA issuer (of a pair: the leader, for both SMs): the warp walks along, one lane issues ----
     if (CTAS == 1 || rank == 0) {
+      auto wait = [&](uint32_t bar, uint32_t parity, unsigned code) { return warp_wait(bar, parity, abort_flag, code, p.status); };
+      auto commit = [&](uint32_t bar) {
+        if constexpr (CTAS == 2) umma_commit_pair(bar);
+        else umma_commit(bar);
+      };
+      // K-major: 128-byte rows along K (stride offset 1024 = eight rows), 32 B per MMA step. MN-major: one 128-byte row of
+      // 64 elements per k, blocks 8192 B apart, 2048 B per MMA step.
+      const uint64_t a_form = smem_desc(0, p.a_mn ? 8192 : 16, 1024, kLayoutSw128);
+      const uint64_t b_form = smem_desc(0, p.b_mn ? 8192 : 16, 1024, kLayoutSw128);
+      const uint32_t a_step = p.a_mn ? (2048u >> 4) : 2u, b_step = p.b_mn ? (2048u >> 4) : 2u;
+      const uint32_t idesc = p.idesc;
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
+      uint32_t tail_phases = 0;
       bool ok = true;
       for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++local) {
         const Tile t = locate<BN>(p, tile, start, tiles);
         int kb0, kb1;
         k_range(t, kb0, kb1);
-        const int acc = local & 1;
-        const uint32_t acc_phase = (local >> 1) & 1u;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag, 2u, p.status));
+        int acc = local & 1;
+        ok = wait(acc_empty_bar(acc), ((local >> 1) & 1u) ^ 1u, 2u);
         if (!ok) break;
         tcgen05_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        int first_kb = kb0;  // first block of the current accumulator
         for (int kb = kb0; kb < kb1; ++kb) {
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait(full_bar(stage), phase, abort_flag, 3u, p.status));
+          if (CHUNKED && kb - first_kb == kChunk) {  // hand this accumulator over and go on in the other one
+            if (elect_one()) commit(acc_full_bar(acc));
+            __syncwarp();
+            ++local;
+            first_kb = kb;
+            acc = local & 1;
+            ok = wait(acc_empty_bar(acc), ((local >> 1) & 1u) ^ 1u, 2u);
+            if (!ok) break;
+            tcgen05_fence_after();
+            d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+          }
+          ok = wait(full_bar(stage), phase, 3u);
           if (!ok) break;
-          const uint32_t a_src = tiles_base + stage * STAGE_BYTES;
-          const uint32_t b_src = a_src + A_BYTES;
           int steps = BK / 16;
-          if (CTAS == 1 && p.kind == kFusedRaggedInner) {
-            // The last block of a group holds inner indices of the next one (or whatever lies behind the matrix). Both
-            // operands have one 128-byte row per inner index and 64 elements of m / n; rows up to the next multiple
-            // of an MMA's 16 are cleared in both (0 * NaN would not be 0), the MMAs behind that are left out.
-            const int valid = t.k_len - kb * BK;
-            if (valid < BK) {
-              steps = (valid + 15) / 16;
-              const int rows = steps * 16 - valid;
-              uint8_t* const s = base_ptr + stage * STAGE_BYTES;
-              constexpr int BLOCKS = BM / 64 + B_ROWS / 64;
-              for (int i = lane; i < rows * BLOCKS * 8; i += 32) {
-                const int chunk = i & 7, r = (i >> 3) % rows, j = (i >> 3) / rows;
-                *reinterpret_cast<uint4*>(s + j * 8192 + (valid + r) * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
-              }
-              fence_proxy_async();
-              __syncwarp();
+          if (p.kind == kFusedRaggedInner && t.k_len - kb * BK < BK) {
+            steps = clear_tail(stage, t.k_len - kb * BK);
+            if (CTAS == 2) {
+              ok = warp_wait_cluster(tail_bar(stage), (tail_phases >> stage) & 1u, abort_flag, 11u, p.status);
+              if (!ok) break;
+              tail_phases ^= 1u << stage;
             }
           }
           tcgen05_fence_after();
-          if (lane == 0) {
-            // K-major: 128-byte rows along K (stride offset 1024 = eight rows), 32 B per MMA step. MN-major: one
-            // 128-byte row of 64 elements per k, blocks 8192 B apart, 2048 B per MMA step.
-            const uint64_t da = p.a_mn ? smem_desc(a_src, 8192, 1024, kLayoutSw128) : smem_desc(a_src, 16, 1024, kLayoutSw128);
-            const uint64_t db = p.b_mn ? smem_desc(b_src, 8192, 1024, kLayoutSw128) : smem_desc(b_src, 16, 1024, kLayoutSw128);
-            const uint32_t a_step = p.a_mn ? (2048u >> 4) : 2u, b_step = p.b_mn ? (2048u >> 4) : 2u;
+          if (elect_one()) {
+            const uint32_t a_src = tiles_base + stage * STAGE_BYTES;
+            // (an address in a cluster carries the CTA's rank above the 18 bits that the descriptor takes)
+            const uint64_t da = a_form | ((a_src >> 4) & 0x3FFFu), db = b_form | (((a_src + A_BYTES) >> 4) & 0x3FFFu);
+            const uint32_t fresh = kb == first_kb ? 0u : 1u;
+            auto mma = [&](int ks) {
+              if constexpr (CTAS == 2) umma_f16_pair(d_tmem, da + a_step * ks, db + b_step * ks, idesc, ks == 0 ? fresh : 1u);
+              else umma_f16(d_tmem, da + a_step * ks, db + b_step * ks, idesc, ks == 0 ? fresh : 1u);
+            };
+            if (steps == BK / 16) {
 #pragma unroll
-            for (int ks = 0; ks < BK / 16; ++ks) {
-              if (ks < steps) {
-                const uint32_t accumulate = (kb != kb0 || ks != 0) ? 1u : 0u;
-                if constexpr (CTAS == 2) umma_f16_pair(d_tmem, da + a_step * ks, db + b_step * ks, p.idesc, accumulate);
-                else umma_f16(d_tmem, da + a_step * ks, db + b_step * ks, p.idesc, accumulate);
-              }
+              for (int ks = 0; ks < BK / 16; ++ks) mma(ks);
+            } else {
+              for (int ks = 0; ks < steps; ++ks) mma(ks);
             }
-            if constexpr (CTAS == 2) umma_commit_pair(empty_bar(stage));
-            else umma_commit(empty_bar(stage));
+            commit(empty_bar(stage));
           }
+          __syncwarp();
           if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
-        if (ok && lane == 0) {  // without inner blocks this arrives at once and the epilogue takes zeros
-          if constexpr (CTAS == 2) umma_commit_pair(acc_full_bar(acc));
-          else umma_commit(acc_full_bar(acc));
+        if (ok && elect_one()) commit(acc_full_bar(acc));  // without inner blocks this arrives at once: zeros are taken
+      }
+    }
+  } else if (warp == 3) {
+    // ---- D and Z of the next tile on their way to L2 while this one's operands are multiplied ----
+    if (MODE != kModeGeneral && p.prefetch && lane == 0) {
+      for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
+        // at most two tiles ahead of the epilogue; a hint, so it does not insist
+        const int n = (tile - first_tile) / tile_step;
+        for (int spin = 0; spin < 20000 && *progress < n - 1 && !*abort_flag; ++spin) __nanosleep(200);
+        const Tile t = locate<BN>(p, tile, start, tiles);
+        const int row0 = (t.tm * CTAS + (CTAS == 2 ? static_cast<int>(rank) : 0)) * BM;
+        const int zc = p.kind == kFusedRaggedCols ? 0 : t.z;
+        if (row0 < p.m) {
+#pragma unroll
+          for (int c = 0; c < BN; c += 32) {
+            if (t.col0 + c >= t.col_end) break;
+            if (p.d != nullptr) tma_prefetch_3d(&map_d, row0, t.col0 + c, zc);
+            if (MODE == kModeGrad && aux) tma_prefetch_3d(&map_z, row0, t.col0 + c, zc);
+          }
         }
       }
     }
-  } else {
+  } else if (warp >= 4) {
     // ---- epilogue ----
-    const int group = EG == 1 ? 0 : (warp - 2) >> 2;
+    using BlockC = typename BlockOf<OT, CB>::type;
+    using BlockD = typename BlockOf<DT, CB>::type;
+    using BlockZ = Block16<T, CB>;
+    constexpr int BLOCKS = GROUP_COLS / CB;
+    const int group = (warp - 4) >> 2;
     const int quad = warp & 3;  // tensor-memory lanes this warp may read
     const int row_in_cta = quad * 32 + lane;
-    const int bar_id = 1 + group;
-    const bool elected = (threadIdx.x & 127) == 64;  // first thread of each group
-    uint8_t* const ring_c = staging + group * RING * SLOT * (aux ? 2 : 1);
-    uint8_t* const ring_z = ring_c + RING * SLOT;
-    const uint32_t load_bars = bar_base + 8u * (40 + group * RING);
     const bool has_d = p.d != nullptr;
-    const bool z_in = aux && p.grad, z_out = aux && !p.grad;
-    const uint32_t load_bytes = (has_d ? Types<T, DT, OT>::C_BYTES : 0) + (z_in ? Types<T, DT, OT>::Z_BYTES : 0);
-    int local = 0, blocks_done = 0;
-    uint32_t load_phases = 0;
+    const bool grad = MODE == kModeGrad || (MODE == kModeGeneral && p.grad);
+    const bool z_in = aux && grad, z_out = aux && !grad;
+    int local = 0;   // accumulators taken so far
+    int tiles_done = 0;
     bool ok = true;
 
-    // requests D and Z of the block that will be number `block` (elected thread only)
-    auto request = [&](int block, int row0, int col, int z) {
-      const int b = block & (RING - 1);
-      const uint32_t bar = load_bars + 8u * b;
-      mbar_arrive_expect_tx(bar, load_bytes);
-      if (has_d) tma_load_3d(smem_u32(ring_c + b * SLOT), &map_d, bar, row0, col, z);
-      if (z_in) tma_load_3d(smem_u32(ring_z + b * SLOT), &map_z, bar, row0, col, z);
-    };
-
-    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++local) {
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++tiles_done) {
+      if (threadIdx.x == 128) *progress = tiles_done + 1;
       const Tile t = locate<BN>(p, tile, start, tiles);
       const int cta_row0 = (t.tm * CTAS + (CTAS == 2 ? static_cast<int>(rank) : 0)) * BM;
+      const int warp_row0 = cta_row0 + quad * 32;
       const int row = cta_row0 + row_in_cta;
-      const bool live = cta_row0 < p.m;  // the second CTA of a pair may lie wholly below C
+      const int rows_left = p.m - warp_row0;  // may be negative: the tile's last warps may lie wholly below C
       const bool in_rows = row < p.m;
-      const int zc = p.kind == kFusedRaggedCols ? 0 : t.z;  // third coordinate of C, D, Z
+      const int zc = p.kind == kFusedRaggedCols ? 0 : t.z;  // plane of C, D, Z
       const float bias = (p.bias != nullptr && in_rows) ? to_float(static_cast<const T*>(p.bias)[t.z * p.bias_stride + row]) : 0.f;
-      OT* const c_ptr = static_cast<OT*>(p.c) + zc * p.c_stride;
-      const DT* const d_ptr = static_cast<const DT*>(p.d) + zc * p.d_stride;
-      T* const z_ptr = static_cast<T*>(p.z) + zc * p.z_stride;
+      const int group_col0 = t.col0 + group * GROUP_COLS;
+      const int group_cols = t.col_end - group_col0;  // columns that exist from this group's first one on
+      // first element of this warp's part
+      OT* const c_ptr = static_cast<OT*>(p.c) + zc * p.c_stride + static_cast<long long>(group_col0) * p.ldc + warp_row0;
+      const DT* const d_ptr = static_cast<const DT*>(p.d) + zc * p.d_stride + static_cast<long long>(group_col0) * p.ldd + warp_row0;
+      T* const z_ptr = static_cast<T*>(p.z) + zc * p.z_stride + static_cast<long long>(group_col0) * p.ldz + warp_row0;
       float row_sum = 0.f;
-      const int acc = local & 1;
-      const uint32_t acc_phase = (local >> 1) & 1u;
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
       int kb0, kb1;
       k_range(t, kb0, kb1);
       const bool empty = kb1 <= kb0;
-
-      if (CTAS == 1 && p.split > 1) {
-        // -- tile shared by a cluster: sums meet in shared memory, every CTA finishes a range of columns --
-        float* const sums = reinterpret_cast<float*>(staging);  // [column][128 rows]
-        ok = mbar_wait(acc_full_bar(acc), acc_phase, abort_flag, 4u, p.status);
-        if (ok && local > 0) ok = mbar_wait_cluster(sums_free, (local - 1) & 1u, abort_flag, 7u, p.status);
-        ok = group_all(bar_id, ok);
-        if (!ok) break;
-        tcgen05_fence_after();
-#pragma unroll 1
-        for (int cb = 0; cb < GROUP_COLS / 16; ++cb) {
-          const int col = group * GROUP_COLS + cb * 16;
-          uint32_t r[16];
-          if (!empty) tmem_ld<16>(t_row + col, r);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) sums[(col + j) * BM + row_in_cta] = empty ? 0.f : __uint_as_float(r[j]);
-        }
+      auto accumulator = [&](int number) {
+        return tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>((number & 1) * BN + group * GROUP_COLS);
+      };
+      auto wait_accumulator = [&](int number) {
+        return warp_wait(acc_full_bar(number & 1), (number >> 1) & 1u, abort_flag, 4u, p.status);
+      };
+      auto release_accumulator = [&](int number) {
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(acc_empty_bar(acc));
-          for (int q = 0; q < p.split; ++q) mbar_arrive_remote(map_to_cta(sums_ready, q));
+          if constexpr (CTAS == 2) mbar_arrive_peer(map_to_cta(acc_empty_bar(number & 1), 0));
+          else mbar_arrive(acc_empty_bar(number & 1));
         }
-        ok = mbar_wait_cluster(sums_ready, local & 1u, abort_flag, 8u, p.status);
-        ok = group_all(bar_id, ok);
-        if (!ok) break;
-        const int mine = BN / p.split;  // a multiple of four
-        for (int q = group; q < mine / 4; q += EG) {
-          const int in_tile = static_cast<int>(rank) * mine + q * 4;
-          const int col = t.col0 + in_tile;
-          if (col >= t.col_end) break;
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int s = 0; s < p.split; ++s) {
-            const uint32_t src = map_to_cta(smem_u32(sums + in_tile * BM + row_in_cta), s);
+      };
+
+      // results in single precision: all partial sums of this warp's columns, in registers
+      float sum[CHUNKED ? GROUP_COLS : 1];
+      if constexpr (CHUNKED) {
+        const int chunks = empty ? 1 : (kb1 - kb0 + kChunk - 1) / kChunk;
+        for (int c = 0; c < chunks; ++c) {
+          ok = wait_accumulator(local);
+          if (!ok) break;
+          tcgen05_fence_after();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] += ld_cluster_f32(src + j * BM * 4);
-          }
+          for (int cb = 0; cb < BLOCKS; ++cb) {
+            uint32_t r[CB];
+            if (empty) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (!in_rows || col + j >= t.col_end) continue;
-            const long long cj = col + j;
-            const float add = has_d ? p.beta * to_float(d_ptr[cj * p.ldd + row]) : 0.f;
-            float y = p.alpha * v[j] + bias;
-            if (p.grad) {
-              y += add;
-              if (z_in) y *= act_slope<FAST>(p.act, to_float(z_ptr[cj * p.ldz + row]));
-              row_sum += y;
+              for (int j = 0; j < CB; ++j) sum[cb * CB + j] = 0.f;
             } else {
-              if (z_out) z_ptr[cj * p.ldz + row] = from_float<T>(y);
-              y = act_value<FAST>(p.act, y) + add;
+              tmem_ld(accumulator(local) + cb * CB, r);
+              tmem_wait(r);
+#pragma unroll
+              for (int j = 0; j < CB; ++j) sum[cb * CB + j] = c == 0 ? __uint_as_float(r[j]) : sum[cb * CB + j] + __uint_as_float(r[j]);
             }
-            c_ptr[cj * p.ldc + row] = from_float<OT>(y);
           }
+          release_accumulator(local);
+          ++local;
         }
-        __syncwarp();
-        if (lane == 0) {
-          for (int q = 0; q < p.split; ++q) mbar_arrive_remote(map_to_cta(sums_free, q));
-        }
-        if (p.partial != nullptr && in_rows)
-          p.partial[(static_cast<long long>(t.col_tile * p.split + static_cast<int>(rank)) * EG + group) * p.m + row] = row_sum;
-        continue;
+        if (!ok) break;
       }
 
-      const int group_col0 = t.col0 + group * GROUP_COLS;
-      const bool loads = p.tma && live && load_bytes != 0;
-      if (elected && loads) {
-        if (group_col0 < t.col_end) request(blocks_done, cta_row0, group_col0, zc);
-        if (group_col0 + CB < t.col_end) request(blocks_done + 1, cta_row0, group_col0 + CB, zc);
-      }
-      ok = mbar_wait(acc_full_bar(acc), acc_phase, abort_flag, 4u, p.status);
-      ok = group_all(bar_id, ok);  // all four warps go on, or none
-      if (!ok) break;
-      tcgen05_fence_after();
-#pragma unroll 1
-      for (int cb = 0; cb < GROUP_COLS / CB; ++cb) {
-        const int col = group_col0 + cb * CB;
-        if (col >= t.col_end) break;  // uniform over the group
-        uint32_t r[CB];
-        if (empty) {
-#pragma unroll
-          for (int j = 0; j < CB; ++j) r[j] = 0u;
-        } else {
-          tmem_ld<CB>(t_row + group * GROUP_COLS + cb * CB, r);
-        }
-        const int valid = min(CB, t.col_end - col);
-        float v[CB];
-        const int b = blocks_done & (RING - 1);
-        OT* const slot_c = reinterpret_cast<OT*>(ring_c + b * SLOT) + row_in_cta;
-        T* const slot_z = reinterpret_cast<T*>(ring_z + b * SLOT) + row_in_cta;
-        if (p.tma) {
-          if (loads) {
-            ok = wait_old_block(load_bars + 8u * b, (load_phases >> b) & 1u, p.status);
-            load_phases ^= 1u << b;
+      if constexpr (MODE == kModeGeneral) {
+        if (split > 1) {
+          // -- tile shared by a cluster: sums meet in shared memory, every CTA finishes a range of columns --
+          float* const sums = reinterpret_cast<float*>(staging);  // [column][128 rows]
+          if constexpr (!CHUNKED) {
+            ok = wait_accumulator(local);
+            if (!ok) break;
+            tcgen05_fence_after();
+          }
+          if (tiles_done > 0) {
+            ok = warp_wait_cluster(sums_free, (tiles_done - 1) & 1u, abort_flag, 7u, p.status);
             if (!ok) break;
           }
 #pragma unroll
-          for (int j = 0; j < CB; ++j) v[j] = p.alpha * __uint_as_float(r[j]) + bias;
-          if (p.grad) {
-            if (has_d) {
+          for (int cb = 0; cb < BLOCKS; ++cb) {
+            const int col = group * GROUP_COLS + cb * CB;
+            if constexpr (CHUNKED) {
 #pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] += p.beta * to_float(reinterpret_cast<const DT*>(slot_c)[j * BM]);
-            }
-            if (z_in) {
+              for (int j = 0; j < CB; ++j) sums[(col + j) * BM + row_in_cta] = sum[cb * CB + j];
+            } else {
+              uint32_t r[CB];
+              if (!empty) {
+                tmem_ld(accumulator(local) + cb * CB, r);
+                tmem_wait(r);
+              }
 #pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] *= act_slope<FAST>(p.act, to_float(slot_z[j * BM]));
+              for (int j = 0; j < CB; ++j) sums[(col + j) * BM + row_in_cta] = empty ? 0.f : __uint_as_float(r[j]);
             }
+          }
+          if constexpr (!CHUNKED) {
+            release_accumulator(local);
+            ++local;
+          }
+          __syncwarp();
+          if (lane == 0) {
+            for (int q = 0; q < split; ++q) mbar_arrive_remote(map_to_cta(sums_ready, q));
+          }
+          ok = warp_wait_cluster(sums_ready, tiles_done & 1u, abort_flag, 8u, p.status);
+          if (!ok) break;
+          const int mine = BN / split;  // a multiple of four
+          for (int q = group; q < mine / 4; q += EG) {
+            const int in_tile = static_cast<int>(rank) * mine + q * 4;
+            const int rel = in_tile - group * GROUP_COLS;  // column relative to group_col0
+            const int cols_left = t.col_end - (t.col0 + in_tile);
+            if (cols_left <= 0) break;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < split; ++s) {
+              const uint32_t src = map_to_cta(smem_u32(sums + in_tile * BM + row_in_cta), s);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] += ld_cluster_f32(src + j * BM * 4);
+            }
+            with_act(p.act, [&](auto tag) {
+              constexpr int ACT = decltype(tag)::value;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (!in_rows || j >= cols_left) continue;
+                const long long cj = rel + j;
+                const float add = has_d ? p.beta * to_float(d_ptr[cj * p.ldd + lane]) : 0.f;
+                float y = p.alpha * v[j] + bias;
+                if (grad) {
+                  y += add;
+                  if (z_in) y *= act_slope<FAST, ACT>(to_float(z_ptr[cj * p.ldz + lane]));
+                  row_sum += y;
+                } else {
+                  if (z_out) z_ptr[cj * p.ldz + lane] = from_float<T>(y);
+                  y = act_value<FAST, ACT>(y) + add;
+                }
+                c_ptr[cj * p.ldc + lane] = from_float<OT>(y);
+              }
+            });
+          }
+          __syncwarp();
+          if (lane == 0) {
+            for (int q = 0; q < split; ++q) mbar_arrive_remote(map_to_cta(sums_free, q));
+          }
+          if (p.partial != nullptr && in_rows)
+            p.partial[(static_cast<long long>(t.col_tile * split + static_cast<int>(rank)) * EG + group) * p.m + row] = row_sum;
+          continue;
+        }
+      }
+
+      // accumulator values of block cb; the load of the next block starts as this one's arrives
+      uint32_t r_next[CB];
+      auto take = [&](int cb, float (&v)[CB]) {
+        if constexpr (CHUNKED) {
+#pragma unroll
+          for (int i = 0; i < BLOCKS; ++i) {
+            if (i == cb) {
+#pragma unroll
+              for (int j = 0; j < CB; ++j) v[j] = sum[i * CB + j];
+            }
+          }
+        } else if (empty) {
+#pragma unroll
+          for (int j = 0; j < CB; ++j) v[j] = 0.f;
+        } else {
+          tmem_wait(r_next);
+#pragma unroll
+          for (int j = 0; j < CB; ++j) v[j] = __uint_as_float(r_next[j]);
+          if (cb + 1 < BLOCKS) tmem_ld(accumulator(local) + (cb + 1) * CB, r_next);
+        }
+#pragma unroll
+        for (int j = 0; j < CB; ++j) v[j] = fmaf(p.alpha, v[j], bias);
+      };
+      auto begin = [&]() {
+        if constexpr (!CHUNKED) {
+          ok = wait_accumulator(local);
+          if (!ok) return false;
+          tcgen05_fence_after();
+          if (!empty) tmem_ld(accumulator(local), r_next);
+        }
+        return true;
+      };
+      auto end = [&]() {
+        if constexpr (!CHUNKED) {
+          if (!empty) tmem_wait(r_next);  // a load may have started for a block that does not exist
+          release_accumulator(local);
+          ++local;
+        }
+      };
+
+      if constexpr (MODE != kModeGeneral) {
+        // D and Z of a block are requested while the block before it is worked on
+        BlockD d_next;
+        BlockZ z_next;
+        auto request = [&](int cb) {
+          if (has_d) d_next.load(d_ptr + static_cast<long long>(cb * CB) * p.ldd, p.ldd, rows_left, group_cols - cb * CB, lane);
+          if (MODE == kModeGrad && aux) z_next.load(z_ptr + static_cast<long long>(cb * CB) * p.ldz, p.ldz, rows_left, group_cols - cb * CB, lane);
+        };
+        if (!CHUNKED) request(0);
+        if (!begin()) break;
+        uint8_t* const own = staging + (warp - 4) * fused_warp_bytes(CHUNKED, aux);
+        uint32_t* const turn_c = reinterpret_cast<uint32_t*>(own);
+        uint32_t* const turn_z = turn_c + BlockC::WORDS;
+        auto block = [&](int cb) {
+          const int cols_left = group_cols - cb * CB;
+          if (CHUNKED) request(cb);  // the sums leave no registers to ask earlier; L2 has the block by now
+          float v[CB];
+          take(cb, v);
+          auto add_d = [&]() {
+            float add[CB];
+            d_next.to_rows(turn_c, add, lane);
+#pragma unroll
+            for (int j = 0; j < CB; ++j) v[j] = fmaf(p.beta, add[j], v[j]);
+          };
+          if constexpr (MODE == kModeGrad) {
+            if (has_d) add_d();
+            if (aux) {
+              float zz[CB];
+              z_next.to_rows(turn_z, zz, lane);
+              if (!CHUNKED && cb + 1 < BLOCKS) request(cb + 1);
+              with_act(p.act, [&](auto tag) {
+#pragma unroll
+                for (int j = 0; j < CB; ++j) v[j] *= act_slope<FAST, decltype(tag)::value>(zz[j]);
+              });
+            } else if (!CHUNKED && cb + 1 < BLOCKS) {
+              request(cb + 1);
+            }
+            if (p.partial != nullptr) {
+              if (cols_left >= CB) {
+                float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < CB; ++j) s4[j & 3] += v[j];
+                row_sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < CB; ++j) row_sum += j < cols_left ? v[j] : 0.f;
+              }
+            }
+          } else {
+            if (aux) BlockZ::store(z_ptr + static_cast<long long>(cb * CB) * p.ldz, p.ldz, rows_left, cols_left, turn_z, v, lane);
+            with_act(p.act, [&](auto tag) {
+#pragma unroll
+              for (int j = 0; j < CB; ++j) v[j] = act_value<FAST, decltype(tag)::value>(v[j]);
+            });
+            if (has_d) add_d();
+            if (!CHUNKED && cb + 1 < BLOCKS) request(cb + 1);
+          }
+          BlockC::store(c_ptr + static_cast<long long>(cb * CB) * p.ldc, p.ldc, rows_left, cols_left, turn_c, v, lane);
+          if constexpr (MODE == kModeForward && sizeof(OT) == 2 && sizeof(T) == sizeof(OT) && BN == CTAS * BM) {
+            if (p.tri && t.tm != t.tn && in_rows) {
+              // mirror image: this lane's columns are consecutive rows there
+              OT* const dst = static_cast<OT*>(p.c) + zc * p.c_stride + static_cast<long long>(row) * p.ldc + group_col0 + cb * CB;
+              uint32_t w[CB / 2];
+#pragma unroll
+              for (int q = 0; q < CB / 2; ++q) w[q] = pack2<OT>(v[2 * q], v[2 * q + 1]);
+#pragma unroll
+              for (int q = 0; q < CB / 8; ++q)
+                if (cols_left >= 8 * (q + 1))
+                  *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+            }
+          }
+        };
+        if constexpr (CHUNKED) {
+#pragma unroll
+          for (int cb = 0; cb < BLOCKS; ++cb) {
+            if (cb * CB < group_cols) block(cb);
+          }
+        } else {
+#pragma unroll 1
+          for (int cb = 0; cb * CB < group_cols && cb < BLOCKS; ++cb) block(cb);
+        }
+        end();
+      } else {
+        if (!begin()) break;
+        auto block = [&](int cb) {
+          const int cols_left = group_cols - cb * CB;
+          float v[CB];
+          take(cb, v);
+          if (!in_rows) return;
+          const long long at = cb * CB;
+          float add[CB];
+#pragma unroll
+          for (int j = 0; j < CB; ++j)
+            add[j] = (has_d && j < cols_left) ? p.beta * to_float(d_ptr[(at + j) * p.ldd + lane]) : 0.f;
+          if (grad) {
+            float zz[CB];
+#pragma unroll
+            for (int j = 0; j < CB; ++j) zz[j] = (z_in && j < cols_left) ? to_float(z_ptr[(at + j) * p.ldz + lane]) : 0.f;
+            with_act(z_in ? p.act : static_cast<int>(kActIdentity), [&](auto tag) {
+#pragma unroll
+              for (int j = 0; j < CB; ++j) v[j] = (v[j] + add[j]) * act_slope<FAST, decltype(tag)::value>(zz[j]);
+            });
+#pragma unroll
+            for (int j = 0; j < CB; ++j) row_sum += j < cols_left ? v[j] : 0.f;
           } else {
             if (z_out) {
 #pragma unroll
-              for (int j = 0; j < CB; ++j) slot_z[j * BM] = from_float<T>(v[j]);
-            }
-            if (p.act != kActIdentity) {
-#pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] = act_value<FAST>(p.act, v[j]);
-            }
-            if (has_d) {
-#pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] += p.beta * to_float(reinterpret_cast<const DT*>(slot_c)[j * BM]);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < CB; ++j) slot_c[j * BM] = from_float<OT>(v[j]);
-          fence_proxy_async();  // the TMA unit reads the buffers through the async proxy
-          group_barrier(bar_id);
-          if (elected) {
-            if (live) {
-              if (p.kind == kFusedRaggedCols && valid < CB) {
-                // the next columns belong to another group: column by column, 16-byte multiples (m is one of 8 / 4)
-                const uint32_t rows = static_cast<uint32_t>(min(BM, p.m - cta_row0));
-                for (int j = 0; j < valid; ++j) {
-                  const long long cj = col + j;
-                  bulk_store(c_ptr + cj * p.ldc + cta_row0, smem_u32(ring_c + b * SLOT) + j * BM * sizeof(OT), rows * sizeof(OT));
-                  if (z_out) bulk_store(z_ptr + cj * p.ldz + cta_row0, smem_u32(ring_z + b * SLOT) + j * BM * 2, rows * 2);
-                }
-              } else {
-                tma_store_3d(&map_c, smem_u32(ring_c + b * SLOT), cta_row0, col, zc);
-                if (z_out) tma_store_3d(&map_z, smem_u32(ring_z + b * SLOT), cta_row0, col, zc);
-              }
-            }
-            bulk_commit();
-            bulk_wait_read<2>();  // the stores of two blocks ago have left their buffers, where block + 2 lands
-            if (loads && cb + 2 < GROUP_COLS / CB && col + 2 * CB < t.col_end)
-              request(blocks_done + 2, cta_row0, col + 2 * CB, zc);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < CB; ++j) v[j] = p.alpha * __uint_as_float(r[j]) + bias;
-          if (in_rows) {
-            float old[CB];
-#pragma unroll
-            for (int j = 0; j < CB; ++j)
-              old[j] = (has_d && j < valid) ? p.beta * to_float(d_ptr[static_cast<long long>(col + j) * p.ldd + row]) : 0.f;
-            if (p.grad) {
-              float zz[CB];
-#pragma unroll
               for (int j = 0; j < CB; ++j)
-                zz[j] = (z_in && j < valid) ? to_float(z_ptr[static_cast<long long>(col + j) * p.ldz + row]) : 0.f;
-#pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] = (v[j] + old[j]) * (z_in ? act_slope<FAST>(p.act, zz[j]) : 1.f);
-            } else {
-              if (z_out) {
-#pragma unroll
-                for (int j = 0; j < CB; ++j)
-                  if (j < valid) z_ptr[static_cast<long long>(col + j) * p.ldz + row] = from_float<T>(v[j]);
-              }
-#pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] = act_value<FAST>(p.act, v[j]) + old[j];
+                if (j < cols_left) z_ptr[(at + j) * p.ldz + lane] = from_float<T>(v[j]);
             }
+            with_act(p.act, [&](auto tag) {
 #pragma unroll
-            for (int j = 0; j < CB; ++j)
-              if (j < valid) c_ptr[static_cast<long long>(col + j) * p.ldc + row] = from_float<OT>(v[j]);
+              for (int j = 0; j < CB; ++j) v[j] = act_value<FAST, decltype(tag)::value>(v[j]) + add[j];
+            });
           }
-        }
-        if (p.partial != nullptr) {
 #pragma unroll
-          for (int j = 0; j < CB; ++j) row_sum += j < valid ? v[j] : 0.f;
-        }
-        if constexpr (sizeof(OT) == 2) {
-          if (p.tri && t.tm != t.tn && in_rows) {
-            // mirror image: this thread's columns are consecutive rows there
-            OT packed[CB];
+          for (int j = 0; j < CB; ++j)
+            if (j < cols_left) c_ptr[(at + j) * p.ldc + lane] = from_float<OT>(v[j]);
+        };
+        if constexpr (CHUNKED) {
 #pragma unroll
-            for (int j = 0; j < CB; ++j) packed[j] = from_float<OT>(v[j]);
-            OT* const dst = c_ptr + static_cast<long long>(row) * p.ldc + col;
-            if (p.tma && valid == CB) {
-              reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(packed)[0];
-              reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(packed)[1];
-            } else {
-              for (int j = 0; j < valid; ++j) dst[j] = packed[j];
-            }
-          }
+          for (int cb = 0; cb < BLOCKS; ++cb)
+            if (cb * CB < group_cols) block(cb);
+        } else {
+#pragma unroll 1
+          for (int cb = 0; cb * CB < group_cols && cb < BLOCKS; ++cb) block(cb);
         }
-        ++blocks_done;
+        end();
       }
-      if (!ok) break;
-      if (p.partial != nullptr && in_rows)
+      if (MODE != kModeForward && p.partial != nullptr && in_rows)
         p.partial[(static_cast<long long>(t.col_tile) * EG + group) * p.m + row] = row_sum;
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CTAS == 2) mbar_arrive_remote(map_to_cta(acc_empty_bar(acc), 0));
-        else mbar_arrive(acc_empty_bar(acc));
-      }
     }
-    if (elected) bulk_wait_all();  // shared memory stays valid until the last store has read it
   }
 
   tcgen05_fence_before();
   __syncthreads();
-  if (CTAS == 2 || p.split > 1) cluster_sync_all();  // nobody exits while a peer may still signal or read
+  if (CTAS == 2 || split > 1) cluster_sync_all();  // nobody exits while a peer may still signal or read
   if (warp == 1) {
     tcgen05_fence_after();
     if constexpr (CTAS == 2) tmem_dealloc_pair(tmem_base, TMEM_COLS);
@@ -652,14 +972,14 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   }
 }
 
-template <int CTAS, int BN, class T, class DT, class OT>
-cudaError_t launch_typed(const CUtensorMap* maps, const FusedParams& p, int grid, int smem, cudaStream_t stream) {
-  auto kernel = fused_gemm_kernel<CTAS, BN, T, DT, OT>;
+template <int CTAS, int BN, class T, class DT, class OT, int MODE>
+cudaError_t launch_mode(const CUtensorMap* maps, const FusedParams& p, int grid, int smem, cudaStream_t stream) {
+  auto kernel = fused_gemm_kernel<CTAS, BN, T, DT, OT, MODE>;
   const cudaError_t e = kernel_ready(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-  cfg.blockDim = dim3(64 + 128 * (BN >= 128 ? 2 : 1), 1, 1);
+  cfg.blockDim = dim3(fused_threads(BN), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -672,17 +992,26 @@ cudaError_t launch_typed(const CUtensorMap* maps, const FusedParams& p, int grid
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], maps[4], p);
+  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], p);
+}
+
+template <int CTAS, int BN, class T, class DT, class OT>
+cudaError_t launch_typed(const CUtensorMap* maps, const FusedParams& p, int grid, int smem, cudaStream_t stream) {
+  if (!p.vec || p.split > 1) return launch_mode<CTAS, BN, T, DT, OT, kModeGeneral>(maps, p, grid, smem, stream);
+  if (!p.grad) return launch_mode<CTAS, BN, T, DT, OT, kModeForward>(maps, p, grid, smem, stream);
+  // gradients are stored in the operands' type
+  if constexpr (std::is_same<T, OT>::value) return launch_mode<CTAS, BN, T, DT, OT, kModeGrad>(maps, p, grid, smem, stream);
+  return cudaErrorInvalidValue;
 }
 
 // Clusters of `cluster` CTAs that the device holds at once (one CTA per SM; a cluster sits in one GPC).
 template <int CTAS, int BN>
 int resident_clusters(int cluster, int smem) {
-  auto kernel = fused_gemm_kernel<CTAS, BN, __half, __half, __half>;
+  auto kernel = fused_gemm_kernel<CTAS, BN, __half, __half, __half, kModeGeneral>;
   if (kernel_ready(reinterpret_cast<const void*>(kernel), smem) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / cluster * cluster), 1, 1);
-  cfg.blockDim = dim3(64 + 128 * (BN >= 128 ? 2 : 1), 1, 1);
+  cfg.blockDim = dim3(fused_threads(BN), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -707,10 +1036,12 @@ cudaError_t launch_by_type(int type, int d_type, int c_type, const CUtensorMap* 
   if (type == 16) {
     if (c_type == 16 && d_type == 16) return launch_typed<CTAS, BN, H, H, H>(maps, p, grid, smem, stream);
     if (c_type == kBFloat16 && d_type == 16) return launch_typed<CTAS, BN, H, H, B>(maps, p, grid, smem, stream);
-    if (c_type == 32 && d_type == 32) return launch_typed<CTAS, BN, H, float, float>(maps, p, grid, smem, stream);
+    if constexpr (BN <= 128)  // half as fast on 256 columns, where the sums spill
+      if (c_type == 32 && d_type == 32) return launch_typed<CTAS, BN, H, float, float>(maps, p, grid, smem, stream);
   } else if (type == kBFloat16) {
     if (c_type == kBFloat16 && d_type == kBFloat16) return launch_typed<CTAS, BN, B, B, B>(maps, p, grid, smem, stream);
-    if (c_type == 32 && d_type == 32) return launch_typed<CTAS, BN, B, float, float>(maps, p, grid, smem, stream);
+    if constexpr (BN <= 128)  // half as fast on 256 columns, where the sums spill
+      if (c_type == 32 && d_type == 32) return launch_typed<CTAS, BN, B, float, float>(maps, p, grid, smem, stream);
   }
   return cudaErrorInvalidValue;
 }

@@ -42,7 +42,8 @@ struct FusedParams {
   const void* d;              // null without residual
   void* z;                    // written (grad == 0) or read; null without
   long long ldc, ldd, ldz, c_stride, d_stride, z_stride;
-  int tma;                    // C, D and Z travel by TMA
+  int vec;                    // C, D and Z: bases, leading dimensions and strides are multiples of 16 bytes
+  int prefetch;               // D and Z have tensor maps and are asked for ahead
   float* partial;             // row sums of C per column tile (bias gradient), or null
   int hint_a, hint_b;
 };
@@ -52,11 +53,27 @@ struct FusedVariant {
   int ctas;           // CTAs per tile: 2 for the pair kernel
   int bn;             // columns per tile; rows are 128 * ctas
   int stage_bytes;
-  int epi_groups;     // epilogue groups of four warps
 };
-constexpr int kFusedVariants = 5;
+// Epilogue groups of four warps that share a tile's columns, next to four warps with other roles.
+#ifdef __CUDACC__
+#define B200_HD __host__ __device__
+#else
+#define B200_HD
+#endif
+B200_HD constexpr int fused_groups(int bn) { return bn >= 128 ? 2 : 1; }
+B200_HD constexpr int fused_threads(int bn) { return 128 + 128 * fused_groups(bn); }
+// Columns of an epilogue block (of 32 rows), and an epilogue warp's shared memory: a block of C or D and one of Z.
+B200_HD constexpr int fused_block_cols(bool single) { return single ? 16 : 32; }
+B200_HD constexpr int fused_warp_bytes(bool single, bool aux) { return 2048 + (aux ? fused_block_cols(single) * 64 : 0); }
+// Shared memory behind the operand ring: the epilogue warps', or the fp32 sums of a split tile; then barriers, then the
+// group table.
+B200_HD constexpr int fused_staging_bytes(int bn, bool single, bool aux, int split) {
+  return split > 1 ? bn * 512 : 4 * fused_groups(bn) * fused_warp_bytes(single, aux);
+}
+constexpr int kFusedBarBytes = 512;
+constexpr int kFusedVariants = 6;
 constexpr FusedVariant kFusedTable[kFusedVariants] = {
-    {2, 256, 32768, 2}, {1, 256, 49152, 2}, {1, 128, 32768, 2}, {1, 64, 24576, 1}, {1, 32, 20480, 1}};
+    {2, 256, 32768}, {1, 256, 49152}, {1, 128, 32768}, {1, 64, 24576}, {1, 32, 20480}, {2, 128, 24576}};
 
 // Enqueues variant `v` with operand type / D type / C type. `grid` counts CTAs, `smem` bytes of dynamic shared memory.
 cudaError_t launch_fused_variant(int v, int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p,
@@ -66,6 +83,8 @@ cudaError_t launch_fused_variant(int v, int type, int d_type, int c_type, const 
 int fused_resident_clusters(int cluster);
 cudaError_t launch_fused_pair(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,
                               int smem, cudaStream_t stream);
+cudaError_t launch_fused_pair128(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,
+                                 int smem, cudaStream_t stream);
 cudaError_t launch_fused_256(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,
                              int smem, cudaStream_t stream);
 cudaError_t launch_fused_128(int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p, int grid,

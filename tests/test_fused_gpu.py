@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 ROW, COL, NO, YES = 101, 102, 111, 112
 OK = cb.StatusCode.kSuccess
-VARIANTS = ["0", "1", "2", "3", "4", "2,2", "2,4", "3,2", "3,8", "4,2", "4,8", "1,2"]
+VARIANTS = ["0", "1", "2", "3", "4", "5", "2,2", "2,4", "3,2", "3,8", "4,2", "4,8", "1,2"]
 
 
 def force(monkeypatch, v):
@@ -172,7 +172,7 @@ def test_in_place(cuda, monkeypatch, v):
         linear(cuda, monkeypatch, v, name, name, ROW, NO, YES, 300, 392, 256, act=163, beta=1.0, inplace="d", grad=True)
 
 
-@pytest.mark.parametrize("v", ["0", "1", "2", "3", "4"])
+@pytest.mark.parametrize("v", ["0", "1", "2", "3", "4", "5"])
 def test_many_tiles_per_cta(cuda, monkeypatch, v):
     """More tiles than SMs: both accumulators, the operand ring and the staging rings go round several times."""
     linear(cuda, monkeypatch, v, "bf16", "bf16", ROW, NO, YES, 3000, 4104, 136, act=165, beta=1.0)
@@ -269,7 +269,7 @@ SIZES = [([5], 5), ([0], 4), ([0, 0, 7, 0], 7), ([1, 1, 1, 1, 1], 5), ([3, 0, 64
 
 
 @pytest.mark.parametrize("sizes,rows", SIZES)
-@pytest.mark.parametrize("v", [None, "0", "1", "2", "3", "4", "4,8", "2,2"])
+@pytest.mark.parametrize("v", [None, "0", "1", "2", "3", "4", "5", "4,8", "2,2"])
 def test_groups(cuda, monkeypatch, sizes, rows, v):
     grouped(cuda, monkeypatch, v, "bf16", "bf16", sizes, rows, 264, 200, act=165, beta=1.0)
     grouped(cuda, monkeypatch, v, "half", "half", sizes, rows, 264, 200, act=163, beta=1.0, grad=True)
@@ -358,11 +358,19 @@ def weight(torch, monkeypatch, v, name, c_name, sizes, rows, m, n, *, first=0, a
 
 
 @pytest.mark.parametrize("sizes,rows", SIZES)
-@pytest.mark.parametrize("v", [None, "1", "2", "3", "2,2", "3,4"])
+@pytest.mark.parametrize("v", [None, "0", "1", "2", "3", "5", "2,2", "3,4"])
 def test_weight_gradients(cuda, monkeypatch, sizes, rows, v):
     weight(cuda, monkeypatch, v, "bf16", "single", sizes, rows, 136, 264, beta=1.0)
     weight(cuda, monkeypatch, v, "half", "half", sizes, rows, 136, 264)
     weight(cuda, monkeypatch, v, "bf16", "single", sizes, rows + 20, 64, 128, first=11, poison=True, alpha=-2.0)
+
+
+@pytest.mark.parametrize("v", ["0", "1", "2", "3", "5", "3,2"])
+def test_weight_gradients_of_many_short_groups(cuda, monkeypatch, v):
+    """Many tiles per CTA, each with a cut-off last block: several of them are in the operand ring at once."""
+    sizes = [(13 * i) % 131 for i in range(40)]
+    weight(cuda, monkeypatch, v, "bf16", "bf16", sizes, sum(sizes), 520, 776)
+    weight(cuda, monkeypatch, v, "half", "single", sizes, sum(sizes) + 5, 520, 776, first=5, poison=True, beta=1.0)
 
 
 @pytest.mark.parametrize("m,n,pad", [(1, 1, 0), (8, 8, 8), (65, 127, 0), (129, 257, 3), (200, 333, 1)])
