@@ -9,6 +9,7 @@
 
 #include "driver_api.h"
 #include "kernels/fused_aux.h"
+#include "kernels/fused_rows.h"
 #include "kernels/launchers.h"
 #include "runtime_state.h"
 #include "scratch.h"
@@ -59,7 +60,6 @@ bool variant_fits(const FusedDesc& d, int v, int split) {
   const FusedVariant& t = kFusedTable[v];
   if (t.ctas == 2 && split > 1) return false;
   if (d.b_mn && t.bn / t.ctas < 64) return false;                               // a 128-byte row is 64 columns
-  if (d.c_type == 32 && t.bn > 128) return false;                               // the epilogue's sums fill the registers
   if (d.tri && t.ctas * 128 != t.bn) return false;                               // square tiles meet their mirror image
   if (split > 1 && (t.bn / split) % 4 != 0) return false;
   if (split > 1 && d.tri) return false;
@@ -101,6 +101,17 @@ double estimate(const FusedDesc& d, int v, int split) {
   return waves * (inner * per_block + 400.0) + drain + 1500.0;
 }
 
+// B200BLAS_FUSED=<variant>[,<split>] forces one for measurements and tests where it can serve the call.
+bool forced_variant(int* variant, int* split) {
+  const char* const env = std::getenv("B200BLAS_FUSED");
+  if (env == nullptr) return false;
+  int v = -1, s = 1;
+  if (std::sscanf(env, "%d,%d", &v, &s) < 1 || v < 0 || v >= kFusedVariants || s < 1 || s > 8 || (s & (s - 1)) != 0) return false;
+  if (variant) *variant = v;
+  if (split) *split = s;
+  return true;
+}
+
 Choice choose(const FusedDesc& d) {
   Choice best = {2, 1};
   double best_time = 1e300;
@@ -114,13 +125,8 @@ Choice choose(const FusedDesc& d) {
       }
     }
   }
-  // B200BLAS_FUSED=<variant>[,<split>] forces one for measurements and tests where it can serve the call.
-  if (const char* env = std::getenv("B200BLAS_FUSED")) {
-    int v = -1, split = 1;
-    if (std::sscanf(env, "%d,%d", &v, &split) >= 1 && v >= 0 && v < kFusedVariants && split >= 1 && split <= 8 &&
-        (split & (split - 1)) == 0 && variant_fits(d, v, split))
-      best = {v, split};
-  }
+  int v, split;
+  if (forced_variant(&v, &split) && variant_fits(d, v, split)) best = {v, split};
   return best;
 }
 
@@ -131,6 +137,20 @@ bool unaddressable(const void* base, long long ld, long long planes, long long s
 }  // namespace
 
 cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** name) {
+  // A handful of vectors and a matrix whose rows are read along the inner extent. The bias gradient is a sum over the
+  // vectors: those calls stay with the kernels that leave partial sums.
+  if (d.kind == kFusedPlain && d.problems == 1 && !d.tri && d.n <= kFewRows && !d.a_mn && !d.b_mn && !d.bias_grad &&
+      d.c_type == d.d_type && !unaddressable(d.a, d.lda, 1, 0) && !forced_variant(nullptr, nullptr)) {
+    FewRowsJob job = {};
+    job.type = d.type; job.c_type = d.c_type;
+    job.m = static_cast<int>(d.m); job.n = static_cast<int>(d.n); job.k = static_cast<int>(d.k);
+    job.w = d.a; job.ldw = d.lda; job.x = d.b; job.ldx = d.ldb;
+    job.alpha = static_cast<float>(d.alpha); job.beta = static_cast<float>(d.beta);
+    job.bias = d.bias; job.act = d.act; job.grad = d.grad;
+    job.d = d.beta != 0.0 ? d.d : nullptr; job.ldd = d.ldd; job.z = d.z; job.ldz = d.ldz; job.c = d.c; job.ldc = d.ldc;
+    *name = "fused_few_rows";
+    return launch_few_rows(job, stream);
+  }
   // an operand with stride 0 is shared by all problems
   const long long a_planes = d.kind == kFusedRaggedInner || d.a_stride == 0 ? 1 : d.problems;
   const long long b_planes = d.kind == kFusedPlain && d.b_stride != 0 ? d.problems : 1;
@@ -224,7 +244,7 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   }
 
   // shared memory: the ring takes what staging, barriers and the group table leave
-  const int table = d.kind == kFusedRaggedCols ? 8 * (p.problems + 1) : 0;
+  const int table = d.kind != kFusedPlain ? 8 * (p.problems + 1) : 0;
   const int fixed = kAlign + fused_staging_bytes(t.bn, single, p.z != nullptr, choice.split) + kFusedBarBytes + table;
   int stages = (kMaxSmem - fixed) / t.stage_bytes;
   if (stages > 12) stages = 12;

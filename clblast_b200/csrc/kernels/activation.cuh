@@ -33,13 +33,13 @@ __device__ __forceinline__ float rcp_fast(float x) {
 constexpr float kLog2E = 1.4426950408889634f;
 
 // s(x) = 1 / (1 + exp(-x)) and, for slopes, 1 - s(x) = exp(-x) s(x), which the subtraction would leave with an absolute
-// error of s's last place. x is held above -80, so that the exponential stays finite (a NaN passes).
+// error of s's last place. The argument is -x log2(e) for FAST, else -x. An exponential beyond the range makes s zero;
+// the other factor is held finite there, so that their product is zero too (a NaN passes through s).
 template <bool FAST>
-__device__ __forceinline__ float logistic(float x, float* complement = nullptr) {
-  const float xc = x < -80.f ? -80.f : x;
-  const float e = FAST ? exp2_fast(-kLog2E * xc) : expf(-xc);
+__device__ __forceinline__ float logistic(float minus_x, float* complement = nullptr) {
+  const float e = FAST ? exp2_fast(minus_x) : expf(minus_x);
   const float s = FAST ? rcp_fast(1.f + e) : 1.f / (1.f + e);
-  if (complement) *complement = e * s;
+  if (complement) *complement = fminf(e, 3.0e38f) * s;
   return s;
 }
 
@@ -66,42 +66,47 @@ __device__ __forceinline__ float normal_cdf(float z, float* bell = nullptr) {
   return 0.5f * erfcf(z * -0.70710678118654752f);
 }
 
-__device__ __forceinline__ float gelu_tanh_arg(float z) {  // 2u
-  constexpr float k2 = 1.5957691216057308f;  // 2 sqrt(2/pi)
-  return k2 * z * fmaf(0.044715f * z, z, 1.f);
+// -2u, times log2(e) for FAST
+template <bool FAST>
+__device__ __forceinline__ float gelu_tanh_arg(float z) {
+  constexpr float k = -1.5957691216057308f * (FAST ? kLog2E : 1.f);  // 2 sqrt(2/pi)
+  return z * fmaf(k * 0.044715f, z * z, k);
 }
+template <bool FAST>
+__device__ __forceinline__ float silu_arg(float z) { return FAST ? -kLog2E * z : -z; }
 
 template <bool FAST, int ACT>
 __device__ __forceinline__ float act_value(float z) {
   switch (ACT) {
     case kActRelu: return z < 0.f ? 0.f : z;
     case kActGelu: return fmaxf(z, -60.f) * normal_cdf<FAST>(z);
-    case kActGeluTanh: return fmaxf(z, -60.f) * logistic<FAST>(gelu_tanh_arg(z));
-    case kActSilu: return fmaxf(z, -80.f) * logistic<FAST>(z);
+    case kActGeluTanh: return fmaxf(z, -60.f) * logistic<FAST>(gelu_tanh_arg<FAST>(z));
+    case kActSilu: return fmaxf(z, -200.f) * logistic<FAST>(silu_arg<FAST>(z));
     default: return z;
   }
 }
 
 template <bool FAST, int ACT>
 __device__ __forceinline__ float act_slope(float z) {
-  const float zc = fminf(fmaxf(z, -60.f), 60.f);
   switch (ACT) {
     case kActRelu: return z > 0.f ? 1.f : (z != z ? z : 0.f);
     case kActGelu: {
       float e;
       const float cdf = normal_cdf<FAST>(z, &e);
+      const float zc = fminf(fmaxf(z, -60.f), 60.f);
       return fmaf(zc * 0.3989422804014327f, e, cdf);
     }
     case kActGeluTanh: {
       float rest;
-      const float s = logistic<FAST>(gelu_tanh_arg(z), &rest);
+      const float s = logistic<FAST>(gelu_tanh_arg<FAST>(z), &rest);
+      const float zc = fminf(fmaxf(z, -60.f), 60.f);
       constexpr float k2 = 1.5957691216057308f;
-      return fmaf(zc * s * rest, fmaf(k2 * 3.f * 0.044715f * zc, zc, k2), s);
+      return fmaf(zc * fmaf(k2 * 3.f * 0.044715f, zc * zc, k2), s * rest, s);
     }
     case kActSilu: {
       float rest;
-      const float s = logistic<FAST>(z, &rest);
-      return s * fmaf(fminf(fmaxf(z, -80.f), 200.f), rest, 1.f);
+      const float s = logistic<FAST>(silu_arg<FAST>(z), &rest);
+      return fmaf(fminf(fmaxf(z, -200.f), 200.f) * rest, s, s);
     }
     default: return 1.f;
   }

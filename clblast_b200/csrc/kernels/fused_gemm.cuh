@@ -24,7 +24,8 @@
 //
 // Sums for results in single precision: the tensor cores cut off instead of rounding when they add to an accumulator, an
 // error of about 4e-8 of the result per 16 inner elements that all points towards zero. Results in 16 bits do not see it.
-// For the others an accumulator takes kChunk blocks at most and is then added, rounded, to fp32 registers.
+// For the others an accumulator takes kChunk blocks at most and is then added, rounded, to sums in further columns of
+// tensor memory (which the widest tile has room for only with one accumulator instead of two).
 //
 // All waits are bounded; on expiry a code is left in the status word and every role leaves its loop.
 #pragma once
@@ -173,19 +174,7 @@ struct BlockOf { using type = Block16<E, COLS>; };
 template <int COLS>
 struct BlockOf<float, COLS> { using type = Block32<COLS>; };
 
-// Starts the load of 32 or 16 accumulator columns; the values may be used after tmem_wait.
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
+// Starts the load of 16 accumulator columns; the values may be used after tmem_wait.
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -195,18 +184,20 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 // The registers are operands, so that no use of them moves above the wait.
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
-}
 __device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                  "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
+
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tma_load_3d_hint(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z,
                                                  uint64_t policy) {
@@ -335,11 +326,8 @@ __device__ __forceinline__ Tile locate(const FusedParams& p, int tile, const int
     t.col0 = t.tn * BN;
     t.col_end = p.n;
     if (p.kind == kFusedRaggedInner) {
-      long long lo = p.offsets[t.z], hi = p.offsets[t.z + 1];
-      lo = lo < 0 ? 0 : (lo > p.k ? p.k : lo);
-      hi = hi < lo ? lo : (hi > p.k ? p.k : hi);
-      t.k0 = static_cast<int>(lo);
-      t.k_len = static_cast<int>(hi - lo);
+      t.k0 = start[t.z];
+      t.k_len = start[t.z + 1] - t.k0;
     }
   }
   return t;
@@ -357,12 +345,15 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   static_assert(sizeof(DT) == sizeof(OT), "D and C share the staging buffers");
   constexpr bool CHUNKED = sizeof(OT) == 4;
   constexpr int EG = fused_groups(BN);
-  constexpr int CB = fused_block_cols(CHUNKED);  // columns per epilogue block
+  constexpr int CB = 16;  // columns per epilogue block
   constexpr int B_ROWS = BN / CTAS;
   constexpr int A_BYTES = BM * BK * 2;
   constexpr int STAGE_BYTES = A_BYTES + B_ROWS * BK * 2;
   constexpr int GROUP_COLS = BN / EG;
-  constexpr uint32_t TMEM_COLS = 2 * BN;
+  // accumulators, then the sums of results in single precision; a power of two
+  constexpr int ACCS = (CHUNKED && BN == 256) ? 1 : 2;
+  constexpr uint32_t SUMS_AT = ACCS * BN;
+  constexpr uint32_t TMEM_COLS = CHUNKED ? (BN == 256 ? 512 : 4 * BN) : 2 * BN;
   constexpr bool FAST = sizeof(OT) == 2;
 
   extern __shared__ uint8_t smem_raw[];
@@ -418,13 +409,18 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     if constexpr (CTAS == 2) tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
     else tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
   }
-  if (warp == 2 && p.kind == kFusedRaggedCols) build_table(p.offsets, p.problems, p.n, BN, start, tiles);
+  if (warp == 2 && p.kind != kFusedPlain)
+    build_table(p.offsets, p.problems, p.kind == kFusedRaggedCols ? p.n : p.k, BN, start, tiles);
   tcgen05_fence_before();
   __syncthreads();
   if (CTAS == 2 || split > 1) cluster_sync_all();  // all barriers exist before anyone signals across CTAs
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int num_tiles = total_tiles(p, tiles);
+
+  // accumulator number n of this CTA: which one, and the parity of its use
+  auto acc_of = [](int n) { return ACCS == 1 ? 0 : (n & 1); };
+  auto acc_parity = [](int n) { return static_cast<uint32_t>(ACCS == 1 ? n : (n >> 1)) & 1u; };
 
   // this CTA's share of a tile's inner blocks
   auto k_range = [&](const Tile& t, int& kb0, int& kb1) {
@@ -556,8 +552,8 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         const Tile t = locate<BN>(p, tile, start, tiles);
         int kb0, kb1;
         k_range(t, kb0, kb1);
-        int acc = local & 1;
-        ok = wait(acc_empty_bar(acc), ((local >> 1) & 1u) ^ 1u, 2u);
+        int acc = acc_of(local);
+        ok = wait(acc_empty_bar(acc), acc_parity(local) ^ 1u, 2u);
         if (!ok) break;
         tcgen05_fence_after();
         uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
@@ -568,8 +564,8 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             __syncwarp();
             ++local;
             first_kb = kb;
-            acc = local & 1;
-            ok = wait(acc_empty_bar(acc), ((local >> 1) & 1u) ^ 1u, 2u);
+            acc = acc_of(local);
+            ok = wait(acc_empty_bar(acc), acc_parity(local) ^ 1u, 2u);
             if (!ok) break;
             tcgen05_fence_after();
             d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
@@ -666,46 +662,53 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       k_range(t, kb0, kb1);
       const bool empty = kb1 <= kb0;
       auto accumulator = [&](int number) {
-        return tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>((number & 1) * BN + group * GROUP_COLS);
+        return tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc_of(number) * BN + group * GROUP_COLS);
       };
       auto wait_accumulator = [&](int number) {
-        return warp_wait(acc_full_bar(number & 1), (number >> 1) & 1u, abort_flag, 4u, p.status);
+        return warp_wait(acc_full_bar(acc_of(number)), acc_parity(number), abort_flag, 4u, p.status);
       };
       auto release_accumulator = [&](int number) {
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (CTAS == 2) mbar_arrive_peer(map_to_cta(acc_empty_bar(number & 1), 0));
-          else mbar_arrive(acc_empty_bar(number & 1));
+          if constexpr (CTAS == 2) mbar_arrive_peer(map_to_cta(acc_empty_bar(acc_of(number)), 0));
+          else mbar_arrive(acc_empty_bar(acc_of(number)));
         }
       };
 
-      // results in single precision: all partial sums of this warp's columns, in registers
-      float sum[CHUNKED ? GROUP_COLS : 1];
+      // Results in single precision: the accumulators are added up in further columns, which only this warp touches.
+      const uint32_t sums_tmem = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + SUMS_AT + static_cast<uint32_t>(group * GROUP_COLS);
       if constexpr (CHUNKED) {
         const int chunks = empty ? 1 : (kb1 - kb0 + kChunk - 1) / kChunk;
         for (int c = 0; c < chunks; ++c) {
           ok = wait_accumulator(local);
           if (!ok) break;
           tcgen05_fence_after();
+          if (!empty) {
 #pragma unroll
-          for (int cb = 0; cb < BLOCKS; ++cb) {
-            uint32_t r[CB];
-            if (empty) {
-#pragma unroll
-              for (int j = 0; j < CB; ++j) sum[cb * CB + j] = 0.f;
-            } else {
+            for (int cb = 0; cb < BLOCKS; ++cb) {
+              uint32_t r[CB];
               tmem_ld(accumulator(local) + cb * CB, r);
-              tmem_wait(r);
+              if (c == 0) {
+                tmem_wait(r);
+              } else {
+                uint32_t s[CB];
+                tmem_ld(sums_tmem + cb * CB, s);
+                tmem_wait(r);
+                tmem_wait(s);
 #pragma unroll
-              for (int j = 0; j < CB; ++j) sum[cb * CB + j] = c == 0 ? __uint_as_float(r[j]) : sum[cb * CB + j] + __uint_as_float(r[j]);
+                for (int j = 0; j < CB; ++j) r[j] = __float_as_uint(__uint_as_float(s[j]) + __uint_as_float(r[j]));
+              }
+              tmem_st(sums_tmem + cb * CB, r);
             }
+            tmem_st_wait();
           }
           release_accumulator(local);
           ++local;
         }
         if (!ok) break;
       }
+      const uint32_t values = CHUNKED ? sums_tmem : accumulator(local);  // where the finished values lie
 
       if constexpr (MODE == kModeGeneral) {
         if (split > 1) {
@@ -723,18 +726,13 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 #pragma unroll
           for (int cb = 0; cb < BLOCKS; ++cb) {
             const int col = group * GROUP_COLS + cb * CB;
-            if constexpr (CHUNKED) {
-#pragma unroll
-              for (int j = 0; j < CB; ++j) sums[(col + j) * BM + row_in_cta] = sum[cb * CB + j];
-            } else {
-              uint32_t r[CB];
-              if (!empty) {
-                tmem_ld(accumulator(local) + cb * CB, r);
-                tmem_wait(r);
-              }
-#pragma unroll
-              for (int j = 0; j < CB; ++j) sums[(col + j) * BM + row_in_cta] = empty ? 0.f : __uint_as_float(r[j]);
+            uint32_t r[CB];
+            if (!empty) {
+              tmem_ld(values + cb * CB, r);
+              tmem_wait(r);
             }
+#pragma unroll
+            for (int j = 0; j < CB; ++j) sums[(col + j) * BM + row_in_cta] = empty ? 0.f : __uint_as_float(r[j]);
           }
           if constexpr (!CHUNKED) {
             release_accumulator(local);
@@ -744,35 +742,62 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           if (lane == 0) {
             for (int q = 0; q < split; ++q) mbar_arrive_remote(map_to_cta(sums_ready, q));
           }
+          const int mine = BN / split;  // columns per CTA, a multiple of four
+          const int first_col = static_cast<int>(rank) * mine;
+          // D and Z of four columns; those of the next four are under way while four are finished
+          float d4[4], z4[4], d_ahead[4], z_ahead[4];
+          auto fetch = [&](int q, float (&d)[4], float (&z)[4]) {
+            const int rel = first_col + q * 4 - group * GROUP_COLS;
+            const int cols_left = t.col_end - (t.col0 + first_col + q * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool in = in_rows && j < cols_left;
+              d[j] = has_d && in ? to_float(d_ptr[static_cast<long long>(rel + j) * p.ldd + lane]) : 0.f;
+              z[j] = z_in && in ? to_float(z_ptr[static_cast<long long>(rel + j) * p.ldz + lane]) : 0.f;
+            }
+          };
+          fetch(group, d_ahead, z_ahead);
           ok = warp_wait_cluster(sums_ready, tiles_done & 1u, abort_flag, 8u, p.status);
           if (!ok) break;
-          const int mine = BN / split;  // a multiple of four
           for (int q = group; q < mine / 4; q += EG) {
-            const int in_tile = static_cast<int>(rank) * mine + q * 4;
+            const int in_tile = first_col + q * 4;
             const int rel = in_tile - group * GROUP_COLS;  // column relative to group_col0
             const int cols_left = t.col_end - (t.col0 + in_tile);
             if (cols_left <= 0) break;
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int s = 0; s < split; ++s) {
-              const uint32_t src = map_to_cta(smem_u32(sums + in_tile * BM + row_in_cta), s);
+            float part[8][4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) v[j] += ld_cluster_f32(src + j * BM * 4);
+            for (int s = 0; s < 8; ++s) {
+              if (s < split) {
+                const uint32_t src = map_to_cta(smem_u32(sums + in_tile * BM + row_in_cta), s);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part[s][j] = ld_cluster_f32(src + j * BM * 4);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part[s][j] = 0.f;
+              }
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { d4[j] = d_ahead[j]; z4[j] = z_ahead[j]; }
+            if (q + EG < mine / 4) fetch(q + EG, d_ahead, z_ahead);
             with_act(p.act, [&](auto tag) {
               constexpr int ACT = decltype(tag)::value;
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
+                float v = part[0][j];
+#pragma unroll
+                for (int s = 1; s < 8; ++s) v += part[s][j];
                 if (!in_rows || j >= cols_left) continue;
                 const long long cj = rel + j;
-                const float add = has_d ? p.beta * to_float(d_ptr[cj * p.ldd + lane]) : 0.f;
-                float y = p.alpha * v[j] + bias;
+                const float add = p.beta * d4[j];
+                float y = fmaf(p.alpha, v, bias);
                 if (grad) {
-                  y += add;
-                  if (z_in) y *= act_slope<FAST, ACT>(to_float(z_ptr[cj * p.ldz + lane]));
+                  if (has_d) y += add;
+                  if (z_in) y *= act_slope<FAST, ACT>(z4[j]);
                   row_sum += y;
                 } else {
                   if (z_out) z_ptr[cj * p.ldz + lane] = from_float<T>(y);
-                  y = act_value<FAST, ACT>(y) + add;
+                  y = act_value<FAST, ACT>(y);
+                  if (has_d) y += add;
                 }
                 c_ptr[cj * p.ldc + lane] = from_float<OT>(y);
               }
@@ -791,38 +816,28 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       // accumulator values of block cb; the load of the next block starts as this one's arrives
       uint32_t r_next[CB];
       auto take = [&](int cb, float (&v)[CB]) {
-        if constexpr (CHUNKED) {
+        if (empty) {
 #pragma unroll
-          for (int i = 0; i < BLOCKS; ++i) {
-            if (i == cb) {
-#pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] = sum[i * CB + j];
-            }
-          }
-        } else if (empty) {
-#pragma unroll
-          for (int j = 0; j < CB; ++j) v[j] = 0.f;
+          for (int j = 0; j < CB; ++j) v[j] = bias;
         } else {
           tmem_wait(r_next);
 #pragma unroll
-          for (int j = 0; j < CB; ++j) v[j] = __uint_as_float(r_next[j]);
-          if (cb + 1 < BLOCKS) tmem_ld(accumulator(local) + (cb + 1) * CB, r_next);
+          for (int j = 0; j < CB; ++j) v[j] = fmaf(p.alpha, __uint_as_float(r_next[j]), bias);
+          if (cb + 1 < BLOCKS) tmem_ld(values + (cb + 1) * CB, r_next);
         }
-#pragma unroll
-        for (int j = 0; j < CB; ++j) v[j] = fmaf(p.alpha, v[j], bias);
       };
       auto begin = [&]() {
         if constexpr (!CHUNKED) {
           ok = wait_accumulator(local);
           if (!ok) return false;
           tcgen05_fence_after();
-          if (!empty) tmem_ld(accumulator(local), r_next);
         }
+        if (!empty) tmem_ld(values, r_next);
         return true;
       };
       auto end = [&]() {
+        if (!empty) tmem_wait(r_next);  // a load may have started for a block that does not exist
         if constexpr (!CHUNKED) {
-          if (!empty) tmem_wait(r_next);  // a load may have started for a block that does not exist
           release_accumulator(local);
           ++local;
         }
@@ -836,14 +851,13 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           if (has_d) d_next.load(d_ptr + static_cast<long long>(cb * CB) * p.ldd, p.ldd, rows_left, group_cols - cb * CB, lane);
           if (MODE == kModeGrad && aux) z_next.load(z_ptr + static_cast<long long>(cb * CB) * p.ldz, p.ldz, rows_left, group_cols - cb * CB, lane);
         };
-        if (!CHUNKED) request(0);
+        request(0);
         if (!begin()) break;
         uint8_t* const own = staging + (warp - 4) * fused_warp_bytes(CHUNKED, aux);
         uint32_t* const turn_c = reinterpret_cast<uint32_t*>(own);
         uint32_t* const turn_z = turn_c + BlockC::WORDS;
         auto block = [&](int cb) {
           const int cols_left = group_cols - cb * CB;
-          if (CHUNKED) request(cb);  // the sums leave no registers to ask earlier; L2 has the block by now
           float v[CB];
           take(cb, v);
           auto add_d = [&]() {
@@ -857,12 +871,12 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             if (aux) {
               float zz[CB];
               z_next.to_rows(turn_z, zz, lane);
-              if (!CHUNKED && cb + 1 < BLOCKS) request(cb + 1);
+              if (cb + 1 < BLOCKS) request(cb + 1);
               with_act(p.act, [&](auto tag) {
 #pragma unroll
                 for (int j = 0; j < CB; ++j) v[j] *= act_slope<FAST, decltype(tag)::value>(zz[j]);
               });
-            } else if (!CHUNKED && cb + 1 < BLOCKS) {
+            } else if (cb + 1 < BLOCKS) {
               request(cb + 1);
             }
             if (p.partial != nullptr) {
@@ -883,7 +897,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
               for (int j = 0; j < CB; ++j) v[j] = act_value<FAST, decltype(tag)::value>(v[j]);
             });
             if (has_d) add_d();
-            if (!CHUNKED && cb + 1 < BLOCKS) request(cb + 1);
+            if (cb + 1 < BLOCKS) request(cb + 1);
           }
           BlockC::store(c_ptr + static_cast<long long>(cb * CB) * p.ldc, p.ldc, rows_left, cols_left, turn_c, v, lane);
           if constexpr (MODE == kModeForward && sizeof(OT) == 2 && sizeof(T) == sizeof(OT) && BN == CTAS * BM) {
@@ -900,15 +914,8 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
           }
         };
-        if constexpr (CHUNKED) {
-#pragma unroll
-          for (int cb = 0; cb < BLOCKS; ++cb) {
-            if (cb * CB < group_cols) block(cb);
-          }
-        } else {
 #pragma unroll 1
-          for (int cb = 0; cb * CB < group_cols && cb < BLOCKS; ++cb) block(cb);
-        }
+        for (int cb = 0; cb * CB < group_cols && cb < BLOCKS; ++cb) block(cb);
         end();
       } else {
         if (!begin()) break;
@@ -947,14 +954,8 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           for (int j = 0; j < CB; ++j)
             if (j < cols_left) c_ptr[(at + j) * p.ldc + lane] = from_float<OT>(v[j]);
         };
-        if constexpr (CHUNKED) {
-#pragma unroll
-          for (int cb = 0; cb < BLOCKS; ++cb)
-            if (cb * CB < group_cols) block(cb);
-        } else {
 #pragma unroll 1
-          for (int cb = 0; cb * CB < group_cols && cb < BLOCKS; ++cb) block(cb);
-        }
+        for (int cb = 0; cb * CB < group_cols && cb < BLOCKS; ++cb) block(cb);
         end();
       }
       if (MODE != kModeForward && p.partial != nullptr && in_rows)
@@ -1036,12 +1037,10 @@ cudaError_t launch_by_type(int type, int d_type, int c_type, const CUtensorMap* 
   if (type == 16) {
     if (c_type == 16 && d_type == 16) return launch_typed<CTAS, BN, H, H, H>(maps, p, grid, smem, stream);
     if (c_type == kBFloat16 && d_type == 16) return launch_typed<CTAS, BN, H, H, B>(maps, p, grid, smem, stream);
-    if constexpr (BN <= 128)  // half as fast on 256 columns, where the sums spill
-      if (c_type == 32 && d_type == 32) return launch_typed<CTAS, BN, H, float, float>(maps, p, grid, smem, stream);
+    if (c_type == 32 && d_type == 32) return launch_typed<CTAS, BN, H, float, float>(maps, p, grid, smem, stream);
   } else if (type == kBFloat16) {
     if (c_type == kBFloat16 && d_type == kBFloat16) return launch_typed<CTAS, BN, B, B, B>(maps, p, grid, smem, stream);
-    if constexpr (BN <= 128)  // half as fast on 256 columns, where the sums spill
-      if (c_type == 32 && d_type == 32) return launch_typed<CTAS, BN, B, float, float>(maps, p, grid, smem, stream);
+    if (c_type == 32 && d_type == 32) return launch_typed<CTAS, BN, B, float, float>(maps, p, grid, smem, stream);
   }
   return cudaErrorInvalidValue;
 }

@@ -60,11 +60,11 @@ struct FusedVariant {
 #else
 #define B200_HD
 #endif
-B200_HD constexpr int fused_groups(int bn) { return bn >= 128 ? 2 : 1; }
+// With more warps the long chains of an epilogue hide each other; on the widest tiles the MMAs leave time enough.
+B200_HD constexpr int fused_groups(int bn) { return bn == 256 ? 2 : (bn == 128 ? 4 : (bn == 64 ? 2 : 1)); }
 B200_HD constexpr int fused_threads(int bn) { return 128 + 128 * fused_groups(bn); }
-// Columns of an epilogue block (of 32 rows), and an epilogue warp's shared memory: a block of C or D and one of Z.
-B200_HD constexpr int fused_block_cols(bool single) { return single ? 16 : 32; }
-B200_HD constexpr int fused_warp_bytes(bool single, bool aux) { return 2048 + (aux ? fused_block_cols(single) * 64 : 0); }
+// Shared memory of an epilogue warp: a block of 16 columns x 32 rows of C or D and one of Z.
+B200_HD constexpr int fused_warp_bytes(bool single, bool aux) { return (single ? 2048 : 1024) + (aux ? 1024 : 0); }
 // Shared memory behind the operand ring: the epilogue warps', or the fp32 sums of a split tile; then barriers, then the
 // group table.
 B200_HD constexpr int fused_staging_bytes(int bn, bool single, bool aux, int split) {
