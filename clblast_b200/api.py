@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import enum
 import struct
+import sys
 from typing import Sequence
 
 import numpy as np
@@ -349,36 +350,58 @@ def Col2im(kernel_mode, channels, height, width, kernel_h, kernel_w, pad_h, pad_
 
 # ---- products around a transformer block (no counterpart in the reference) -------------------------------------------
 
-_TORCH_CODE = {}
+_CODE_OF = {}   # torch dtype -> precision code
+_DTYPE_OF = {}  # precision code -> torch dtype
+_OK = StatusCode.kSuccess
 
 
-def _code(dtype) -> int:
-    """Precision code of a torch dtype, 0 for one that the library does not know."""
-    if not _TORCH_CODE:
+def _learn_types():
+    import torch
+    _CODE_OF.update({torch.float16: 16, torch.bfloat16: 1016, torch.float32: 32, torch.float64: 64,
+                     torch.complex64: 3232, torch.complex128: 6464})
+    _DTYPE_OF.update({code: dtype for dtype, code in _CODE_OF.items()})
+
+
+def _types(operand, result, precision, c_precision):
+    """(precision code, torch dtype) of the operands and of the result, from the arguments or from the tensors."""
+    if not _CODE_OF and "torch" in sys.modules:  # there are no tensors without it
+        _learn_types()
+    if precision is None:
+        precision = _CODE_OF.get(getattr(operand, "dtype", None))
+        if precision is None:
+            raise TypeError("pass precision= for raw pointers or unsupported tensor dtypes")
+    if c_precision is None:
+        c_precision = _CODE_OF.get(getattr(result, "dtype", None), precision)
+    return precision, _DTYPE_OF.get(precision), c_precision, _DTYPE_OF.get(c_precision)
+
+
+def _address(buf, dtype):
+    """Device address of an optional buffer; a tensor of another type than the call's is refused."""
+    if buf is None or type(buf) is int:
+        return buf
+    if not hasattr(buf, "data_ptr"):
+        raise TypeError(f"unsupported buffer type {type(buf)}")
+    if buf.dtype is not dtype:
+        raise TypeError(f"a tensor of {buf.dtype} where the call needs {dtype}")
+    if not buf.is_cuda:
+        raise ValueError("buffers must live in device memory")
+    return buf.data_ptr()
+
+
+def _offsets(buf):
+    if hasattr(buf, "data_ptr"):
         import torch
-        _TORCH_CODE.update({torch.float16: 16, torch.bfloat16: 1016, torch.float32: 32, torch.float64: 64,
-                            torch.complex64: 3232, torch.complex128: 6464})
-    return _TORCH_CODE.get(dtype, 0)
-
-
-def _types(operand, result, others, precision, c_precision):
-    """(dtype, c_dtype) of a call, from the arguments or from the tensors; tensors of another type are refused."""
-    p = int(precision) if precision is not None else _code(getattr(operand, "dtype", None))
-    if p == 0:
-        raise TypeError("pass precision= for raw pointers or unsupported tensor dtypes")
-    c = int(c_precision) if c_precision is not None else (_code(getattr(result, "dtype", None)) or p)
-    for buf, want in others:
-        if buf is not None and hasattr(buf, "dtype") and _code(buf.dtype) != (c if want == "c" else p):
-            raise TypeError(f"a tensor of {buf.dtype} where the call needs precision {c if want == 'c' else p}")
-    return p, c
-
-
-def _offsets(buf) -> int:
-    if hasattr(buf, "dtype"):
-        import torch
-        if buf.dtype != torch.int64 or not buf.is_contiguous():
+        if buf.dtype is not torch.int64 or not buf.is_contiguous():
             raise TypeError("group offsets are contiguous 64-bit integers")
-    return _ptr(buf)
+        return _address(buf, torch.int64)
+    return buf
+
+
+def _on(stream):
+    """(stream handle, asynchronous) as the C ABI takes them."""
+    if stream is None:
+        return None, 0
+    return (stream if type(stream) is int else stream.cuda_stream), 1
 
 
 def GemmEpilogue(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer, a_offset, a_ld, b_buffer, b_offset, b_ld,
@@ -388,13 +411,13 @@ def GemmEpilogue(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer, a_o
 
     ``bias_buffer``, ``z_buffer`` (stores Z for the backward pass) and ``d_buffer`` may be None. Half, bfloat16 or
     single; C and D may be single with 16-bit operands (``c_precision``)."""
-    p, c = _types(a_buffer, c_buffer, ((b_buffer, "a"), (bias_buffer, "a"), (z_buffer, "a"), (d_buffer, "c"), (c_buffer, "c")),
-                  precision, c_precision)
-    sp, is_async = _stream_arg(stream)
-    return _status(lib().b200blas_gemm_epilogue(
-        p, c, layout, a_transpose, b_transpose, m, n, k, alpha, _ptr(a_buffer), a_offset, a_ld,
-        _ptr(b_buffer), b_offset, b_ld, _ptr(bias_buffer), bias_offset, activation, _ptr(z_buffer), z_offset, z_ld,
-        beta, _ptr(d_buffer), d_offset, d_ld, _ptr(c_buffer), c_offset, c_ld, sp, is_async))
+    p, t, c, ct = _types(a_buffer, c_buffer, precision, c_precision)
+    sp, is_async = _on(stream)
+    st = lib().b200blas_gemm_epilogue(
+        p, c, layout, a_transpose, b_transpose, m, n, k, alpha, _address(a_buffer, t), a_offset, a_ld,
+        _address(b_buffer, t), b_offset, b_ld, _address(bias_buffer, t), bias_offset, activation, _address(z_buffer, t),
+        z_offset, z_ld, beta, _address(d_buffer, ct), d_offset, d_ld, _address(c_buffer, ct), c_offset, c_ld, sp, is_async)
+    return _OK if st == 0 else _status(st)
 
 
 def GemmEpilogueGrad(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer, a_offset, a_ld, b_buffer, b_offset, b_ld,
@@ -404,13 +427,14 @@ def GemmEpilogueGrad(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer,
 
     The backward pass through the activation of :func:`GemmEpilogue`: A is the gradient behind the next product, op(B)
     that product's weights the other way round. ``d_buffer`` and ``bias_grad_buffer`` may be None."""
-    p, _ = _types(a_buffer, c_buffer, ((b_buffer, "a"), (d_buffer, "a"), (z_buffer, "a"), (c_buffer, "a"), (bias_grad_buffer, "a")),
-                  precision, precision)
-    sp, is_async = _stream_arg(stream)
-    return _status(lib().b200blas_gemm_epilogue_grad(
-        p, layout, a_transpose, b_transpose, m, n, k, alpha, _ptr(a_buffer), a_offset, a_ld,
-        _ptr(b_buffer), b_offset, b_ld, beta, _ptr(d_buffer), d_offset, d_ld, activation, _ptr(z_buffer), z_offset,
-        z_ld, _ptr(c_buffer), c_offset, c_ld, _ptr(bias_grad_buffer), bias_grad_offset, sp, is_async))
+    p, t, _, _ = _types(a_buffer, None, precision, None)
+    sp, is_async = _on(stream)
+    st = lib().b200blas_gemm_epilogue_grad(
+        p, layout, a_transpose, b_transpose, m, n, k, alpha, _address(a_buffer, t), a_offset, a_ld,
+        _address(b_buffer, t), b_offset, b_ld, beta, _address(d_buffer, t), d_offset, d_ld, activation,
+        _address(z_buffer, t), z_offset, z_ld, _address(c_buffer, t), c_offset, c_ld, _address(bias_grad_buffer, t),
+        bias_grad_offset, sp, is_async)
+    return _OK if st == 0 else _status(st)
 
 
 def ActivationGrad(rows, n, activation, dy_buffer, dy_offset, dy_ld, z_buffer, z_offset, z_ld, dz_buffer, dz_offset, dz_ld,
@@ -418,12 +442,13 @@ def ActivationGrad(rows, n, activation, dy_buffer, dy_offset, dy_ld, z_buffer, z
                    stream=None):
     """DZ = DY * activation'(Z) for ``rows`` contiguous vectors of n elements, bias_grad = sums of DZ over the rows (of
     each group, when ``groups`` > 0). DZ or bias_grad may be None."""
-    p, _ = _types(dy_buffer, dz_buffer, ((z_buffer, "a"), (dz_buffer, "a"), (bias_grad_buffer, "a")), precision, precision)
-    sp, is_async = _stream_arg(stream)
-    return _status(lib().b200blas_activation_grad(
-        p, rows, n, activation, _ptr(dy_buffer), dy_offset, dy_ld, _ptr(z_buffer), z_offset, z_ld, _ptr(dz_buffer),
-        dz_offset, dz_ld, _ptr(bias_grad_buffer), bias_grad_offset, groups, _offsets(group_offsets), bias_grad_ld, sp,
-        is_async))
+    p, t, _, _ = _types(dy_buffer, None, precision, None)
+    sp, is_async = _on(stream)
+    st = lib().b200blas_activation_grad(
+        p, rows, n, activation, _address(dy_buffer, t), dy_offset, dy_ld, _address(z_buffer, t), z_offset, z_ld,
+        _address(dz_buffer, t), dz_offset, dz_ld, _address(bias_grad_buffer, t), bias_grad_offset, groups,
+        _offsets(group_offsets), bias_grad_ld, sp, is_async)
+    return _OK if st == 0 else _status(st)
 
 
 def GemmGrouped(w_transpose, groups, rows, n, k, alpha, x_buffer, x_offset, x_ld, w_buffer, w_offset, w_ld, w_stride,
@@ -433,36 +458,39 @@ def GemmGrouped(w_transpose, groups, rows, n, k, alpha, x_buffer, x_offset, x_ld
 
     ``group_offsets``: device array of groups + 1 ascending 64-bit row numbers, read when the work runs. Rows of no
     group are left as they were. Half or bfloat16; C and D may be single."""
-    p, c = _types(x_buffer, c_buffer, ((w_buffer, "a"), (bias_buffer, "a"), (z_buffer, "a"), (d_buffer, "c"), (c_buffer, "c")),
-                  precision, c_precision)
-    sp, is_async = _stream_arg(stream)
-    return _status(lib().b200blas_gemm_grouped(
-        p, c, w_transpose, groups, rows, n, k, alpha, _ptr(x_buffer), x_offset, x_ld, _ptr(w_buffer), w_offset, w_ld,
-        w_stride, _offsets(group_offsets), _ptr(bias_buffer), bias_offset, bias_ld, activation, _ptr(z_buffer),
-        z_offset, z_ld, beta, _ptr(d_buffer), d_offset, d_ld, _ptr(c_buffer), c_offset, c_ld, sp, is_async))
+    p, t, c, ct = _types(x_buffer, c_buffer, precision, c_precision)
+    sp, is_async = _on(stream)
+    st = lib().b200blas_gemm_grouped(
+        p, c, w_transpose, groups, rows, n, k, alpha, _address(x_buffer, t), x_offset, x_ld, _address(w_buffer, t),
+        w_offset, w_ld, w_stride, _offsets(group_offsets), _address(bias_buffer, t), bias_offset, bias_ld, activation,
+        _address(z_buffer, t), z_offset, z_ld, beta, _address(d_buffer, ct), d_offset, d_ld, _address(c_buffer, ct),
+        c_offset, c_ld, sp, is_async)
+    return _OK if st == 0 else _status(st)
 
 
 def GemmGroupedGrad(w_transpose, groups, rows, n, k, alpha, x_buffer, x_offset, x_ld, w_buffer, w_offset, w_ld, w_stride,
                     group_offsets, beta, d_buffer, d_offset, d_ld, activation, z_buffer, z_offset, z_ld, c_buffer,
                     c_offset, c_ld, bias_grad_buffer, bias_grad_offset, bias_grad_ld, *, precision=None, stream=None):
     """C = (alpha*X*op(W_g) + beta*D) * activation'(Z) row by row, bias_grad_g = sums of C over the rows of group g."""
-    p, _ = _types(x_buffer, c_buffer, ((w_buffer, "a"), (d_buffer, "a"), (z_buffer, "a"), (c_buffer, "a"), (bias_grad_buffer, "a")),
-                  precision, precision)
-    sp, is_async = _stream_arg(stream)
-    return _status(lib().b200blas_gemm_grouped_grad(
-        p, w_transpose, groups, rows, n, k, alpha, _ptr(x_buffer), x_offset, x_ld, _ptr(w_buffer), w_offset, w_ld,
-        w_stride, _offsets(group_offsets), beta, _ptr(d_buffer), d_offset, d_ld, activation, _ptr(z_buffer), z_offset,
-        z_ld, _ptr(c_buffer), c_offset, c_ld, _ptr(bias_grad_buffer), bias_grad_offset, bias_grad_ld, sp, is_async))
+    p, t, _, _ = _types(x_buffer, None, precision, None)
+    sp, is_async = _on(stream)
+    st = lib().b200blas_gemm_grouped_grad(
+        p, w_transpose, groups, rows, n, k, alpha, _address(x_buffer, t), x_offset, x_ld, _address(w_buffer, t), w_offset,
+        w_ld, w_stride, _offsets(group_offsets), beta, _address(d_buffer, t), d_offset, d_ld, activation,
+        _address(z_buffer, t), z_offset, z_ld, _address(c_buffer, t), c_offset, c_ld, _address(bias_grad_buffer, t),
+        bias_grad_offset, bias_grad_ld, sp, is_async)
+    return _OK if st == 0 else _status(st)
 
 
 def GemmGroupedWeight(groups, rows, m, n, alpha, x_buffer, x_offset, x_ld, y_buffer, y_offset, y_ld, group_offsets, beta,
                       c_buffer, c_offset, c_ld, c_stride, *, precision=None, c_precision=None, stream=None):
     """C_g = alpha*X_g^T*Y_g + beta*C_g over the rows of group g: the weight gradients of :func:`GemmGrouped`."""
-    p, c = _types(x_buffer, c_buffer, ((y_buffer, "a"), (c_buffer, "c")), precision, c_precision)
-    sp, is_async = _stream_arg(stream)
-    return _status(lib().b200blas_gemm_grouped_weight(
-        p, c, groups, rows, m, n, alpha, _ptr(x_buffer), x_offset, x_ld, _ptr(y_buffer), y_offset, y_ld,
-        _offsets(group_offsets), beta, _ptr(c_buffer), c_offset, c_ld, c_stride, sp, is_async))
+    p, t, c, ct = _types(x_buffer, c_buffer, precision, c_precision)
+    sp, is_async = _on(stream)
+    st = lib().b200blas_gemm_grouped_weight(
+        p, c, groups, rows, m, n, alpha, _address(x_buffer, t), x_offset, x_ld, _address(y_buffer, t), y_offset, y_ld,
+        _offsets(group_offsets), beta, _address(c_buffer, ct), c_offset, c_ld, c_stride, sp, is_async)
+    return _OK if st == 0 else _status(st)
 
 
 def NewtonSchulz(layout, m, n, alpha, a_buffer, a_offset, a_ld, a_stride, b_buffer, b_offset, b_ld, b_stride, batch_count, *,
@@ -471,12 +499,13 @@ def NewtonSchulz(layout, m, n, alpha, a_buffer, a_offset, a_ld, a_stride, b_buff
     X <- a*X + (b*G + c*G*G)*X with G = X*X^T on the shorter side.
 
     ``coefficients``: one triple (a, b, c), or a sequence of at least ``steps`` triples. B may be A."""
-    p, _ = _types(a_buffer, b_buffer, ((b_buffer, "a"),), precision, precision)
+    p, t, _, _ = _types(a_buffer, None, precision, None)
     flat = np.ascontiguousarray(np.asarray(coefficients, dtype=np.float64)).reshape(-1, 3)
-    sp, is_async = _stream_arg(stream)
-    return _status(lib().b200blas_newton_schulz(
-        p, layout, m, n, alpha, _ptr(a_buffer), a_offset, a_ld, a_stride, _ptr(b_buffer), b_offset, b_ld, b_stride,
-        batch_count, steps, flat.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), len(flat), epsilon, sp, is_async))
+    sp, is_async = _on(stream)
+    st = lib().b200blas_newton_schulz(
+        p, layout, m, n, alpha, _address(a_buffer, t), a_offset, a_ld, a_stride, _address(b_buffer, t), b_offset, b_ld,
+        b_stride, batch_count, steps, flat.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), len(flat), epsilon, sp, is_async)
+    return _OK if st == 0 else _status(st)
 
 
 def GemmTempBufferSize(layout, a_transpose, b_transpose, m, n, k, a_offset, a_ld, b_offset, b_ld, c_offset, c_ld, *,

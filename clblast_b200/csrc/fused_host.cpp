@@ -155,12 +155,12 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   const long long a_planes = d.kind == kFusedRaggedInner || d.a_stride == 0 ? 1 : d.problems;
   const long long b_planes = d.kind == kFusedPlain && d.b_stride != 0 ? d.problems : 1;
   // Operands that TMA cannot address are copied once to an aligned pitch.
-  PoolScratch a_copy, b_copy, partial;
+  PoolScratch copies, partial;
   FusedDesc r = d;
-  auto pack = [&](PoolScratch& to, const void*& base, long long& ld, long long& stride, bool mn, long long rows,
-                  long long planes) -> cudaError_t {
-    if (!unaddressable(base, ld, planes, stride)) return cudaSuccess;
-    PackJob job;
+  PackJob jobs[2] = {};
+  const auto plan = [&](PackJob& job, const void* base, long long ld, long long stride, bool mn, long long rows,
+                        long long planes) -> size_t {
+    if (!unaddressable(base, ld, planes, stride)) return 0;
     job.one = mn ? rows : d.k;
     job.two = mn ? d.k : rows;
     job.planes = planes;
@@ -168,17 +168,25 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
     job.src_ld = ld;
     job.src_stride = planes > 1 ? stride : 0;
     job.pitch = (job.one + 7) / 8 * 8;
-    const cudaError_t e = to.get(static_cast<size_t>(job.pitch) * job.two * planes * 2, stream);
-    if (e != cudaSuccess) return e;
-    job.dst = to.ptr();
-    base = to.ptr();
-    ld = job.pitch;
-    stride = job.pitch * job.two;
-    return launch_pack(job, stream);
+    return (static_cast<size_t>(job.pitch) * job.two * planes * 2 + 255) / 256 * 256;
   };
-  cudaError_t e = pack(a_copy, r.a, r.lda, r.a_stride, d.a_mn != 0, d.m, a_planes);
-  if (e == cudaSuccess) e = pack(b_copy, r.b, r.ldb, r.b_stride, d.b_mn != 0, d.n, b_planes);
-  if (e != cudaSuccess) return e;
+  const size_t a_bytes = plan(jobs[0], d.a, d.lda, d.a_stride, d.a_mn != 0, d.m, a_planes);
+  const size_t b_bytes = plan(jobs[1], d.b, d.ldb, d.b_stride, d.b_mn != 0, d.n, b_planes);
+  cudaError_t e = cudaSuccess;
+  if (a_bytes + b_bytes > 0) {
+    e = copies.get(a_bytes + b_bytes, stream);
+    if (e != cudaSuccess) return e;
+    if (a_bytes) {
+      jobs[0].dst = copies.ptr();
+      r.a = jobs[0].dst; r.lda = jobs[0].pitch; r.a_stride = jobs[0].pitch * jobs[0].two;
+    }
+    if (b_bytes) {
+      jobs[1].dst = copies.ptr() + a_bytes;
+      r.b = jobs[1].dst; r.ldb = jobs[1].pitch; r.b_stride = jobs[1].pitch * jobs[1].two;
+    }
+    e = launch_pack(jobs, stream);
+    if (e != cudaSuccess) return e;
+  }
 
   const Choice choice = choose(d);
   const FusedVariant& t = kFusedTable[choice.variant];

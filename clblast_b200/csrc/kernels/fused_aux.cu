@@ -21,10 +21,19 @@ constexpr int kPackThreads = 256, kPackVec = 8;
 
 // A block covers kPackThreads * kPackVec elements of one line: element loads that are consecutive across the lanes (the
 // source may start at any element), one exchange through shared memory, 16-byte stores.
-__global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackJob job, int segments) {
+struct PackPair {
+  PackJob job[2];
+  int segments[2];
+  unsigned first_of_second;
+};
+__global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackPair pair) {
   __shared__ __align__(16) unsigned short buf[kPackThreads * kPackVec];
-  const long long line = blockIdx.x / segments;
-  const int x0 = static_cast<int>(blockIdx.x % segments) * (kPackThreads * kPackVec);
+  const int which = blockIdx.x >= pair.first_of_second ? 1 : 0;
+  const unsigned block = blockIdx.x - (which ? pair.first_of_second : 0u);
+  const PackJob& job = pair.job[which];
+  const unsigned segments = static_cast<unsigned>(pair.segments[which]);
+  const long long line = block / segments;
+  const int x0 = static_cast<int>(block % segments) * (kPackThreads * kPackVec);
   const long long plane = line / job.two, in_plane = line - plane * job.two;
   const unsigned short* const src = static_cast<const unsigned short*>(job.src) + plane * job.src_stride + in_plane * job.src_ld + x0;
   const long long left = job.one - x0;
@@ -224,13 +233,22 @@ int table_smem(const long long* offsets, int groups) { return offsets != nullptr
 
 }  // namespace
 
-cudaError_t launch_pack(const PackJob& job, cudaStream_t stream) {
+cudaError_t launch_pack(const PackJob (&jobs)[2], cudaStream_t stream) {
   const long long seg = kPackThreads * kPackVec;
-  const long long segments = (job.pitch + seg - 1) / seg;
-  const long long blocks = segments * job.two * job.planes;
-  if (blocks <= 0) return cudaSuccess;
-  if (blocks > 0x7FFFFFFFLL || job.pitch > 0x7FFFFFFFLL || (job.pitch & 7)) return cudaErrorInvalidValue;
-  pack_kernel<<<static_cast<unsigned>(blocks), kPackThreads, 0, stream>>>(job, static_cast<int>(segments));
+  PackPair pair = {};
+  long long total = 0;
+  for (int i = 0; i < 2; ++i) {
+    const PackJob& job = jobs[i];
+    pair.job[i] = job;
+    if (i == 1) pair.first_of_second = static_cast<unsigned>(total);
+    const long long segments = (job.pitch + seg - 1) / seg;
+    const long long blocks = job.planes > 0 ? segments * job.two * job.planes : 0;
+    if (blocks > 0x3FFFFFFFLL || job.pitch > 0x7FFFFFFFLL || (job.pitch & 7)) return cudaErrorInvalidValue;
+    pair.segments[i] = blocks > 0 ? static_cast<int>(segments) : 1;
+    total += blocks;
+  }
+  if (total <= 0) return cudaSuccess;
+  pack_kernel<<<static_cast<unsigned>(total), kPackThreads, 0, stream>>>(pair);
   return cudaGetLastError();
 }
 

@@ -7,13 +7,14 @@
 namespace b200 {
 
 // Copies `planes` matrices of `two` lines of `one` contiguous 2-byte elements each (any alignment, leading dimension and
-// plane stride) to lines of `pitch` elements (a multiple of 8, the rest zero), planes two * pitch apart.
+// plane stride) to lines of `pitch` elements (a multiple of 8, the rest zero), planes two * pitch apart. Two jobs go in one
+// launch; one with planes == 0 is skipped.
 struct PackJob {
   const void* src;
   void* dst;
   long long one, two, planes, src_ld, src_stride, pitch;
 };
-cudaError_t launch_pack(const PackJob& job, cudaStream_t stream);
+cudaError_t launch_pack(const PackJob (&jobs)[2], cudaStream_t stream);
 
 // Element-wise tail of a product P (m x n, m contiguous; n vectors of m features):
 //   grad == 0: Z = P + bias, C = act(Z) + beta D;   grad == 1: C = (P + beta D) * slope(Z), partial sums over vectors.

@@ -243,6 +243,17 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, code, status) ? 1 : 0;
   return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
 }
+// The same for the epilogue's long waits: sleeping between polls leaves the issue slots and the power to the MMAs (1.5 % of
+// 8192^3, which runs at the power limit).
+__device__ __forceinline__ bool warp_wait_relaxed(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned code,
+                                                  unsigned int* status) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) {
+    for (int i = 0; i < 10000 && !mbar_try_wait(bar, parity); ++i) __nanosleep(200);
+    ok = mbar_wait(bar, parity, abort_flag, code, status) ? 1 : 0;
+  }
+  return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
+}
 __device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned code,
                                                   unsigned int* status) {
   int ok = 1;
@@ -665,7 +676,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         return tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc_of(number) * BN + group * GROUP_COLS);
       };
       auto wait_accumulator = [&](int number) {
-        return warp_wait(acc_full_bar(acc_of(number)), acc_parity(number), abort_flag, 4u, p.status);
+        return warp_wait_relaxed(acc_full_bar(acc_of(number)), acc_parity(number), abort_flag, 4u, p.status);
       };
       auto release_accumulator = [&](int number) {
         tcgen05_fence_before();

@@ -94,7 +94,7 @@ def test_types_of_tensors():
     import torch
     half, single, offsets = torch.zeros(4, dtype=torch.float16), torch.zeros(4), torch.zeros(2, dtype=torch.int32)
     with pytest.raises(TypeError):  # B is not half
-        cb.GemmEpilogue(ROW, NO, NO, 2, 2, 2, 1.0, half, 0, 2, single, 0, 2, None, 0, 161, None, 0, 2, 0.0, None, 0, 2, half, 0, 2)
+        cb.GemmEpilogue(ROW, NO, NO, 2, 2, 2, 1.0, 0, 0, 2, single, 0, 2, None, 0, 161, None, 0, 2, 0.0, None, 0, 2, 0, 0, 2, precision=16)
     with pytest.raises(TypeError):  # no precision for raw pointers
         cb.GemmEpilogue(ROW, NO, NO, 2, 2, 2, 1.0, 0, 0, 2, 0, 0, 2, None, 0, 161, None, 0, 2, 0.0, None, 0, 2, 0, 0, 2)
     with pytest.raises(TypeError):  # offsets are 64-bit
