@@ -97,8 +97,16 @@ double estimate(const FusedDesc& d, int v, int split) {
   const double teams = static_cast<double>(resident_teams(t.ctas * split));
   const double waves = static_cast<double>(static_cast<long long>((tiles + teams - 1) / teams));
   const double inner = static_cast<double>(static_cast<long long>((blocks + split - 1) / split));
-  const double drain = 1500.0 + 12.0 * t.bn + (split > 1 ? 1500.0 : 0.0);
-  return waves * (inner * per_block + 400.0) + drain + 1500.0;
+  const double drain = 1500.0 + 12.0 * t.bn + (split > 1 ? 1500.0 + 6.0 * t.bn : 0.0);
+  const double work = waves * (inner * per_block + 400.0);
+  // each operand read once and C written once: what no variant avoids (in bytes per cycle of all SMs)
+  const double planes = d.kind == kFusedRaggedCols ? static_cast<double>(d.problems < d.n ? d.problems : d.n)
+                                                   : static_cast<double>(d.a_stride != 0 ? d.problems : 1);
+  const double c_planes = d.kind == kFusedRaggedCols ? 1.0 : static_cast<double>(d.problems);
+  const double bytes = 2.0 * static_cast<double>(d.k) * (planes * d.m + static_cast<double>(d.n) * (d.kind == kFusedPlain ? problems : 1.0)) +
+                       c_planes * static_cast<double>(d.m) * d.n * (d.c_type == 32 ? 4.0 : 2.0);
+  const double memory = bytes / 3300.0;
+  return (work > memory ? work : memory) + drain;
 }
 
 // B200BLAS_FUSED=<variant>[,<split>] forces one for measurements and tests where it can serve the call.

@@ -213,6 +213,9 @@ __device__ __forceinline__ void tma_load_3d_hint(uint32_t dst, const CUtensorMap
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // Asks L2 for a tile of an epilogue matrix.
 __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
@@ -400,6 +403,10 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   const int first_tile = static_cast<int>(blockIdx.x) / team;
   const int tile_step = static_cast<int>(gridDim.x) / team;
 
+  if (threadIdx.x == 32) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar(s), 1);
@@ -416,6 +423,62 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     *progress = 0;
     fence_barrier_init();
   }
+  // this CTA's share of a tile's inner blocks
+  auto k_range = [&](const Tile& t, int& kb0, int& kb1) {
+    const int blocks = (t.k_len + BK - 1) / BK;
+    if (split > 1) {
+      kb0 = blocks * static_cast<int>(rank) / split;
+      kb1 = blocks * (static_cast<int>(rank) + 1) / split;
+    } else {
+      kb0 = 0;
+      kb1 = blocks;
+    }
+  };
+
+
+  // Loads of one inner block into a stage of the ring, by one lane.
+  auto issue_block = [&](const Tile& t, int kb, int stage, uint64_t pol_a, uint64_t pol_b) {
+    const int a_row0 = (t.tm * CTAS + (CTAS == 2 ? static_cast<int>(rank) : 0)) * BM;
+    const int b_row0 = t.col0 + (CTAS == 2 ? static_cast<int>(rank) * B_ROWS : 0);
+    const int az = p.a_batched ? t.z : 0, bz = p.b_batched ? t.z : 0;
+    const uint32_t a_dst = tiles_base + stage * STAGE_BYTES;
+    const uint32_t b_dst = a_dst + A_BYTES;
+    const int x = t.k0 + kb * BK;
+    uint32_t bar;
+    if constexpr (CTAS == 2) {
+      // a block whose end has to be cleared is counted by each CTA for itself
+      const bool tail = p.kind == kFusedRaggedInner && t.k_len - kb * BK < BK;
+      if (rank == 0) {
+        bar = map_to_cta(full_bar(stage), 0);
+        mbar_arrive_expect_tx(full_bar(stage), (tail ? 1 : 2) * STAGE_BYTES);  // otherwise the bytes of both CTAs
+      } else if (tail) {
+        bar = map_to_cta(full_bar(stage), 1);
+        mbar_arrive_expect_tx(full_bar(stage), STAGE_BYTES);
+      } else {
+        bar = map_to_cta(full_bar(stage), 0);
+      }
+    } else {
+      bar = full_bar(stage);
+      mbar_arrive_expect_tx(bar, STAGE_BYTES);
+    }
+    auto load = [&](uint32_t dst, const CUtensorMap* map, int cx, int cy, int cz, uint64_t pol) {
+      if constexpr (CTAS == 2) tma_load_3d_pair_hint(dst, map, bar, cx, cy, cz, pol);
+      else tma_load_3d_hint(dst, map, bar, cx, cy, cz, pol);
+    };
+    if (p.a_mn) {
+#pragma unroll
+      for (int j = 0; j < BM / 64; ++j) load(a_dst + j * 8192, &map_a, a_row0 + j * 64, x, az, pol_a);
+    } else {
+      load(a_dst, &map_a, x, a_row0, az, pol_a);
+    }
+    if (p.b_mn) {
+#pragma unroll
+      for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * 8192, &map_b, b_row0 + j * 64, x, bz, pol_b);
+    } else {
+      load(b_dst, &map_b, x, b_row0, bz, pol_b);
+    }
+  };
+
   if (warp == 1) {
     if constexpr (CTAS == 2) tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
     else tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
@@ -433,18 +496,6 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   auto acc_of = [](int n) { return ACCS == 1 ? 0 : (n & 1); };
   auto acc_parity = [](int n) { return static_cast<uint32_t>(ACCS == 1 ? n : (n >> 1)) & 1u; };
 
-  // this CTA's share of a tile's inner blocks
-  auto k_range = [&](const Tile& t, int& kb0, int& kb1) {
-    const int blocks = (t.k_len + BK - 1) / BK;
-    if (split > 1) {
-      kb0 = blocks * static_cast<int>(rank) / split;
-      kb1 = blocks * (static_cast<int>(rank) + 1) / split;
-    } else {
-      kb0 = 0;
-      kb1 = blocks;
-    }
-  };
-
   if (warp == 0) {
     // ---- TMA producer: the warp walks along, one lane issues ----
     {
@@ -454,52 +505,12 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       const uint64_t pol_a = l2_policy(p.hint_a), pol_b = l2_policy(p.hint_b);
       for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
         const Tile t = locate<BN>(p, tile, start, tiles);
-        const int a_row0 = (t.tm * CTAS + (CTAS == 2 ? static_cast<int>(rank) : 0)) * BM;
-        const int b_row0 = t.col0 + (CTAS == 2 ? static_cast<int>(rank) * B_ROWS : 0);
-        const int az = p.a_batched ? t.z : 0, bz = p.b_batched ? t.z : 0;
         int kb0, kb1;
         k_range(t, kb0, kb1);
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, 1u, p.status);
           if (!ok) break;
-          if (elect_one()) {
-            const uint32_t a_dst = tiles_base + stage * STAGE_BYTES;
-            const uint32_t b_dst = a_dst + A_BYTES;
-            const int x = t.k0 + kb * BK;
-            uint32_t bar;
-            if constexpr (CTAS == 2) {
-              // a block whose end has to be cleared is counted by each CTA for itself
-              const bool tail = p.kind == kFusedRaggedInner && t.k_len - kb * BK < BK;
-              if (rank == 0) {
-                bar = map_to_cta(full_bar(stage), 0);
-                mbar_arrive_expect_tx(full_bar(stage), (tail ? 1 : 2) * STAGE_BYTES);  // otherwise the bytes of both CTAs
-              } else if (tail) {
-                bar = map_to_cta(full_bar(stage), 1);
-                mbar_arrive_expect_tx(full_bar(stage), STAGE_BYTES);
-              } else {
-                bar = map_to_cta(full_bar(stage), 0);
-              }
-            } else {
-              bar = full_bar(stage);
-              mbar_arrive_expect_tx(bar, STAGE_BYTES);
-            }
-            auto load = [&](uint32_t dst, const CUtensorMap* map, int cx, int cy, int cz, uint64_t pol) {
-              if constexpr (CTAS == 2) tma_load_3d_pair_hint(dst, map, bar, cx, cy, cz, pol);
-              else tma_load_3d_hint(dst, map, bar, cx, cy, cz, pol);
-            };
-            if (p.a_mn) {
-#pragma unroll
-              for (int j = 0; j < BM / 64; ++j) load(a_dst + j * 8192, &map_a, a_row0 + j * 64, x, az, pol_a);
-            } else {
-              load(a_dst, &map_a, x, a_row0, az, pol_a);
-            }
-            if (p.b_mn) {
-#pragma unroll
-              for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * 8192, &map_b, b_row0 + j * 64, x, bz, pol_b);
-            } else {
-              load(b_dst, &map_b, x, b_row0, bz, pol_b);
-            }
-          }
+          if (elect_one()) issue_block(t, kb, stage, pol_a, pol_b);
           __syncwarp();
           if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
@@ -648,6 +659,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const bool has_d = p.d != nullptr;
     const bool grad = MODE == kModeGrad || (MODE == kModeGeneral && p.grad);
     const bool z_in = aux && grad, z_out = aux && !grad;
+    const bool one_tile = num_tiles <= tile_step;  // a short kernel: its end is what counts
     int local = 0;   // accumulators taken so far
     int tiles_done = 0;
     bool ok = true;
@@ -676,7 +688,8 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         return tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc_of(number) * BN + group * GROUP_COLS);
       };
       auto wait_accumulator = [&](int number) {
-        return warp_wait_relaxed(acc_full_bar(acc_of(number)), acc_parity(number), abort_flag, 4u, p.status);
+        return one_tile ? warp_wait(acc_full_bar(acc_of(number)), acc_parity(number), abort_flag, 4u, p.status)
+                        : warp_wait_relaxed(acc_full_bar(acc_of(number)), acc_parity(number), abort_flag, 4u, p.status);
       };
       auto release_accumulator = [&](int number) {
         tcgen05_fence_before();
@@ -725,95 +738,121 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (split > 1) {
           // -- tile shared by a cluster: sums meet in shared memory, every CTA finishes a range of columns --
           float* const sums = reinterpret_cast<float*>(staging);  // [column][128 rows]
-          if constexpr (!CHUNKED) {
-            ok = wait_accumulator(local);
-            if (!ok) break;
-            tcgen05_fence_after();
-          }
-          if (tiles_done > 0) {
-            ok = warp_wait_cluster(sums_free, (tiles_done - 1) & 1u, abort_flag, 7u, p.status);
-            if (!ok) break;
-          }
-#pragma unroll
-          for (int cb = 0; cb < BLOCKS; ++cb) {
-            const int col = group * GROUP_COLS + cb * CB;
-            uint32_t r[CB];
-            if (!empty) {
-              tmem_ld(values + cb * CB, r);
-              tmem_wait(r);
-            }
-#pragma unroll
-            for (int j = 0; j < CB; ++j) sums[(col + j) * BM + row_in_cta] = empty ? 0.f : __uint_as_float(r[j]);
-          }
-          if constexpr (!CHUNKED) {
-            release_accumulator(local);
-            ++local;
-          }
-          __syncwarp();
-          if (lane == 0) {
-            for (int q = 0; q < split; ++q) mbar_arrive_remote(map_to_cta(sums_ready, q));
-          }
-          const int mine = BN / split;  // columns per CTA, a multiple of four
+          // This CTA's columns in steps of STEP per group; D and Z of the next step are under way while one is finished.
+          constexpr int STEP = 4;
+          const int mine = BN / split;  // a multiple of STEP
           const int first_col = static_cast<int>(rank) * mine;
-          // D and Z of four columns; those of the next four are under way while four are finished
-          float d4[4], z4[4], d_ahead[4], z_ahead[4];
-          auto fetch = [&](int q, float (&d)[4], float (&z)[4]) {
-            const int rel = first_col + q * 4 - group * GROUP_COLS;
-            const int cols_left = t.col_end - (t.col0 + first_col + q * 4);
+          float d_ahead[STEP], z_ahead[STEP];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < STEP; ++j) d_ahead[j] = z_ahead[j] = 0.f;
+          auto fetch = [&](int q) {
+            const int rel = first_col + q * STEP - group * GROUP_COLS;
+            const int cols_left = t.col_end - (t.col0 + first_col + q * STEP);
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) {
               const bool in = in_rows && j < cols_left;
-              d[j] = has_d && in ? to_float(d_ptr[static_cast<long long>(rel + j) * p.ldd + lane]) : 0.f;
-              z[j] = z_in && in ? to_float(z_ptr[static_cast<long long>(rel + j) * p.ldz + lane]) : 0.f;
+              d_ahead[j] = has_d && in ? to_float(d_ptr[static_cast<long long>(rel + j) * p.ldd + lane]) : 0.f;
+              z_ahead[j] = z_in && in ? to_float(z_ptr[static_cast<long long>(rel + j) * p.ldz + lane]) : 0.f;
             }
           };
-          fetch(group, d_ahead, z_ahead);
-          ok = warp_wait_cluster(sums_ready, tiles_done & 1u, abort_flag, 8u, p.status);
-          if (!ok) break;
-          for (int q = group; q < mine / 4; q += EG) {
-            const int in_tile = first_col + q * 4;
+          if (tiles_done > 0) fetch(group);
+          // Step -1 of a CTA's first tile requests that and brings the code into the instruction caches (see run_blocks).
+#pragma unroll 1
+          for (int step = tiles_done == 0 ? -1 : 0; ok; ++step) {
+            if (step == 0) {
+              if constexpr (!CHUNKED) {
+                ok = wait_accumulator(local);
+                if (!ok) break;
+                tcgen05_fence_after();
+              }
+              if (tiles_done > 0) {
+                ok = warp_wait_cluster(sums_free, (tiles_done - 1) & 1u, abort_flag, 7u, p.status);
+                if (!ok) break;
+              }
+#pragma unroll 1
+              for (int cb = 0; cb < BLOCKS; ++cb) {
+                const int col = group * GROUP_COLS + cb * CB;
+                uint32_t r[CB];
+                if (!empty) {
+                  tmem_ld(values + cb * CB, r);
+                  tmem_wait(r);
+                }
+#pragma unroll
+                for (int j = 0; j < CB; ++j) sums[(col + j) * BM + row_in_cta] = empty ? 0.f : __uint_as_float(r[j]);
+              }
+              if constexpr (!CHUNKED) {
+                release_accumulator(local);
+                ++local;
+              }
+              __syncwarp();
+              if (lane == 0) {
+                for (int q = 0; q < split; ++q) mbar_arrive_remote(map_to_cta(sums_ready, q));
+              }
+              ok = warp_wait_cluster(sums_ready, tiles_done & 1u, abort_flag, 8u, p.status);
+              if (!ok) break;
+            }
+            const bool dry = step < 0;
+            const int q = group + step * EG;
+            if (!dry && q >= mine / STEP) break;
+            const int in_tile = dry ? 0 : first_col + q * STEP;
             const int rel = in_tile - group * GROUP_COLS;  // column relative to group_col0
-            const int cols_left = t.col_end - (t.col0 + in_tile);
-            if (cols_left <= 0) break;
-            float part[8][4];
+            const int cols_left = dry ? 0 : t.col_end - (t.col0 + in_tile);
+            if (!dry && cols_left <= 0) break;
+            const uint32_t at = smem_u32(sums + in_tile * BM + row_in_cta);
+            float v[STEP], d4[STEP], z4[STEP];
+            // all reads of a pair of ranks before their sum; the order of the additions is that of the ranks
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-              if (s < split) {
-                const uint32_t src = map_to_cta(smem_u32(sums + in_tile * BM + row_in_cta), s);
+            for (int j = 0; j < STEP; ++j) v[j] = 0.f;
+#pragma unroll 1
+            for (int s = 0; s < split; s += 2) {
+              const uint32_t src0 = map_to_cta(at, s), src1 = map_to_cta(at, s + 1);
+              float u0[STEP], u1[STEP];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) part[s][j] = ld_cluster_f32(src + j * BM * 4);
-              } else {
+              for (int j = 0; j < STEP; ++j) {
+                u0[j] = ld_cluster_f32(src0 + j * BM * 4);
+                u1[j] = ld_cluster_f32(src1 + j * BM * 4);
+              }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) part[s][j] = 0.f;
+              for (int j = 0; j < STEP; ++j) v[j] = (v[j] + u0[j]) + u1[j];
+            }
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) { d4[j] = d_ahead[j]; z4[j] = z_ahead[j]; }
+            if (q + EG < mine / STEP) fetch(q + EG);
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) v[j] = fmaf(p.alpha, v[j], bias);
+            if (grad) {
+              if (has_d) {
+#pragma unroll
+                for (int j = 0; j < STEP; ++j) v[j] = fmaf(p.beta, d4[j], v[j]);
+              }
+              if (z_in) {
+                with_act(p.act, [&](auto tag) {
+#pragma unroll
+                  for (int j = 0; j < STEP; ++j) v[j] *= act_slope<FAST, decltype(tag)::value>(z4[j]);
+                });
+              }
+#pragma unroll
+              for (int j = 0; j < STEP; ++j) row_sum += j < cols_left ? v[j] : 0.f;
+            } else {
+              if (z_out) {
+#pragma unroll
+                for (int j = 0; j < STEP; ++j)
+                  if (in_rows && j < cols_left) z_ptr[static_cast<long long>(rel + j) * p.ldz + lane] = from_float<T>(v[j]);
+              }
+              with_act(p.act, [&](auto tag) {
+#pragma unroll
+                for (int j = 0; j < STEP; ++j) v[j] = act_value<FAST, decltype(tag)::value>(v[j]);
+              });
+              if (has_d) {
+#pragma unroll
+                for (int j = 0; j < STEP; ++j) v[j] = fmaf(p.beta, d4[j], v[j]);
               }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { d4[j] = d_ahead[j]; z4[j] = z_ahead[j]; }
-            if (q + EG < mine / 4) fetch(q + EG, d_ahead, z_ahead);
-            with_act(p.act, [&](auto tag) {
-              constexpr int ACT = decltype(tag)::value;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float v = part[0][j];
-#pragma unroll
-                for (int s = 1; s < 8; ++s) v += part[s][j];
-                if (!in_rows || j >= cols_left) continue;
-                const long long cj = rel + j;
-                const float add = p.beta * d4[j];
-                float y = fmaf(p.alpha, v, bias);
-                if (grad) {
-                  if (has_d) y += add;
-                  if (z_in) y *= act_slope<FAST, ACT>(z4[j]);
-                  row_sum += y;
-                } else {
-                  if (z_out) z_ptr[cj * p.ldz + lane] = from_float<T>(y);
-                  y = act_value<FAST, ACT>(y);
-                  if (has_d) y += add;
-                }
-                c_ptr[cj * p.ldc + lane] = from_float<OT>(y);
-              }
-            });
+            for (int j = 0; j < STEP; ++j)
+              if (in_rows && j < cols_left) c_ptr[static_cast<long long>(rel + j) * p.ldc + lane] = from_float<OT>(v[j]);
           }
+          if (!ok) break;
           __syncwarp();
           if (lane == 0) {
             for (int q = 0; q < split; ++q) mbar_arrive_remote(map_to_cta(sums_free, q));
@@ -827,7 +866,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       // accumulator values of block cb; the load of the next block starts as this one's arrives
       uint32_t r_next[CB];
       auto take = [&](int cb, float (&v)[CB]) {
-        if (empty) {
+        if (empty || cb < 0) {
 #pragma unroll
           for (int j = 0; j < CB; ++j) v[j] = bias;
         } else {
@@ -846,6 +885,22 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (!empty) tmem_ld(values, r_next);
         return true;
       };
+      // All blocks of the tile. On a CTA's first tile they are preceded by a dry one without columns: it brings the code
+      // into the instruction caches and requests the first block's D and Z while the operands are still on their way.
+      // (Cold code cost 15000 cycles at the end of a kernel of one tile per CTA.)
+      auto run_blocks = [&](auto& block, auto& request) {
+        int cb = -1;
+        if (tiles_done > 0) {
+          request(0);
+          cb = 0;
+        }
+#pragma unroll 1
+        for (; cb < BLOCKS; ++cb) {
+          if (cb == 0 && !begin()) break;
+          if (cb >= 0 && cb * CB >= group_cols) break;
+          block(cb);
+        }
+      };
       auto end = [&]() {
         if (!empty) tmem_wait(r_next);  // a load may have started for a block that does not exist
         if constexpr (!CHUNKED) {
@@ -856,19 +911,17 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
       if constexpr (MODE != kModeGeneral) {
         // D and Z of a block are requested while the block before it is worked on
-        BlockD d_next;
-        BlockZ z_next;
+        BlockD d_next = {};
+        BlockZ z_next = {};
         auto request = [&](int cb) {
           if (has_d) d_next.load(d_ptr + static_cast<long long>(cb * CB) * p.ldd, p.ldd, rows_left, group_cols - cb * CB, lane);
           if (MODE == kModeGrad && aux) z_next.load(z_ptr + static_cast<long long>(cb * CB) * p.ldz, p.ldz, rows_left, group_cols - cb * CB, lane);
         };
-        request(0);
-        if (!begin()) break;
         uint8_t* const own = staging + (warp - 4) * fused_warp_bytes(CHUNKED, aux);
         uint32_t* const turn_c = reinterpret_cast<uint32_t*>(own);
         uint32_t* const turn_z = turn_c + BlockC::WORDS;
         auto block = [&](int cb) {
-          const int cols_left = group_cols - cb * CB;
+          const int cols_left = cb < 0 ? 0 : group_cols - cb * CB;
           float v[CB];
           take(cb, v);
           auto add_d = [&]() {
@@ -925,48 +978,72 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
           }
         };
-#pragma unroll 1
-        for (int cb = 0; cb * CB < group_cols && cb < BLOCKS; ++cb) block(cb);
+        run_blocks(block, request);
+        if (!ok) break;
         end();
       } else {
-        if (!begin()) break;
+        // row by row, element by element; D and Z of a block are requested while the block before it is worked on
+        DT d_next[CB];
+        T z_next[CB];
+        auto request = [&](int cb) {
+          const int cols_left = in_rows ? group_cols - cb * CB : 0;
+          const DT* d_at = d_ptr + static_cast<long long>(cb * CB) * p.ldd + lane;
+          const T* z_at = z_ptr + static_cast<long long>(cb * CB) * p.ldz + lane;
+          if (has_d) {
+#pragma unroll
+            for (int j = 0; j < CB; ++j, d_at += p.ldd) d_next[j] = j < cols_left ? *d_at : from_float<DT>(0.f);
+          }
+          if (z_in) {
+#pragma unroll
+            for (int j = 0; j < CB; ++j, z_at += p.ldz) z_next[j] = j < cols_left ? *z_at : from_float<T>(0.f);
+          }
+        };
+#pragma unroll
+        for (int j = 0; j < CB; ++j) {
+          d_next[j] = from_float<DT>(0.f);
+          z_next[j] = from_float<T>(0.f);
+        }
         auto block = [&](int cb) {
-          const int cols_left = group_cols - cb * CB;
+          const int cols_left = in_rows && cb >= 0 ? group_cols - cb * CB : 0;
           float v[CB];
           take(cb, v);
-          if (!in_rows) return;
-          const long long at = cb * CB;
-          float add[CB];
-#pragma unroll
-          for (int j = 0; j < CB; ++j)
-            add[j] = (has_d && j < cols_left) ? p.beta * to_float(d_ptr[(at + j) * p.ldd + lane]) : 0.f;
           if (grad) {
-            float zz[CB];
+            if (has_d) {
 #pragma unroll
-            for (int j = 0; j < CB; ++j) zz[j] = (z_in && j < cols_left) ? to_float(z_ptr[(at + j) * p.ldz + lane]) : 0.f;
-            with_act(z_in ? p.act : static_cast<int>(kActIdentity), [&](auto tag) {
+              for (int j = 0; j < CB; ++j) v[j] = fmaf(p.beta, to_float(d_next[j]), v[j]);
+            }
+            if (z_in) {
+              with_act(p.act, [&](auto tag) {
 #pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] = (v[j] + add[j]) * act_slope<FAST, decltype(tag)::value>(zz[j]);
-            });
+                for (int j = 0; j < CB; ++j) v[j] *= act_slope<FAST, decltype(tag)::value>(to_float(z_next[j]));
+              });
+            }
 #pragma unroll
             for (int j = 0; j < CB; ++j) row_sum += j < cols_left ? v[j] : 0.f;
           } else {
             if (z_out) {
+              T* at = z_ptr + static_cast<long long>(cb * CB) * p.ldz + lane;
 #pragma unroll
-              for (int j = 0; j < CB; ++j)
-                if (j < cols_left) z_ptr[(at + j) * p.ldz + lane] = from_float<T>(v[j]);
+              for (int j = 0; j < CB; ++j, at += p.ldz)
+                if (j < cols_left) *at = from_float<T>(v[j]);
             }
             with_act(p.act, [&](auto tag) {
 #pragma unroll
-              for (int j = 0; j < CB; ++j) v[j] = act_value<FAST, decltype(tag)::value>(v[j]) + add[j];
+              for (int j = 0; j < CB; ++j) v[j] = act_value<FAST, decltype(tag)::value>(v[j]);
             });
-          }
+            if (has_d) {
 #pragma unroll
-          for (int j = 0; j < CB; ++j)
-            if (j < cols_left) c_ptr[(at + j) * p.ldc + lane] = from_float<OT>(v[j]);
+              for (int j = 0; j < CB; ++j) v[j] = fmaf(p.beta, to_float(d_next[j]), v[j]);
+            }
+          }
+          if (cb + 1 < BLOCKS) request(cb + 1);
+          OT* at = c_ptr + static_cast<long long>(cb * CB) * p.ldc + lane;
+#pragma unroll
+          for (int j = 0; j < CB; ++j, at += p.ldc)
+            if (j < cols_left) *at = from_float<OT>(v[j]);
         };
-#pragma unroll 1
-        for (int cb = 0; cb * CB < group_cols && cb < BLOCKS; ++cb) block(cb);
+        run_blocks(block, request);
+        if (!ok) break;
         end();
       }
       if (MODE != kModeForward && p.partial != nullptr && in_rows)
