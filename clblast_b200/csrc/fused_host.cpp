@@ -2,6 +2,7 @@
 
 #include <cuda.h>
 
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -73,40 +74,46 @@ int resident_teams(int team) {
   return n > 0 ? n : 1;
 }
 
-// Time in SM cycles by a small model: waves of tiles x (inner blocks x the slower of the MMAs and the operand loads of a
-// block) + the drain of the last tile, against the memory traffic of the whole call.
-double estimate(const FusedDesc& d, int v, int split) {
+// Time in SM cycles by a small model: waves of tiles, each the slower of its inner blocks and its epilogue, against the
+// memory traffic of the whole call, and what nothing hides at both ends. The constants were fitted to 277 problems with
+// every variant timed on each (sizes 1 to 8192, all kinds and types): the choice is within 2 % of the best one in the mean.
+// An inner block costs nearly the same on every width, since the operands' way through shared memory and the issue bound
+// the narrow ones; results in single precision wait for their one accumulator on 256 columns.
+double estimate(const FusedDesc& d, int v, int split, bool vec) {
+  static constexpr double kBlock[kFusedVariants] = {540.0, 570.0, 530.0, 490.0, 510.0, 735.0};
   const FusedVariant& t = kFusedTable[v];
-  const double tm = static_cast<double>((d.m + 128 * t.ctas - 1) / (128 * t.ctas));
-  double tn, problems = 1, k = static_cast<double>(d.k);
+  const auto whole = [](double x) { return std::ceil(x); };
+  const bool single = d.c_type == 32;
+  const double rows = static_cast<double>(d.m), cols = static_cast<double>(d.n);
+  const double tm = whole(rows / (128 * t.ctas));
+  const double active = static_cast<double>(d.problems < d.n ? d.problems : d.n);  // groups that can have vectors
+  double tn = whole(cols / t.bn), problems = 1.0, k = static_cast<double>(d.k);
   if (d.kind == kFusedRaggedCols) {
-    const double active = static_cast<double>(d.problems < d.n ? d.problems : d.n);
-    const double each = static_cast<double>(d.n) / active;
-    tn = active * static_cast<double>(static_cast<long long>((each + t.bn - 1) / t.bn));
+    tn = active * whole(cols / active / t.bn);
   } else {
-    tn = static_cast<double>((d.n + t.bn - 1) / t.bn);
     problems = static_cast<double>(d.problems);
-    if (d.kind == kFusedRaggedInner) k = k / problems;
+    if (d.kind == kFusedRaggedInner) k /= problems;
   }
-  double tiles = tm * tn * problems;
-  if (d.tri) tiles = tm * (tm + 1) / 2 * problems;
-  const double blocks = static_cast<double>(static_cast<long long>((k + 63) / 64));
-  const double per_block_mma = t.ctas == 2 ? (t.bn == 256 ? 530.0 : 270.0) : (t.bn == 256 ? 530.0 : (t.bn == 128 ? 270.0 : (t.bn == 64 ? 150.0 : 110.0)));
-  const double per_block_load = t.stage_bytes / 60.0;
-  const double per_block = per_block_mma > per_block_load ? per_block_mma : per_block_load;
-  const double teams = static_cast<double>(resident_teams(t.ctas * split));
-  const double waves = static_cast<double>(static_cast<long long>((tiles + teams - 1) / teams));
-  const double inner = static_cast<double>(static_cast<long long>((blocks + split - 1) / split));
-  const double drain = 1500.0 + 12.0 * t.bn + (split > 1 ? 1500.0 + 6.0 * t.bn : 0.0);
-  const double work = waves * (inner * per_block + 400.0);
-  // each operand read once and C written once: what no variant avoids (in bytes per cycle of all SMs)
-  const double planes = d.kind == kFusedRaggedCols ? static_cast<double>(d.problems < d.n ? d.problems : d.n)
-                                                   : static_cast<double>(d.a_stride != 0 ? d.problems : 1);
+  const double tiles = d.tri ? tm * (tm + 1.0) / 2.0 * problems : tm * tn * problems;
+  const double block = kBlock[v] * (single && t.bn == 256 ? 1.7 : 1.0);
+  const double load = t.stage_bytes / 62.0;
+  const double waves = whole(tiles / resident_teams(t.ctas * split));
+  const double main = whole(whole(k / 64.0) / split) * (block > load ? block : load) + 1140.0;
+  // per column of a tile
+  const bool reads_z = d.z != nullptr && d.grad, writes_z = d.z != nullptr && !d.grad;
+  const bool adds = d.beta != 0.0 && d.d != nullptr;
+  double column = 15.0 + (d.act != 161 ? 10.6 : 0.0) + (adds ? 6.0 : 0.0) + (d.z != nullptr ? 6.0 : 0.0);
+  if (single) column *= 1.5;
+  if (!vec) column += (t.bn == 128 ? 29.0 : 8.8) * (1.0 + (writes_z ? 1.0 : 0.0) + (reads_z ? 0.5 : 0.0) + (adds ? 0.5 : 0.0));
+  double epilogue = column * t.bn;
+  if (split > 1) epilogue = 2.55 * epilogue / split + 4800.0 + 10.0 * t.bn;
+  // each operand read once and C written once
+  const double a_planes = d.kind == kFusedRaggedCols ? active : (d.a_stride != 0 ? problems : 1.0);
   const double c_planes = d.kind == kFusedRaggedCols ? 1.0 : static_cast<double>(d.problems);
-  const double bytes = 2.0 * static_cast<double>(d.k) * (planes * d.m + static_cast<double>(d.n) * (d.kind == kFusedPlain ? problems : 1.0)) +
-                       c_planes * static_cast<double>(d.m) * d.n * (d.c_type == 32 ? 4.0 : 2.0);
-  const double memory = bytes / 3300.0;
-  return (work > memory ? work : memory) + drain;
+  const double bytes = 2.0 * d.k * (a_planes * rows + cols * (d.kind == kFusedPlain ? problems : 1.0)) +
+                       c_planes * rows * cols * (single ? 4.0 : 2.0);
+  const double work = waves * (main > epilogue ? main : epilogue), memory = bytes / 3600.0;
+  return (work > memory ? work : memory) + 6000.0 + epilogue;
 }
 
 // B200BLAS_FUSED=<variant>[,<split>] forces one for measurements and tests where it can serve the call.
@@ -120,13 +127,13 @@ bool forced_variant(int* variant, int* split) {
   return true;
 }
 
-Choice choose(const FusedDesc& d) {
+Choice choose(const FusedDesc& d, bool vec) {
   Choice best = {2, 1};
   double best_time = 1e300;
   for (int v = 0; v < kFusedVariants; ++v) {
     for (int split = 1; split <= 8; split *= 2) {
       if (!variant_fits(d, v, split)) continue;
-      const double time = estimate(d, v, split);
+      const double time = estimate(d, v, split, vec);
       if (time < best_time * 0.999) {
         best_time = time;
         best = {v, split};
@@ -180,6 +187,7 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   };
   const size_t a_bytes = plan(jobs[0], d.a, d.lda, d.a_stride, d.a_mn != 0, d.m, a_planes);
   const size_t b_bytes = plan(jobs[1], d.b, d.ldb, d.b_stride, d.b_mn != 0, d.n, b_planes);
+  if (d.kind == kFusedRaggedCols && a_planes > 1) jobs[0].offsets = d.offsets;
   cudaError_t e = cudaSuccess;
   if (a_bytes + b_bytes > 0) {
     e = copies.get(a_bytes + b_bytes, stream);
@@ -196,7 +204,12 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
     if (e != cudaSuccess) return e;
   }
 
-  const Choice choice = choose(d);
+  const void* const residual = d.beta != 0.0 ? d.d : nullptr;
+  const long long c_planes = d.kind == kFusedRaggedCols ? 1 : d.problems;
+  const bool vec = d.m % 8 == 0 && aligned16(d.c, d.ldc, c_planes, d.c_stride, elem_size(d.c_type)) &&
+                   (!residual || aligned16(residual, d.ldd, c_planes, d.d_stride, elem_size(d.d_type))) &&
+                   (!d.z || aligned16(d.z, d.ldz, c_planes, d.z_stride, 2));
+  const Choice choice = choose(d, vec);
   const FusedVariant& t = kFusedTable[choice.variant];
   FusedParams p = {};
   p.status = tc_status_device();
@@ -226,20 +239,16 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   p.act = d.act;
   p.grad = d.grad;
   p.c = d.c; p.ldc = d.ldc; p.c_stride = d.c_stride;
-  p.d = d.beta != 0.0 ? d.d : nullptr; p.ldd = d.ldd; p.d_stride = d.d_stride;
+  p.d = residual; p.ldd = d.ldd; p.d_stride = d.d_stride;
   p.z = d.z; p.ldz = d.ldz; p.z_stride = d.z_stride;
   p.hint_a = p.hint_b = 2;
+  p.vec = vec ? 1 : 0;
 
   CUtensorMap maps[4];
   std::memset(maps + 2, 0, 2 * sizeof(CUtensorMap));
   if (!encode_operand_map(&maps[0], 2, r.a, d.m, d.k, r.lda, d.a_mn != 0, 128, a_planes, r.a_stride) ||
       !encode_operand_map(&maps[1], 2, r.b, d.n, d.k, r.ldb, d.b_mn != 0, t.bn / t.ctas, b_planes, r.b_stride))
     return cudaErrorInvalidValue;
-  const long long c_planes = d.kind == kFusedRaggedCols ? 1 : d.problems;
-  p.vec = d.m % 8 == 0 && aligned16(d.c, d.ldc, c_planes, d.c_stride, elem_size(d.c_type)) &&
-          (!p.d || aligned16(p.d, d.ldd, c_planes, d.d_stride, elem_size(d.d_type))) &&
-          (!p.z || aligned16(p.z, d.ldz, c_planes, d.z_stride, 2));
-
   const bool reads_z = p.z && d.grad;
   if (p.vec && choice.split == 1 && (p.d || reads_z))
     p.prefetch = (!p.d || encode_prefetch_map(&maps[2], elem_size(d.d_type), p.d, d.m, d.n, d.ldd, c_planes, d.d_stride)) &&

@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackPair pair)
   const long long line = block / segments;
   const int x0 = static_cast<int>(block % segments) * (kPackThreads * kPackVec);
   const long long plane = line / job.two, in_plane = line - plane * job.two;
+  if (job.offsets != nullptr && job.offsets[plane + 1] <= job.offsets[plane]) return;
   const unsigned short* const src = static_cast<const unsigned short*>(job.src) + plane * job.src_stride + in_plane * job.src_ld + x0;
   const long long left = job.one - x0;
 #pragma unroll

@@ -8,11 +8,13 @@ namespace b200 {
 
 // Copies `planes` matrices of `two` lines of `one` contiguous 2-byte elements each (any alignment, leading dimension and
 // plane stride) to lines of `pitch` elements (a multiple of 8, the rest zero), planes two * pitch apart. Two jobs go in one
-// launch; one with planes == 0 is skipped.
+// launch; one with planes == 0 is skipped. With `offsets` (device, planes + 1 of them) a plane whose group has no rows is
+// left out.
 struct PackJob {
   const void* src;
   void* dst;
   long long one, two, planes, src_ld, src_stride, pitch;
+  const long long* offsets;
 };
 cudaError_t launch_pack(const PackJob (&jobs)[2], cudaStream_t stream);
 

@@ -854,7 +854,8 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           }
           if (!ok) break;
           __syncwarp();
-          if (lane == 0) {
+          // (the arrival is a release that waits for the stores above, so the last tile goes without)
+          if (lane == 0 && tile + tile_step < num_tiles) {
             for (int q = 0; q < split; ++q) mbar_arrive_remote(map_to_cta(sums_free, q));
           }
           if (p.partial != nullptr && in_rows)
