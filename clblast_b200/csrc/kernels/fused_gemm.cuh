@@ -264,6 +264,10 @@ __device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity,
   return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
 }
 
+// The same value as the compiler sees it in every lane: what the tensor and TMA units take from uniform registers is
+// computed there if it stems from such values, and moved there operand by operand if not.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
+
 // One tile of the walk.
 struct Tile {
   int z;             // problem
@@ -503,8 +507,14 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       uint32_t phase = 0;
       bool ok = true;
       const uint64_t pol_a = l2_policy(p.hint_a), pol_b = l2_policy(p.hint_b);
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-        const Tile t = locate<BN>(p, tile, start, tiles);
+      const int last_tile = uniform(num_tiles);
+      for (int tile = first_tile; tile < last_tile && ok; tile += tile_step) {
+        Tile t = locate<BN>(p, tile, start, tiles);
+        t.z = uniform(t.z);
+        t.tm = uniform(t.tm);
+        t.col0 = uniform(t.col0);
+        t.k0 = uniform(t.k0);
+        t.k_len = uniform(t.k_len);
         int kb0, kb1;
         k_range(t, kb0, kb1);
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -570,15 +580,18 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       int local = 0;
       uint32_t tail_phases = 0;
       bool ok = true;
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++local) {
-        const Tile t = locate<BN>(p, tile, start, tiles);
+      const int last_tile = uniform(num_tiles);
+      const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(tmem_base)));
+      for (int tile = first_tile; tile < last_tile && ok; tile += tile_step, ++local) {
+        Tile t = locate<BN>(p, tile, start, tiles);
+        t.k_len = uniform(t.k_len);
         int kb0, kb1;
         k_range(t, kb0, kb1);
         int acc = acc_of(local);
         ok = wait(acc_empty_bar(acc), acc_parity(local) ^ 1u, 2u);
         if (!ok) break;
         tcgen05_fence_after();
-        uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        uint32_t d_tmem = tmem + static_cast<uint32_t>(acc * BN);
         int first_kb = kb0;  // first block of the current accumulator
         for (int kb = kb0; kb < kb1; ++kb) {
           if (CHUNKED && kb - first_kb == kChunk) {  // hand this accumulator over and go on in the other one
@@ -590,7 +603,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             ok = wait(acc_empty_bar(acc), acc_parity(local) ^ 1u, 2u);
             if (!ok) break;
             tcgen05_fence_after();
-            d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+            d_tmem = tmem + static_cast<uint32_t>(acc * BN);
           }
           ok = wait(full_bar(stage), phase, 3u);
           if (!ok) break;

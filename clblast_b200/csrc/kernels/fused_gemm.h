@@ -60,8 +60,8 @@ struct FusedVariant {
 #else
 #define B200_HD
 #endif
-// With more warps the long chains of an epilogue hide each other; on the widest tiles the MMAs leave time enough.
-B200_HD constexpr int fused_groups(int bn) { return bn == 256 ? 2 : (bn == 128 ? 4 : (bn == 64 ? 2 : 1)); }
+// (Four groups on 128 columns halve the registers of a thread: 25 % slower where stores go element by element.)
+B200_HD constexpr int fused_groups(int bn) { return bn >= 64 ? 2 : 1; }
 B200_HD constexpr int fused_threads(int bn) { return 128 + 128 * fused_groups(bn); }
 // Shared memory of an epilogue warp: a block of 16 columns x 32 rows of C or D and one of Z.
 B200_HD constexpr int fused_warp_bytes(bool single, bool aux) { return (single ? 2048 : 1024) + (aux ? 1024 : 0); }
