@@ -534,7 +534,7 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
     const void* const from = x[i & 1];
     FusedDesc f = {};
     f.type = f.c_type = f.d_type = 16;
-    f.kind = kFusedPlain; f.problems = batch; f.act = kActIdentityCode;
+    f.kind = kFusedPlain; f.problems = batch; f.act = kActIdentityCode; f.chained = 1;
     // A = X X^T
     f.m = f.n = side; f.k = gram_of_lines ? pitch : lines;
     f.a = f.b = from; f.lda = f.ldb = pitch; f.a_stride = f.b_stride = lines * pitch;
@@ -573,7 +573,114 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
   return e;
 }
 
-// The same in single precision on the SGEMM kernels; a product that adds to another matrix adds to a copy of it.
+// Largest singular value that a step can leave, given the largest before it: the polynomial's extreme on [0, s], sampled
+// densely enough (its slope is bounded by the coefficients) and with a margin for rounding.
+double step_bound(double s, const double* q) {
+  double most = 0.0;
+  for (int i = 0; i <= 2000; ++i) {
+    const double x = s * i / 2000.0, y = std::fabs(x * (q[0] + x * x * (q[1] + x * x * q[2])));
+    if (!(y <= most)) most = y;
+  }
+  return 1.02 * most;
+}
+// The power of two that brings a matrix with entries up to `bound` under 2^15, half of half precision's largest number.
+double parts_scale(double bound) {
+  if (!(bound > 0.0)) return 1.0;
+  int e = 0;
+  std::frexp(bound, &e);  // bound < 2^e
+  e = 15 - e;
+  return std::ldexp(1.0, e > 13 ? 13 : e);
+}
+
+// The same iteration in single precision: every matrix is kept as a sum of two halves, hi + lo, about 22 bits, scaled by
+// powers of two so that neither part leaves half's range, and a product takes three terms on the 16-bit tensor cores
+// (three times their time, where the single-precision kernels take six). Sums run in fp32 as for every result in single
+// precision. Returns cudaErrorNotSupported when the coefficients let the iteration grow beyond the scales' reach.
+cudaError_t newton_schulz_parts(long long one, long long two, double alpha, const void* a, long long a_ld, long long a_stride,
+                                void* b, long long b_ld, long long b_stride, long long batch, int steps,
+                                const double* coefficients, bool per_step, double eps, cudaStream_t s) {
+  double bound = 1.02;  // of a normalised matrix
+  for (int i = 0; i < steps; ++i) {
+    const double* const q = coefficients + (per_step ? 3 * i : 0);
+    const double bracket = std::fabs(q[1]) * bound * bound + std::fabs(q[2]) * bound * bound * bound * bound;
+    if (!(bracket < 4096.0)) return cudaErrorNotSupported;
+    bound = step_bound(bound, q);
+    if (!(bound < 64.0)) return cudaErrorNotSupported;
+  }
+  const bool gram_of_lines = one > two;
+  const long long pitch = (one + 7) / 8 * 8, lines = (two + 7) / 8 * 8;
+  const long long side = gram_of_lines ? lines : pitch;
+  const long long x_plane = lines * pitch, g_plane = side * side;
+  const auto round = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t x_bytes = round(static_cast<size_t>(batch) * x_plane * 4), g_bytes = round(static_cast<size_t>(batch) * g_plane * 4);
+  const size_t s_bytes = round(static_cast<size_t>(batch) * kNormBlocks * sizeof(double));
+  PoolScratch scratch;
+  cudaError_t e = scratch.get(2 * x_bytes + 2 * g_bytes + s_bytes, s);
+  if (e != cudaSuccess) return e;
+  unsigned char* const base = scratch.ptr();
+  void* x[2] = {base, base + x_bytes};
+  void* const gram = base + 2 * x_bytes;
+  void* const poly = base + 2 * x_bytes + g_bytes;
+  bound = 1.02;
+  double x_scale = parts_scale(bound);
+  NormaliseJob norm = {};
+  norm.type = 32; norm.x_type = kParts; norm.g = a; norm.one = one; norm.two = two; norm.ld = a_ld; norm.stride = a_stride;
+  norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.lines = lines; norm.eps = eps; norm.scale = x_scale;
+  norm.sums = reinterpret_cast<double*>(base + 2 * x_bytes + 2 * g_bytes);
+  e = launch_normalise(norm, s);
+  const char* name = "none";
+  for (int i = 0; i < steps && e == cudaSuccess; ++i) {
+    const double* const q = coefficients + (per_step ? 3 * i : 0);
+    const double g_scale = parts_scale(bound * bound);
+    const double p_scale = parts_scale(std::fabs(q[1]) * bound * bound + std::fabs(q[2]) * bound * bound * bound * bound);
+    bound = step_bound(bound, q);
+    const double next_scale = parts_scale(bound);
+    const void* const from = x[i & 1];
+    FusedDesc f = {};
+    f.type = f.c_type = f.d_type = 16;
+    f.kind = kFusedPlain; f.problems = batch; f.act = kActIdentityCode; f.parts = 1; f.chained = 1;
+    // G = X X^T
+    f.m = f.n = side; f.k = gram_of_lines ? pitch : lines;
+    f.a = f.b = from; f.lda = f.ldb = pitch; f.a_stride = f.b_stride = x_plane;
+    f.a_mn = f.b_mn = gram_of_lines ? 0 : 1;
+    f.alpha = g_scale / (x_scale * x_scale); f.tri = 1;
+    f.c = gram; f.ldc = side; f.c_stride = g_plane;
+    e = launch_fused(f, s, &name);
+    if (e != cudaSuccess) break;
+    // b G + c G G
+    f.k = side;
+    f.a = f.b = gram; f.lda = f.ldb = side; f.a_stride = f.b_stride = g_plane;
+    f.a_mn = f.b_mn = 0;
+    f.alpha = p_scale * q[2] / (g_scale * g_scale);
+    f.beta = p_scale * q[1] / g_scale; f.d = gram; f.ldd = side; f.d_stride = g_plane;
+    f.c = poly;
+    e = launch_fused(f, s, &name);
+    if (e != cudaSuccess) break;
+    // a X + (.) X
+    f.tri = 0;
+    f.m = pitch; f.n = lines; f.k = side;
+    if (gram_of_lines) {
+      f.a = from; f.lda = pitch; f.a_stride = x_plane; f.a_mn = 1;
+      f.b = poly; f.ldb = side; f.b_stride = g_plane; f.b_mn = 0;
+    } else {
+      f.a = poly; f.lda = side; f.a_stride = g_plane; f.a_mn = 0;
+      f.b = from; f.ldb = pitch; f.b_stride = x_plane; f.b_mn = 0;
+    }
+    f.alpha = next_scale / (p_scale * x_scale);
+    f.beta = next_scale * q[0] / x_scale; f.d = from; f.ldd = pitch; f.d_stride = x_plane;
+    f.c = x[(i + 1) & 1]; f.ldc = pitch; f.c_stride = x_plane;
+    e = launch_fused(f, s, &name);
+    x_scale = next_scale;
+  }
+  if (e != cudaSuccess) return e;
+  JoinJob join = {};
+  join.x = x[steps & 1]; join.lines = lines; join.pitch = pitch;
+  join.b = static_cast<float*>(b); join.one = one; join.two = two; join.ld = b_ld; join.stride = b_stride; join.batch = batch;
+  join.scale = static_cast<float>(alpha / x_scale);
+  return launch_join(join, s);
+}
+
+// The same on the SGEMM kernels; a product that adds to another matrix adds to a copy of it.
 cudaError_t newton_schulz_single(long long one, long long two, double alpha, const void* a, long long a_ld,
                                  long long a_stride, void* b, long long b_ld, long long b_stride, long long batch, int steps,
                                  const double* coefficients, bool per_step, double eps, cudaStream_t s) {
@@ -666,13 +773,21 @@ extern "C" int b200blas_newton_schulz(int dtype, int layout, size_t m, size_t n,
     const char* name = "newton_schulz_single";
     const bool per_step = coefficient_count > 1;
     cudaError_t e;
-    if (dtype == 32)
-      e = newton_schulz_single(static_cast<long long>(one), static_cast<long long>(two), alpha, at(a, a_offset, elem),
-                               static_cast<long long>(a_ld), static_cast<long long>(a_stride), at(b, b_offset, elem),
-                               static_cast<long long>(b_ld), static_cast<long long>(b_stride),
-                               static_cast<long long>(batch_count), static_cast<int>(steps), coefficients, per_step, epsilon, s);
-    else
-      e = newton_schulz_half(dtype, static_cast<long long>(one), static_cast<long long>(two), alpha, at(a, a_offset, elem),
+    if (dtype == 32) {
+      const auto run = [&](auto* f) {
+        return f(static_cast<long long>(one), static_cast<long long>(two), alpha, at(a, a_offset, elem),
+                 static_cast<long long>(a_ld), static_cast<long long>(a_stride), at(b, b_offset, elem),
+                 static_cast<long long>(b_ld), static_cast<long long>(b_stride), static_cast<long long>(batch_count),
+                 static_cast<int>(steps), coefficients, per_step, epsilon, s);
+      };
+      name = "newton_schulz_parts";
+      e = run(&newton_schulz_parts);
+      if (e == cudaErrorNotSupported) {
+        name = "newton_schulz_single";
+        e = run(&newton_schulz_single);
+      }
+    }
+    else e = newton_schulz_half(dtype, static_cast<long long>(one), static_cast<long long>(two), alpha, at(a, a_offset, elem),
                              static_cast<long long>(a_ld), static_cast<long long>(a_stride), at(b, b_offset, elem),
                              static_cast<long long>(b_ld), static_cast<long long>(b_stride),
                              static_cast<long long>(batch_count), static_cast<int>(steps), coefficients, per_step, epsilon, s, &name);

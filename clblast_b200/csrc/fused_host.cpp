@@ -63,7 +63,8 @@ bool variant_fits(const FusedDesc& d, int v, int split) {
   if (d.b_mn && t.bn / t.ctas < 64) return false;                               // a 128-byte row is 64 columns
   if (d.tri && t.ctas * 128 != t.bn) return false;                               // square tiles meet their mirror image
   if (split > 1 && (t.bn / split) % 4 != 0) return false;
-  if (split > 1 && d.tri) return false;
+  if (split > 1 && (d.tri || d.parts)) return false;
+  if (d.parts && v != 0 && v != 2) return false;
   return true;
 }
 
@@ -83,7 +84,7 @@ double estimate(const FusedDesc& d, int v, int split, bool vec) {
   static constexpr double kBlock[kFusedVariants] = {537.0, 569.0, 476.0, 507.0, 510.0, 700.0};
   const FusedVariant& t = kFusedTable[v];
   const auto whole = [](double x) { return std::ceil(x); };
-  const bool single = d.c_type == 32;
+  const bool single = d.c_type == 32 || d.parts;
   const double rows = static_cast<double>(d.m), cols = static_cast<double>(d.n);
   const double tm = whole(rows / (128 * t.ctas));
   const double active = static_cast<double>(d.problems < d.n ? d.problems : d.n);  // groups that can have vectors
@@ -98,7 +99,7 @@ double estimate(const FusedDesc& d, int v, int split, bool vec) {
   const double block = kBlock[v] * (single && t.bn == 256 ? 1.7 : 1.0);
   const double load = t.stage_bytes / 70.0;
   const double waves = whole(tiles / resident_teams(t.ctas * split));
-  const double main = whole(whole(k / 64.0) / split) * (block > load ? block : load) + 1450.0;
+  const double main = whole((d.parts ? 3.0 : 1.0) * whole(k / 64.0) / split) * (block > load ? block : load) + 1450.0;
   // per column of a tile
   const bool reads_z = d.z != nullptr && d.grad, writes_z = d.z != nullptr && !d.grad;
   const bool adds = d.beta != 0.0 && d.d != nullptr;
@@ -167,8 +168,9 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
     return launch_few_rows(job, stream);
   }
   // an operand with stride 0 is shared by all problems
-  const long long a_planes = d.kind == kFusedRaggedInner || d.a_stride == 0 ? 1 : d.problems;
-  const long long b_planes = d.kind == kFusedPlain && d.b_stride != 0 ? d.problems : 1;
+  const long long per_problem = d.parts ? 2 : 1;
+  const long long a_planes = d.kind == kFusedRaggedInner || d.a_stride == 0 ? 1 : d.problems * per_problem;
+  const long long b_planes = d.kind == kFusedPlain && d.b_stride != 0 ? d.problems * per_problem : 1;
   // Operands that TMA cannot address are copied once to an aligned pitch.
   PoolScratch copies, partial;
   FusedDesc r = d;
@@ -205,7 +207,7 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   }
 
   const void* const residual = d.beta != 0.0 ? d.d : nullptr;
-  const long long c_planes = d.kind == kFusedRaggedCols ? 1 : d.problems;
+  const long long c_planes = d.kind == kFusedRaggedCols ? 1 : d.problems * per_problem;
   const bool vec = d.m % 8 == 0 && aligned16(d.c, d.ldc, c_planes, d.c_stride, elem_size(d.c_type)) &&
                    (!residual || aligned16(residual, d.ldd, c_planes, d.d_stride, elem_size(d.d_type))) &&
                    (!d.z || aligned16(d.z, d.ldz, c_planes, d.z_stride, 2));
@@ -223,6 +225,8 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   p.tiles_n = static_cast<int>((d.n + t.bn - 1) / t.bn);
   p.raster = t.ctas == 2 ? 8 : 16;
   p.tri = d.tri;
+  p.parts = d.parts;
+  p.chained = d.chained;
   p.a_mn = d.a_mn;
   p.b_mn = d.b_mn;
   const unsigned format = d.type == 16 ? 0u : 1u;  // fp32 accumulator; f16 or bf16 operands
@@ -253,14 +257,15 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   if (p.vec && choice.split == 1 && (p.d || reads_z))
     p.prefetch = (!p.d || encode_prefetch_map(&maps[2], elem_size(d.d_type), p.d, d.m, d.n, d.ldd, c_planes, d.d_stride)) &&
                  (!reads_z || encode_prefetch_map(&maps[3], 2, p.z, d.m, d.n, d.ldz, c_planes, d.z_stride));
-  if (d.tri && (!p.vec || p.z || d.n != d.m)) return cudaErrorInvalidValue;  // mirrored with 16-byte stores only
+  if ((d.tri || d.parts) && (!p.vec || p.z)) return cudaErrorInvalidValue;  // 16-byte stores only
+  if (d.tri && d.n != d.m) return cudaErrorInvalidValue;
 
   const long long col_tiles = column_tiles(d, t.bn);
   long long tiles = col_tiles * p.tiles_m;
   if (d.kind != kFusedRaggedCols) tiles *= d.problems;
   if (d.tri) tiles = static_cast<long long>(p.tiles_m) * (p.tiles_m + 1) / 2 * d.problems;
   if (tiles > 0x3FFFFFFF) return cudaErrorInvalidValue;
-  const bool single = d.c_type == 32;
+  const bool single = d.c_type == 32 || d.parts;  // sums beside the accumulators, blocks of four bytes
   const int lines_per_tile = fused_groups(t.bn) * choice.split;
   if (d.bias_grad != nullptr) {
     e = partial.get(static_cast<size_t>(col_tiles) * lines_per_tile * d.m * sizeof(float), stream);

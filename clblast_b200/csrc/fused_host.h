@@ -19,7 +19,8 @@ struct FusedDesc {
   const void* b; long long ldb, b_stride; int b_mn;
   double alpha, beta;
   const void* bias; long long bias_stride;
-  int act, grad, tri;
+  int act, grad, tri, parts;   // parts: all matrices are pairs of halves, planes `stride` apart, problems two of them
+  int chained;                 // one of a chain of launches that read each other's results
   const void* d; long long ldd, d_stride;
   void* z; long long ldz, z_stride;
   void* c; long long ldc, c_stride;

@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormaliseJob job) {
   }
 }
 
-template <class T, class X>
+template <class T, class X, bool PARTS>
 __global__ void __launch_bounds__(256) scale_kernel(const NormaliseJob job, int blocks) {
   __shared__ double factor;
   if (threadIdx.x < 32) {
@@ -207,12 +207,28 @@ __global__ void __launch_bounds__(256) scale_kernel(const NormaliseJob job, int 
   __syncthreads();
   const double f = factor;
   const T* const g = static_cast<const T*>(job.g) + static_cast<long long>(blockIdx.y) * job.stride;
-  X* const x = static_cast<X*>(job.x) + static_cast<long long>(blockIdx.y) * job.lines * job.pitch;
+  X* const x = static_cast<X*>(job.x) + static_cast<long long>(blockIdx.y) * (PARTS ? 2 : 1) * job.lines * job.pitch;
   for (long long line = blockIdx.x; line < job.lines; line += gridDim.x) {
     const T* const row = g + line * job.ld;
 #pragma unroll 4
-    for (long long i = threadIdx.x; i < job.pitch; i += 256)
-      x[line * job.pitch + i] = from_float<X>(i < job.one && line < job.two ? static_cast<float>(static_cast<double>(to_float(row[i])) * f) : 0.f);
+    for (long long i = threadIdx.x; i < job.pitch; i += 256) {
+      const float v = i < job.one && line < job.two ? static_cast<float>(static_cast<double>(to_float(row[i])) * f) : 0.f;
+      const X high = from_float<X>(v);
+      x[line * job.pitch + i] = high;
+      if (PARTS) x[(job.lines + line) * job.pitch + i] = from_float<X>(v - to_float(high));
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) join_kernel(const JoinJob job) {
+  const __half* const x = static_cast<const __half*>(job.x) + static_cast<long long>(blockIdx.y) * 2 * job.lines * job.pitch;
+  float* const b = job.b + static_cast<long long>(blockIdx.y) * job.stride;
+  for (long long line = blockIdx.x; line < job.two; line += gridDim.x) {
+    const __half* const high = x + line * job.pitch;
+    const __half* const low = high + job.lines * job.pitch;
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < job.one; i += 256)
+      b[line * job.ld + i] = job.scale * (__half2float(high[i]) + __half2float(low[i]));
   }
 }
 
@@ -316,10 +332,18 @@ cudaError_t launch_normalise(const NormaliseJob& job, cudaStream_t stream) {
   return by_type(job.type, [&](auto* tag) {
     using T = typename std::remove_pointer<decltype(tag)>::type;
     norm_kernel<T><<<grid, 256, 0, stream>>>(job);
-    if (job.x_type == 16) scale_kernel<T, __half><<<scale_grid, 256, 0, stream>>>(job, blocks);
-    else scale_kernel<T, float><<<scale_grid, 256, 0, stream>>>(job, blocks);
+    if (job.x_type == 16) scale_kernel<T, __half, false><<<scale_grid, 256, 0, stream>>>(job, blocks);
+    else if (job.x_type == kParts) scale_kernel<T, __half, true><<<scale_grid, 256, 0, stream>>>(job, blocks);
+    else scale_kernel<T, float, false><<<scale_grid, 256, 0, stream>>>(job, blocks);
     return cudaGetLastError();
   });
+}
+
+cudaError_t launch_join(const JoinJob& job, cudaStream_t stream) {
+  if (job.batch > 65535) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(job.two < 4096 ? job.two : 4096), static_cast<unsigned>(job.batch));
+  join_kernel<<<grid, 256, 0, stream>>>(job);
+  return cudaGetLastError();
 }
 
 }  // namespace b200

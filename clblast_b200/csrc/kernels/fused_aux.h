@@ -55,8 +55,9 @@ cudaError_t launch_sum_partials(const SumJob& job, cudaStream_t stream);
 
 // Newton-Schulz input: X = scale * G / (|G|_F + eps) for `batch` matrices (lines of `one` contiguous elements, `two`
 // lines), X dense with `lines` lines of `pitch` elements (what G does not have is zero), planes lines * pitch apart, in half (x_type 16) or single
-// (32) precision. `sums` is scratch of norm_scratch_doubles(batch) doubles.
+// (32) precision, or (x_type kParts) as a sum of two halves in consecutive planes. `sums` is scratch of norm_scratch_doubles(batch) doubles.
 constexpr int kNormBlocks = 256;  // blocks per matrix
+constexpr int kParts = 1616;
 struct NormaliseJob {
   int type, x_type;
   const void* g;
@@ -67,5 +68,15 @@ struct NormaliseJob {
   double* sums;
 };
 cudaError_t launch_normalise(const NormaliseJob& job, cudaStream_t stream);
+
+// B = scale * (hi + lo): `batch` matrices from planes 2z and 2z + 1 of x (lines x pitch halves each) to single precision.
+struct JoinJob {
+  const void* x;
+  long long lines, pitch;
+  float* b;
+  long long one, two, ld, stride, batch;
+  float scale;
+};
+cudaError_t launch_join(const JoinJob& job, cudaStream_t stream);
 
 }  // namespace b200

@@ -24,7 +24,7 @@
 //
 // Sums for results in single precision: the tensor cores cut off instead of rounding when they add to an accumulator, an
 // error of about 4e-8 of the result per 16 inner elements that all points towards zero. Results in 16 bits do not see it.
-// For the others an accumulator takes kChunk blocks at most and is then added, rounded, to sums in further columns of
+// For the others an accumulator takes a few blocks at most and is then added, rounded, to sums in further columns of
 // tensor memory (which the widest tile has room for only with one accumulator instead of two).
 //
 // All waits are bounded; on expiry a code is left in the status word and every role leaves its loop.
@@ -49,7 +49,9 @@ using namespace tc;
 
 constexpr int BM = 128;   // rows of op(A) per CTA
 constexpr int BK = 64;    // inner elements per stage: 128-byte swizzle rows
-constexpr int kChunk = 4; // operand stages (64 inner elements each) per accumulator for results in single precision
+// operand stages (64 inner elements each) per accumulator: results in single precision; sums of two halves, whose users
+// (the Newton-Schulz steps) amplify an error that all entries share
+constexpr int kChunkSingle = 4, kChunkParts = 2;
 
 // Two values rounded to 16 bits in one word (the packed conversion runs on the full-rate pipe, the single one does not).
 template <class E>
@@ -239,7 +241,7 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(one)::"memory");
   return one != 0;
 }
-// Bounded wait of a whole converged warp: one lane polls (32 lanes polling cost the MMA issuer 150 us of 920 at 8192^3).
+// Bounded wait of a whole converged warp: one lane polls.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned code,
                                           unsigned int* status) {
   int ok = 1;
@@ -256,6 +258,14 @@ __device__ __forceinline__ bool warp_wait_relaxed(uint32_t bar, uint32_t parity,
     ok = mbar_wait(bar, parity, abort_flag, code, status) ? 1 : 0;
   }
   return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
+}
+// The same for the inner loops of the producer and of the MMA issuer: a try by all lanes and a vote take 30 ns less per
+// stage than one lane's poll and its broadcast where the barrier is ready, as it mostly is (128 x 128 tiles 344 -> 303 ns).
+__device__ __forceinline__ bool loop_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned code,
+                                          unsigned int* status) {
+  const bool ready = mbar_try_wait(bar, parity);
+  if (__all_sync(0xFFFFFFFFu, ready)) return true;
+  return warp_wait(bar, parity, abort_flag, code, status);
 }
 __device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned code,
                                                   unsigned int* status) {
@@ -353,7 +363,10 @@ __device__ __forceinline__ Tile locate(const FusedParams& p, int tile, const int
 
 // What the epilogue is compiled for. The first two need 16-byte accesses to C, D and Z; the third takes everything else,
 // tiles shared by a cluster included.
-enum FusedMode : int { kModeForward = 0, kModeGrad = 1, kModeGeneral = 2 };
+// The fourth multiplies matrices that are kept as a sum of two halves, hi + lo: about 22 bits. Planes 2z and 2z + 1 of every
+// matrix are the two parts of problem z. The product takes three terms one after the other, hi hi + hi lo + lo hi (lo lo
+// lies below the rounding), C and D are split and joined in the epilogue.
+enum FusedMode : int { kModeForward = 0, kModeGrad = 1, kModeGeneral = 2, kModeParts = 3 };
 
 template <int CTAS, int BN, class T, class DT, class OT, int MODE>
 __global__ void __launch_bounds__(fused_threads(BN), 1)
@@ -361,7 +374,8 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                   const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_z,
                   const FusedParams p) {
   static_assert(sizeof(DT) == sizeof(OT), "D and C share the staging buffers");
-  constexpr bool CHUNKED = sizeof(OT) == 4;
+  constexpr bool CHUNKED = sizeof(OT) == 4 || MODE == kModeParts;  // sums beyond what the accumulators give
+  constexpr int CHUNK = MODE == kModeParts ? kChunkParts : kChunkSingle;
   constexpr int EG = fused_groups(BN);
   constexpr int CB = 16;  // columns per epilogue block
   constexpr int B_ROWS = BN / CTAS;
@@ -429,7 +443,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   }
   // this CTA's share of a tile's inner blocks
   auto k_range = [&](const Tile& t, int& kb0, int& kb1) {
-    const int blocks = (t.k_len + BK - 1) / BK;
+    const int blocks = (t.k_len + BK - 1) / BK * (MODE == kModeParts ? 3 : 1);
     if (split > 1) {
       kb0 = blocks * static_cast<int>(rank) / split;
       kb1 = blocks * (static_cast<int>(rank) + 1) / split;
@@ -444,7 +458,14 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   auto issue_block = [&](const Tile& t, int kb, int stage, uint64_t pol_a, uint64_t pol_b) {
     const int a_row0 = (t.tm * CTAS + (CTAS == 2 ? static_cast<int>(rank) : 0)) * BM;
     const int b_row0 = t.col0 + (CTAS == 2 ? static_cast<int>(rank) * B_ROWS : 0);
-    const int az = p.a_batched ? t.z : 0, bz = p.b_batched ? t.z : 0;
+    int az = p.a_batched ? t.z : 0, bz = p.b_batched ? t.z : 0;
+    if constexpr (MODE == kModeParts) {
+      const int per_term = (t.k_len + BK - 1) / BK;
+      const int term = kb >= 2 * per_term ? 2 : (kb >= per_term ? 1 : 0);
+      kb -= term * per_term;
+      az = 2 * t.z + (term == 2 ? 1 : 0);
+      bz = 2 * t.z + (term == 1 ? 1 : 0);
+    }
     const uint32_t a_dst = tiles_base + stage * STAGE_BYTES;
     const uint32_t b_dst = a_dst + A_BYTES;
     const int x = t.k0 + kb * BK;
@@ -489,6 +510,11 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   }
   if (warp == 2 && p.kind != kFusedPlain)
     build_table(p.offsets, p.problems, p.kind == kFusedRaggedCols ? p.n : p.k, BN, start, tiles);
+  // A launch that follows another one closely is set up under the end of that one; from here on its results are read.
+  if (p.chained) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+  }
   tcgen05_fence_before();
   __syncthreads();
   if (CTAS == 2 || split > 1) cluster_sync_all();  // all barriers exist before anyone signals across CTAs
@@ -518,7 +544,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         int kb0, kb1;
         k_range(t, kb0, kb1);
         for (int kb = kb0; kb < kb1; ++kb) {
-          ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, 1u, p.status);
+          ok = loop_wait(empty_bar(stage), phase ^ 1u, abort_flag, 1u, p.status);
           if (!ok) break;
           if (elect_one()) issue_block(t, kb, stage, pol_a, pol_b);
           __syncwarp();
@@ -564,7 +590,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
     // ---- MMA issuer (of a pair: the leader, for both SMs): the warp walks along, one lane issues ----
     if (CTAS == 1 || rank == 0) {
-      auto wait = [&](uint32_t bar, uint32_t parity, unsigned code) { return warp_wait(bar, parity, abort_flag, code, p.status); };
+      auto wait = [&](uint32_t bar, uint32_t parity, unsigned code) { return loop_wait(bar, parity, abort_flag, code, p.status); };
       auto commit = [&](uint32_t bar) {
         if constexpr (CTAS == 2) umma_commit_pair(bar);
         else umma_commit(bar);
@@ -594,7 +620,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         uint32_t d_tmem = tmem + static_cast<uint32_t>(acc * BN);
         int first_kb = kb0;  // first block of the current accumulator
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (CHUNKED && kb - first_kb == kChunk) {  // hand this accumulator over and go on in the other one
+          if (CHUNKED && kb - first_kb == CHUNK) {  // hand this accumulator over and go on in the other one
             if (elect_one()) commit(acc_full_bar(acc));
             __syncwarp();
             ++local;
@@ -649,12 +675,13 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         for (int spin = 0; spin < 20000 && *progress < n - 1 && !*abort_flag; ++spin) __nanosleep(200);
         const Tile t = locate<BN>(p, tile, start, tiles);
         const int row0 = (t.tm * CTAS + (CTAS == 2 ? static_cast<int>(rank) : 0)) * BM;
-        const int zc = p.kind == kFusedRaggedCols ? 0 : t.z;
+        const int zc = p.kind == kFusedRaggedCols ? 0 : (MODE == kModeParts ? 2 * t.z : t.z);
         if (row0 < p.m) {
 #pragma unroll
           for (int c = 0; c < BN; c += 32) {
             if (t.col0 + c >= t.col_end) break;
             if (p.d != nullptr) tma_prefetch_3d(&map_d, row0, t.col0 + c, zc);
+            if (MODE == kModeParts && p.d != nullptr) tma_prefetch_3d(&map_d, row0, t.col0 + c, zc + 1);
             if (MODE == kModeGrad && aux) tma_prefetch_3d(&map_z, row0, t.col0 + c, zc);
           }
         }
@@ -685,7 +712,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       const int row = cta_row0 + row_in_cta;
       const int rows_left = p.m - warp_row0;  // may be negative: the tile's last warps may lie wholly below C
       const bool in_rows = row < p.m;
-      const int zc = p.kind == kFusedRaggedCols ? 0 : t.z;  // plane of C, D, Z
+      const int zc = p.kind == kFusedRaggedCols ? 0 : (MODE == kModeParts ? 2 * t.z : t.z);  // plane of C, D, Z
       const float bias = (p.bias != nullptr && in_rows) ? to_float(static_cast<const T*>(p.bias)[t.z * p.bias_stride + row]) : 0.f;
       const int group_col0 = t.col0 + group * GROUP_COLS;
       const int group_cols = t.col_end - group_col0;  // columns that exist from this group's first one on
@@ -716,7 +743,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       // Results in single precision: the accumulators are added up in further columns, which only this warp touches.
       const uint32_t sums_tmem = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + SUMS_AT + static_cast<uint32_t>(group * GROUP_COLS);
       if constexpr (CHUNKED) {
-        const int chunks = empty ? 1 : (kb1 - kb0 + kChunk - 1) / kChunk;
+        const int chunks = empty ? 1 : (kb1 - kb0 + CHUNK - 1) / CHUNK;
         for (int c = 0; c < chunks; ++c) {
           ok = wait_accumulator(local);
           if (!ok) break;
@@ -925,10 +952,12 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
       if constexpr (MODE != kModeGeneral) {
         // D and Z of a block are requested while the block before it is worked on
-        BlockD d_next = {};
+        BlockD d_next = {}, d_low = {};
         BlockZ z_next = {};
         auto request = [&](int cb) {
           if (has_d) d_next.load(d_ptr + static_cast<long long>(cb * CB) * p.ldd, p.ldd, rows_left, group_cols - cb * CB, lane);
+          if (MODE == kModeParts && has_d)
+            d_low.load(d_ptr + p.d_stride + static_cast<long long>(cb * CB) * p.ldd, p.ldd, rows_left, group_cols - cb * CB, lane);
           if (MODE == kModeGrad && aux) z_next.load(z_ptr + static_cast<long long>(cb * CB) * p.ldz, p.ldz, rows_left, group_cols - cb * CB, lane);
         };
         uint8_t* const own = staging + (warp - 4) * fused_warp_bytes(CHUNKED, aux);
@@ -943,6 +972,11 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             d_next.to_rows(turn_c, add, lane);
 #pragma unroll
             for (int j = 0; j < CB; ++j) v[j] = fmaf(p.beta, add[j], v[j]);
+            if constexpr (MODE == kModeParts) {
+              d_low.to_rows(turn_c, add, lane);
+#pragma unroll
+              for (int j = 0; j < CB; ++j) v[j] = fmaf(p.beta, add[j], v[j]);
+            }
           };
           if constexpr (MODE == kModeGrad) {
             if (has_d) add_d();
@@ -977,19 +1011,28 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             if (has_d) add_d();
             if (cb + 1 < BLOCKS) request(cb + 1);
           }
-          BlockC::store(c_ptr + static_cast<long long>(cb * CB) * p.ldc, p.ldc, rows_left, cols_left, turn_c, v, lane);
-          if constexpr (MODE == kModeForward && sizeof(OT) == 2 && sizeof(T) == sizeof(OT) && BN == CTAS * BM) {
-            if (p.tri && t.tm != t.tn && in_rows) {
-              // mirror image: this lane's columns are consecutive rows there
-              OT* const dst = static_cast<OT*>(p.c) + zc * p.c_stride + static_cast<long long>(row) * p.ldc + group_col0 + cb * CB;
-              uint32_t w[CB / 2];
+          // stores the block, and its mirror image where the result is symmetric
+          auto put = [&](long long plane) {
+            BlockC::store(c_ptr + plane + static_cast<long long>(cb * CB) * p.ldc, p.ldc, rows_left, cols_left, turn_c, v, lane);
+            if constexpr ((MODE == kModeForward || MODE == kModeParts) && sizeof(OT) == 2 && BN == CTAS * BM) {
+              if (p.tri && t.tm != t.tn && in_rows) {
+                // this lane's columns are consecutive rows there
+                OT* const dst = static_cast<OT*>(p.c) + zc * p.c_stride + plane + static_cast<long long>(row) * p.ldc + group_col0 + cb * CB;
+                uint32_t w[CB / 2];
 #pragma unroll
-              for (int q = 0; q < CB / 2; ++q) w[q] = pack2<OT>(v[2 * q], v[2 * q + 1]);
+                for (int q = 0; q < CB / 2; ++q) w[q] = pack2<OT>(v[2 * q], v[2 * q + 1]);
 #pragma unroll
-              for (int q = 0; q < CB / 8; ++q)
-                if (cols_left >= 8 * (q + 1))
-                  *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+                for (int q = 0; q < CB / 8; ++q)
+                  if (cols_left >= 8 * (q + 1))
+                    *reinterpret_cast<uint4*>(dst + 8 * q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+              }
             }
+          };
+          put(0);
+          if constexpr (MODE == kModeParts) {
+#pragma unroll
+            for (int j = 0; j < CB; ++j) v[j] -= to_float(from_float<OT>(v[j]));
+            put(p.c_stride);
           }
         };
         run_blocks(block, request);
@@ -1060,7 +1103,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (!ok) break;
         end();
       }
-      if (MODE != kModeForward && p.partial != nullptr && in_rows)
+      if (MODE != kModeForward && MODE != kModeParts && p.partial != nullptr && in_rows)
         p.partial[(static_cast<long long>(t.col_tile) * EG + group) * p.m + row] = row_sum;
     }
   }
@@ -1085,21 +1128,34 @@ cudaError_t launch_mode(const CUtensorMap* maps, const FusedParams& p, int grid,
   cfg.blockDim = dim3(fused_threads(BN), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   const int cluster = CTAS == 2 ? 2 : p.split;
+  unsigned attrs = 0;
   if (cluster > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    attr[attrs].id = cudaLaunchAttributeClusterDimension;
+    attr[attrs].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[attrs].val.clusterDim.y = 1;
+    attr[attrs].val.clusterDim.z = 1;
+    ++attrs;
   }
+  if (p.chained) {
+    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[attrs].val.programmaticStreamSerializationAllowed = 1;
+    ++attrs;
+  }
+  cfg.attrs = attrs ? attr : nullptr;
+  cfg.numAttrs = attrs;
   return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], p);
 }
 
 template <int CTAS, int BN, class T, class DT, class OT>
 cudaError_t launch_typed(const CUtensorMap* maps, const FusedParams& p, int grid, int smem, cudaStream_t stream) {
+  if constexpr ((BN == 256 && CTAS == 2) || (BN == 128 && CTAS == 1)) {
+    if constexpr (std::is_same<T, __half>::value && std::is_same<OT, __half>::value) {
+      if (p.parts) return launch_mode<CTAS, BN, T, DT, OT, kModeParts>(maps, p, grid, smem, stream);
+    }
+  }
+  if (p.parts) return cudaErrorInvalidValue;
   if (!p.vec || p.split > 1) return launch_mode<CTAS, BN, T, DT, OT, kModeGeneral>(maps, p, grid, smem, stream);
   if (!p.grad) return launch_mode<CTAS, BN, T, DT, OT, kModeForward>(maps, p, grid, smem, stream);
   // gradients are stored in the operands' type

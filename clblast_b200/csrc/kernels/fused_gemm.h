@@ -33,6 +33,8 @@ struct FusedParams {
   unsigned int idesc;
   int a_batched, b_batched;
   int stages;                 // depth of the operand ring
+  int parts;                  // every matrix is a sum of two halves in consecutive planes (see kModeParts)
+  int chained;                // the launch may be set up before the one in front of it in the stream has finished
   int split;                  // CTAs of a cluster that share one tile's inner extent (kernels of one CTA per tile)
   float alpha, beta;
   const void* bias;           // one value per row of C, or null
