@@ -48,10 +48,10 @@ namespace fused {
 using namespace tc;
 
 constexpr int BM = 128;   // rows of op(A) per CTA
-constexpr int BK = 64;    // inner elements per stage: 128-byte swizzle rows
-// operand stages (64 inner elements each) per accumulator: results in single precision; sums of two halves, whose users
-// (the Newton-Schulz steps) amplify an error that all entries share
-constexpr int kChunkSingle = 4, kChunkParts = 2;
+constexpr int ROW_K = 64; // inner elements of a 128-byte swizzle row
+// inner elements per accumulator: results in single precision; sums of two halves, whose users (the Newton-Schulz steps)
+// amplify an error that all entries share
+constexpr int kChunkSingle = 256, kChunkParts = 128;
 
 // Two values rounded to 16 bits in one word (the packed conversion runs on the full-rate pipe, the single one does not).
 template <class E>
@@ -375,12 +375,15 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                   const FusedParams p) {
   static_assert(sizeof(DT) == sizeof(OT), "D and C share the staging buffers");
   constexpr bool CHUNKED = sizeof(OT) == 4 || MODE == kModeParts;  // sums beyond what the accumulators give
-  constexpr int CHUNK = MODE == kModeParts ? kChunkParts : kChunkSingle;
+  constexpr int CHUNK = (MODE == kModeParts ? kChunkParts : kChunkSingle) / (ROW_K * fused_stage_rows(BN));  // stages
   constexpr int EG = fused_groups(BN);
   constexpr int CB = 16;  // columns per epilogue block
   constexpr int B_ROWS = BN / CTAS;
-  constexpr int A_BYTES = BM * BK * 2;
-  constexpr int STAGE_BYTES = A_BYTES + B_ROWS * BK * 2;
+  constexpr int SUBS = fused_stage_rows(BN);  // a stage holds SUBS blocks of 64 inner elements, one after the other
+  constexpr int BK = ROW_K * SUBS;
+  constexpr int A_BYTES = BM * ROW_K * 2;
+  constexpr int SUB_BYTES = A_BYTES + B_ROWS * ROW_K * 2;
+  constexpr int STAGE_BYTES = SUB_BYTES * SUBS;
   constexpr int GROUP_COLS = BN / EG;
   // accumulators, then the sums of results in single precision; a power of two
   constexpr int ACCS = (CHUNKED && BN == 256) ? 1 : 2;
@@ -466,9 +469,6 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       az = 2 * t.z + (term == 2 ? 1 : 0);
       bz = 2 * t.z + (term == 1 ? 1 : 0);
     }
-    const uint32_t a_dst = tiles_base + stage * STAGE_BYTES;
-    const uint32_t b_dst = a_dst + A_BYTES;
-    const int x = t.k0 + kb * BK;
     uint32_t bar;
     if constexpr (CTAS == 2) {
       // a block whose end has to be cleared is counted by each CTA for itself
@@ -490,17 +490,23 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       if constexpr (CTAS == 2) tma_load_3d_pair_hint(dst, map, bar, cx, cy, cz, pol);
       else tma_load_3d_hint(dst, map, bar, cx, cy, cz, pol);
     };
-    if (p.a_mn) {
 #pragma unroll
-      for (int j = 0; j < BM / 64; ++j) load(a_dst + j * 8192, &map_a, a_row0 + j * 64, x, az, pol_a);
-    } else {
-      load(a_dst, &map_a, x, a_row0, az, pol_a);
-    }
-    if (p.b_mn) {
+    for (int sub = 0; sub < SUBS; ++sub) {
+      const uint32_t a_dst = tiles_base + stage * STAGE_BYTES + sub * SUB_BYTES;
+      const uint32_t b_dst = a_dst + A_BYTES;
+      const int x = t.k0 + kb * BK + sub * ROW_K;
+      if (p.a_mn) {
 #pragma unroll
-      for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * 8192, &map_b, b_row0 + j * 64, x, bz, pol_b);
-    } else {
-      load(b_dst, &map_b, x, b_row0, bz, pol_b);
+        for (int j = 0; j < BM / 64; ++j) load(a_dst + j * 8192, &map_a, a_row0 + j * 64, x, az, pol_a);
+      } else {
+        load(a_dst, &map_a, x, a_row0, az, pol_a);
+      }
+      if (p.b_mn) {
+#pragma unroll
+        for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * 8192, &map_b, b_row0 + j * 64, x, bz, pol_b);
+      } else {
+        load(b_dst, &map_b, x, b_row0, bz, pol_b);
+      }
     }
   };
 
@@ -563,11 +569,13 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     // MMA's 16 are cleared in both (0 * NaN would not be 0), the MMAs behind that are left out. Called by the whole warp.
     auto clear_tail = [&](int stage, int valid) {
       const int steps = (valid + 15) / 16, rows = steps * 16 - valid;
-      uint8_t* const s = base_ptr + stage * STAGE_BYTES;
+      // (a block that ends at a swizzle row's end has nothing to clear; otherwise the end lies inside one)
+      const int in_row = valid % ROW_K;
+      uint8_t* const s = base_ptr + stage * STAGE_BYTES + valid / ROW_K * SUB_BYTES;
       constexpr int TILES = BM / 64 + B_ROWS / 64;
       for (int i = lane; i < rows * TILES * 8; i += 32) {
         const int chunk = i & 7, r = (i >> 3) % rows, j = (i >> 3) / rows;
-        *reinterpret_cast<uint4*>(s + j * 8192 + (valid + r) * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(s + j * 8192 + (in_row + r) * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
       }
       fence_proxy_async();
       __syncwarp();
@@ -644,13 +652,15 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           }
           tcgen05_fence_after();
           if (elect_one()) {
-            const uint32_t a_src = tiles_base + stage * STAGE_BYTES;
             // (an address in a cluster carries the CTA's rank above the 18 bits that the descriptor takes)
+            const uint32_t a_src = tiles_base + stage * STAGE_BYTES;
             const uint64_t da = a_form | ((a_src >> 4) & 0x3FFFu), db = b_form | (((a_src + A_BYTES) >> 4) & 0x3FFFu);
             const uint32_t fresh = kb == first_kb ? 0u : 1u;
             auto mma = [&](int ks) {
-              if constexpr (CTAS == 2) umma_f16_pair(d_tmem, da + a_step * ks, db + b_step * ks, idesc, ks == 0 ? fresh : 1u);
-              else umma_f16(d_tmem, da + a_step * ks, db + b_step * ks, idesc, ks == 0 ? fresh : 1u);
+              const uint32_t sub = static_cast<uint32_t>(ks / 4) * (SUB_BYTES >> 4), in_sub = static_cast<uint32_t>(ks % 4);
+              const uint64_t ma = da + sub + a_step * in_sub, mb = db + sub + b_step * in_sub;
+              if constexpr (CTAS == 2) umma_f16_pair(d_tmem, ma, mb, idesc, ks == 0 ? fresh : 1u);
+              else umma_f16(d_tmem, ma, mb, idesc, ks == 0 ? fresh : 1u);
             };
             if (steps == BK / 16) {
 #pragma unroll

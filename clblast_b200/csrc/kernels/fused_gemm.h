@@ -50,6 +50,15 @@ struct FusedParams {
   int hint_a, hint_b;
 };
 
+#ifdef __CUDACC__
+#define B200_HD __host__ __device__
+#else
+#define B200_HD
+#endif
+// Inner elements per operand stage, in swizzle rows of 64. The loops over the stages cost the same whatever a stage holds, and
+// up to 128 columns the MMAs of one swizzle row are shorter than that.
+B200_HD constexpr int fused_stage_rows(int bn) { return bn <= 128 ? 2 : 1; }
+
 // Sizes of one kernel variant as the selection sees it.
 struct FusedVariant {
   int ctas;           // CTAs per tile: 2 for the pair kernel
@@ -57,11 +66,6 @@ struct FusedVariant {
   int stage_bytes;
 };
 // Epilogue groups of four warps that share a tile's columns, next to four warps with other roles.
-#ifdef __CUDACC__
-#define B200_HD __host__ __device__
-#else
-#define B200_HD
-#endif
 // (Four groups on 128 columns halve the registers of a thread: 25 % slower where stores go element by element.)
 B200_HD constexpr int fused_groups(int bn) { return bn >= 64 ? 2 : 1; }
 B200_HD constexpr int fused_threads(int bn) { return 128 + 128 * fused_groups(bn); }
@@ -75,7 +79,7 @@ B200_HD constexpr int fused_staging_bytes(int bn, bool single, bool aux, int spl
 constexpr int kFusedBarBytes = 512;
 constexpr int kFusedVariants = 6;
 constexpr FusedVariant kFusedTable[kFusedVariants] = {
-    {2, 256, 32768}, {1, 256, 49152}, {1, 128, 32768}, {1, 64, 24576}, {1, 32, 20480}, {2, 128, 24576}};
+    {2, 256, 32768}, {1, 256, 49152}, {1, 128, 65536}, {1, 64, 49152}, {1, 32, 40960}, {2, 128, 49152}};
 
 // Enqueues variant `v` with operand type / D type / C type. `grid` counts CTAs, `smem` bytes of dynamic shared memory.
 cudaError_t launch_fused_variant(int v, int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p,
