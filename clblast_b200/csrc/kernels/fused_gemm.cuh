@@ -759,21 +759,29 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           if (!ok) break;
           tcgen05_fence_after();
           if (!empty) {
+            // two blocks at a time: all their loads under way before the first wait
+            constexpr int PAIR = BLOCKS % 2 == 0 ? 2 : 1;
+            const uint32_t from = accumulator(local);
+#pragma unroll 2
+            for (int cb = 0; cb < BLOCKS; cb += PAIR) {
+              uint32_t r[PAIR][CB], s[PAIR][CB];
 #pragma unroll
-            for (int cb = 0; cb < BLOCKS; ++cb) {
-              uint32_t r[CB];
-              tmem_ld(accumulator(local) + cb * CB, r);
-              if (c == 0) {
-                tmem_wait(r);
-              } else {
-                uint32_t s[CB];
-                tmem_ld(sums_tmem + cb * CB, s);
-                tmem_wait(r);
-                tmem_wait(s);
-#pragma unroll
-                for (int j = 0; j < CB; ++j) r[j] = __float_as_uint(__uint_as_float(s[j]) + __uint_as_float(r[j]));
+              for (int i = 0; i < PAIR; ++i) {
+                tmem_ld(from + (cb + i) * CB, r[i]);
+                if (c > 0) tmem_ld(sums_tmem + (cb + i) * CB, s[i]);
               }
-              tmem_st(sums_tmem + cb * CB, r);
+#pragma unroll
+              for (int i = 0; i < PAIR; ++i) tmem_wait(r[i]);
+              if (c > 0) {
+#pragma unroll
+                for (int i = 0; i < PAIR; ++i) {
+                  tmem_wait(s[i]);
+#pragma unroll
+                  for (int j = 0; j < CB; ++j) r[i][j] = __float_as_uint(__uint_as_float(s[i][j]) + __uint_as_float(r[i][j]));
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < PAIR; ++i) tmem_st(sums_tmem + (cb + i) * CB, r[i]);
             }
             tmem_st_wait();
           }
