@@ -11,6 +11,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <type_traits>
 
 #include "driver_api.h"
@@ -96,19 +97,26 @@ Span span_of(const void* p, size_t one, size_t two, size_t ld, int elem) {
 }
 bool overlap(const Span& a, const Span& b) { return a.first && b.first && a.first < b.last && b.first < a.last; }
 
-// A matrix beside C (residual, saved or read Z) may be C itself, element for element, or lie apart from it.
-bool beside(const void* x, size_t x_ld, const void* c, size_t c_ld, size_t one, size_t two, int x_elem, int c_elem,
-            bool same_allowed) {
-  if (!x || !overlap(span_of(x, one, two, x_ld, x_elem), span_of(c, one, two, c_ld, c_elem))) return true;
-  if (same_allowed && x == c && x_ld == c_ld && x_elem == c_elem) return true;
-  // interleaved columns of one buffer do not meet either
-  if (x_ld == c_ld && x_elem == c_elem) {
-    const unsigned char *p = static_cast<const unsigned char*>(x), *q = static_cast<const unsigned char*>(c);
-    const size_t pitch = x_ld * x_elem, gap = static_cast<size_t>(p > q ? p - q : q - p) % pitch;
-    const size_t line = one * x_elem;
-    return gap >= line && gap + line <= pitch;
-  }
-  return false;
+// A matrix in memory: `two` lines of `one` elements.
+struct Area {
+  const void* p;
+  size_t one, two, ld;
+  int elem;
+  Span span() const { return span_of(p, one, two, ld, elem); }
+};
+
+// Whether a matrix may lie where it does beside one that is written: apart from it, as other columns of the same lines, or
+// (where `same_allowed`) as the very same elements, each read before it is written.
+bool beside(const Area& x, const Area& c, bool same_allowed) {
+  if (!x.p || !c.p || !overlap(x.span(), c.span())) return true;
+  const size_t pitch = c.ld * c.elem;
+  if (x.ld * x.elem != pitch) return false;
+  if (same_allowed && x.p == c.p && x.elem == c.elem) return true;
+  const unsigned char *p = static_cast<const unsigned char*>(x.p), *q = static_cast<const unsigned char*>(c.p);
+  const size_t x_line = x.one * x.elem, c_line = c.one * c.elem;
+  // where x's lines begin relative to c's, within a pitch
+  const size_t gap = p >= q ? static_cast<size_t>(p - q) % pitch : (pitch - static_cast<size_t>(q - p) % pitch) % pitch;
+  return gap >= c_line && gap + x_line <= pitch;
 }
 
 template <class F>
@@ -211,10 +219,12 @@ extern "C" int b200blas_gemm_epilogue(int dtype, int c_dtype, int layout, int ta
     if ((st = check_c(e.c_one, e.c_two, 1, c, c_offset, c_ld, 0, c_elem))) return st;
     a = at(a, a_offset, elem); b = at(b, b_offset, elem); bias = at(bias, bias_offset, elem);
     z = at(z, z_offset, elem); d = has_d ? at(d, d_offset, c_elem) : nullptr; c = at(c, c_offset, c_elem);
-    if (!beside(z, z_ld, c, c_ld, e.c_one, e.c_two, elem, c_elem, false) ||
-        !beside(d, d_ld, c, c_ld, e.c_one, e.c_two, c_elem, c_elem, true) ||
-        !beside(z, z_ld, d, d_ld, e.c_one, e.c_two, elem, c_elem, false))
-      return kInvalidMatrixC;
+    const Area at_c = {c, e.c_one, e.c_two, c_ld, c_elem}, at_d = {d, e.c_one, e.c_two, d_ld, c_elem};
+    const Area at_z = {z, e.c_one, e.c_two, z_ld, elem}, at_a = {a, e.a_one, e.a_two, a_ld, elem};
+    const Area at_b = {b, e.b_one, e.b_two, b_ld, elem}, at_bias = {bias, e.c_one, 1, e.c_one, elem};
+    for (const Area& out : {at_c, at_z})
+      if (!beside(at_a, out, false) || !beside(at_b, out, false) || !beside(at_bias, out, false)) return kInvalidMatrixC;
+    if (!beside(at_z, at_c, false) || !beside(at_d, at_c, true) || !beside(at_d, at_z, false)) return kInvalidMatrixC;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
@@ -265,8 +275,13 @@ extern "C" int b200blas_gemm_epilogue_grad(int dtype, int layout, int ta, int tb
     a = at(a, a_offset, elem); b = at(b, b_offset, elem);
     d = has_d ? at(d, d_offset, elem) : nullptr; z = has_z ? at(z, z_offset, elem) : nullptr;
     c = at(c, c_offset, elem); bias_grad = at(bias_grad, bias_grad_offset, elem);
-    if (!beside(z, z_ld, c, c_ld, e.c_one, e.c_two, elem, elem, true) || !beside(d, d_ld, c, c_ld, e.c_one, e.c_two, elem, elem, true))
+    const Area at_c = {c, e.c_one, e.c_two, c_ld, elem}, at_d = {d, e.c_one, e.c_two, d_ld, elem};
+    const Area at_z = {z, e.c_one, e.c_two, z_ld, elem}, at_a = {a, e.a_one, e.a_two, a_ld, elem};
+    const Area at_b = {b, e.b_one, e.b_two, b_ld, elem}, at_sum = {bias_grad, e.c_one, 1, e.c_one, elem};
+    if (!beside(at_a, at_c, false) || !beside(at_b, at_c, false) || !beside(at_z, at_c, true) || !beside(at_d, at_c, true))
       return kInvalidMatrixC;
+    for (const Area& in : {at_a, at_b, at_c, at_d, at_z})
+      if (overlap(in.span(), at_sum.span())) return kInvalidVectorY;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
@@ -317,8 +332,10 @@ extern "C" int b200blas_activation_grad(int dtype, size_t rows, size_t n, int ac
     if (groups && (st = check_offsets(group_offsets, groups))) return st;
     dy = at(dy, dy_offset, elem); z = has_z ? at(z, z_offset, elem) : nullptr;
     dz = at(dz, dz_offset, elem); bias_grad = at(bias_grad, bias_grad_offset, elem);
-    if (!beside(dy, dy_ld, dz, dz_ld, n, rows, elem, elem, true) || !beside(z, z_ld, dz, dz_ld, n, rows, elem, elem, true))
-      return kInvalidMatrixC;
+    const Area at_dy = {dy, n, rows, dy_ld, elem}, at_z = {z, n, rows, z_ld, elem}, at_dz = {dz, n, rows, dz_ld, elem};
+    if (!beside(at_dy, at_dz, true) || !beside(at_z, at_dz, true)) return kInvalidMatrixC;
+    for (const Area& in : {at_dy, at_z, at_dz})
+      if (overlap(in.span(), span_of(bias_grad, n, lines, line_ld, elem))) return kInvalidVectorY;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
@@ -349,6 +366,10 @@ extern "C" int b200blas_activation_grad(int dtype, size_t rows, size_t n, int ac
 
 namespace {
 
+// Extents of W_g as stored.
+size_t w_one(int w_transpose, size_t n, size_t k) { return w_transpose == kNo ? n : k; }
+size_t w_two(int w_transpose, size_t n, size_t k) { return w_transpose == kNo ? k : n; }
+
 // The grouped products share everything but the epilogue.
 struct GroupedCall {
   int dtype, c_dtype, w_transpose;
@@ -366,8 +387,16 @@ int check_grouped(const GroupedCall& g) {
   int st = check_a(g.k, g.rows, 1, g.x, g.x_offset, g.x_ld, 0, elem);
   if (st) return st;
   // W_g: k x n (kNo) or n x k, rows contiguous
-  const size_t one = g.w_transpose == kNo ? g.n : g.k, two = g.w_transpose == kNo ? g.k : g.n;
-  return check_b(one, two, g.groups, g.w, g.w_offset, g.w_ld, g.w_stride, elem);
+  return check_b(w_one(g.w_transpose, g.n, g.k), w_two(g.w_transpose, g.n, g.k), g.groups, g.w, g.w_offset, g.w_ld, g.w_stride, elem);
+}
+
+// The weights of all groups as one stretch of memory.
+Span weights_span(const GroupedCall& g) {
+  const int elem = elem_of(g.dtype);
+  const size_t one = w_one(g.w_transpose, g.n, g.k), two = w_two(g.w_transpose, g.n, g.k);
+  Span s = span_of(at(g.w, g.w_offset, elem), one, two, g.w_ld, elem);
+  s.last += (g.groups - 1) * g.w_stride * elem;
+  return s;
 }
 
 FusedDesc grouped_desc(const GroupedCall& g) {
@@ -410,9 +439,13 @@ extern "C" int b200blas_gemm_grouped(int dtype, int c_dtype, int w_transpose, si
     f.z = at(z, z_offset, elem); f.ldz = static_cast<long long>(z_ld);
     f.d = has_d ? at(d, d_offset, c_elem) : nullptr; f.ldd = static_cast<long long>(d_ld);
     f.c = at(c, c_offset, c_elem); f.ldc = static_cast<long long>(c_ld);
-    if (!beside(f.z, z_ld, f.c, c_ld, n, rows, elem, c_elem, false) || !beside(f.d, d_ld, f.c, c_ld, n, rows, c_elem, c_elem, true) ||
-        !beside(f.z, z_ld, f.d, d_ld, n, rows, elem, c_elem, false))
-      return kInvalidMatrixC;
+    const Area at_c = {f.c, n, rows, c_ld, c_elem}, at_d = {f.d, n, rows, d_ld, c_elem}, at_z = {f.z, n, rows, z_ld, elem};
+    const Area at_x = {f.b, k, rows, x_ld, elem};
+    for (const Area& out : {at_c, at_z})
+      if (!beside(at_x, out, false) || overlap(weights_span(g), out.span()) ||
+          overlap(span_of(f.bias, n, groups, bias_ld, elem), out.span()))
+        return kInvalidMatrixC;
+    if (!beside(at_z, at_c, false) || !beside(at_d, at_c, true) || !beside(at_d, at_z, false)) return kInvalidMatrixC;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
@@ -448,8 +481,14 @@ extern "C" int b200blas_gemm_grouped_grad(int dtype, int w_transpose, size_t gro
     f.d = has_d ? at(d, d_offset, elem) : nullptr; f.ldd = static_cast<long long>(d_ld);
     f.c = at(c, c_offset, elem); f.ldc = static_cast<long long>(c_ld);
     f.bias_grad = at(bias_grad, bias_grad_offset, elem); f.bias_grad_stride = static_cast<long long>(bias_grad_ld);
-    if (!beside(f.z, z_ld, f.c, c_ld, n, rows, elem, elem, true) || !beside(f.d, d_ld, f.c, c_ld, n, rows, elem, elem, true))
+    const Area at_c = {f.c, n, rows, c_ld, elem}, at_d = {f.d, n, rows, d_ld, elem}, at_z = {f.z, n, rows, z_ld, elem};
+    const Area at_x = {f.b, k, rows, x_ld, elem};
+    if (!beside(at_x, at_c, false) || overlap(weights_span(g), at_c.span()) || !beside(at_z, at_c, true) || !beside(at_d, at_c, true))
       return kInvalidMatrixC;
+    const Span sums = span_of(f.bias_grad, n, groups, bias_grad_ld, elem);
+    for (const Area& in : {at_x, at_c, at_d, at_z})
+      if (overlap(in.span(), sums)) return kInvalidVectorY;
+    if (overlap(weights_span(g), sums)) return kInvalidVectorY;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
@@ -476,6 +515,10 @@ extern "C" int b200blas_gemm_grouped_weight(int dtype, int c_dtype, size_t group
     // the groups' results must not meet
     if (groups > 1 && c_stride < c_ld * (m - 1) + n) return kInvalidDimension;
     if ((st = check_offsets(group_offsets, groups))) return st;
+    Span all = span_of(at(c, c_offset, c_elem), n, m, c_ld, c_elem);
+    all.last += (groups - 1) * c_stride * c_elem;
+    if (overlap(span_of(at(x, x_offset, elem), m, rows, x_ld, elem), all) || overlap(span_of(at(y, y_offset, elem), n, rows, y_ld, elem), all))
+      return kInvalidMatrixC;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
@@ -496,13 +539,56 @@ extern "C" int b200blas_gemm_grouped_weight(int dtype, int c_dtype, size_t group
 
 namespace {
 
+// Largest singular value of a normalised matrix, with a margin for rounding.
+constexpr double kNormalisedBound = 1.02;
+// Largest singular value that a step can leave, given the largest before it: |a x + b x^3 + c x^5| on [0, s] is largest at s
+// or where the slope a + 3 b t + 5 c t^2, t = x^2, is zero. With a margin for rounding.
+double step_bound(double s, const double* q) {
+  const auto size = [&](double t) { return std::fabs(std::sqrt(t) * (q[0] + t * (q[1] + t * q[2]))); };
+  double most = size(s * s);
+  const auto candidate = [&](double t) {
+    if (t > 0.0 && t < s * s) most = std::fmax(most, size(t));
+  };
+  const double disc = 9.0 * q[1] * q[1] - 20.0 * q[0] * q[2];
+  if (disc >= 0.0) {
+    // both roots without cancellation
+    const double h = -0.5 * (3.0 * q[1] + std::copysign(std::sqrt(disc), q[1]));
+    if (q[2] != 0.0) candidate(h / (5.0 * q[2]));
+    if (h != 0.0) candidate(q[0] / h);
+  }
+  return 1.02 * most;
+}
+// The power of two that brings a matrix with entries up to `bound` under 2^15, half of half precision's largest number.
+double parts_scale(double bound) {
+  if (!(bound > 0.0) || !std::isfinite(bound)) return 1.0;
+  int e = 0;
+  std::frexp(bound, &e);  // bound < 2^e
+  e = 15 - e;
+  return std::ldexp(1.0, e > 13 ? 13 : e);
+}
+
+// Whether halves hold the iteration whatever its matrix: beyond these bounds scales that keep the largest possible values
+// finite would push those of most matrices into half's subnormal range.
+bool bounded(const double* coefficients, bool per_step, int steps) {
+  double bound = kNormalisedBound;
+  for (int i = 0; i < steps; ++i) {
+    const double* const q = coefficients + (per_step ? 3 * i : 0);
+    const double bracket = std::fabs(q[1]) * bound * bound + std::fabs(q[2]) * bound * bound * bound * bound;
+    bound = step_bound(bound, q);
+    if (!(bracket < 4096.0) || !(bound < 64.0)) return false;
+  }
+  return true;
+}
+
 // X <- a X + (b A + c A A) X with A = X X^T (or X^T X on the shorter side) on 16-bit tensor cores. X, A and the bracket
-// are kept in half precision between products whatever the caller's 16-bit type: the singular values lie in [0, 1.2], so
-// half's 11 bits apply (bfloat16 has 8), and X starts scaled by a power of two (undone in the first step) so that the
-// entries of a normalised large matrix stay out of half's subnormal range. Sums run in fp32 throughout.
-cudaError_t newton_schulz_half(int dtype, long long one, long long two, double alpha, const void* a, long long a_ld,
-                               long long a_stride, void* b, long long b_ld, long long b_stride, long long batch, int steps,
-                               const double* coefficients, bool per_step, double eps, cudaStream_t s, const char** name) {
+// are kept in half precision between products whatever the caller's 16-bit type: their entries are bounded by what the
+// polynomial makes of the singular values, so half's 11 bits apply (bfloat16 has 8), each matrix scaled by a power of two
+// that brings the bound under 2^15 and keeps the entries of large matrices out of half's subnormal range. Sums run in
+// fp32 throughout.
+cudaError_t newton_schulz_half(long long one, long long two, double alpha, const void* a, long long a_ld, long long a_stride,
+                               void* b, long long b_ld, long long b_stride, long long batch, int steps,
+                               const double* coefficients, bool per_step, double eps, cudaStream_t s, int dtype,
+                               const char** name) {
   const bool gram_of_lines = one > two;  // the shorter side is the number of lines
   // extents inside are multiples of 8, the rest zero: the symmetric products store 16 bytes at a time
   const long long pitch = (one + 7) / 8 * 8, lines = (two + 7) / 8 * 8;
@@ -518,18 +604,17 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
   void* x[2] = {base, base + x_bytes};
   void* const gram = base + 2 * x_bytes;
   void* const poly = base + 2 * x_bytes + g_bytes;
-  // entries of the normalised matrix are about 1 / sqrt(one * two); bring them near 1 / 8, the largest possible to 2^13
-  int shift = static_cast<int>(std::floor(0.5 * std::log2(static_cast<double>(one) * static_cast<double>(two)))) - 3;
-  shift = shift < 0 ? 0 : (shift > 13 ? 13 : shift);
-  const double scale0 = std::ldexp(1.0, shift);
+  double bound = kNormalisedBound, x_scale = parts_scale(bound);
   NormaliseJob norm = {};
   norm.type = dtype; norm.x_type = 16; norm.g = a; norm.one = one; norm.two = two; norm.ld = a_ld; norm.stride = a_stride;
-  norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.lines = lines; norm.eps = eps; norm.scale = scale0;
+  norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.lines = lines; norm.eps = eps; norm.scale = x_scale;
   norm.sums = reinterpret_cast<double*>(base + 2 * x_bytes + 2 * g_bytes);
   e = launch_normalise(norm, s);
   for (int i = 0; i < steps && e == cudaSuccess; ++i) {
     const double* const q = coefficients + (per_step ? 3 * i : 0);
-    const double undo = i == 0 ? 1.0 / scale0 : 1.0;
+    const double bracket = std::fabs(q[1]) * bound * bound + std::fabs(q[2]) * bound * bound * bound * bound;
+    const double g_scale = parts_scale(bound * bound), p_scale = parts_scale(bracket);
+    bound = step_bound(bound, q);
     const bool last = i == steps - 1;
     const void* const from = x[i & 1];
     FusedDesc f = {};
@@ -539,7 +624,7 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
     f.m = f.n = side; f.k = gram_of_lines ? pitch : lines;
     f.a = f.b = from; f.lda = f.ldb = pitch; f.a_stride = f.b_stride = lines * pitch;
     f.a_mn = f.b_mn = gram_of_lines ? 0 : 1;
-    f.alpha = undo * undo; f.tri = 1;
+    f.alpha = g_scale / (x_scale * x_scale); f.tri = 1;
     f.c = gram; f.ldc = gram_pitch; f.c_stride = side * gram_pitch;
     e = launch_fused(f, s, name);
     if (e != cudaSuccess) break;
@@ -547,12 +632,12 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
     f.k = side;
     f.a = f.b = gram; f.lda = f.ldb = gram_pitch; f.a_stride = f.b_stride = side * gram_pitch;
     f.a_mn = f.b_mn = 0;
-    f.alpha = q[2]; f.beta = q[1]; f.d = gram; f.ldd = gram_pitch; f.d_stride = side * gram_pitch;
+    f.alpha = p_scale * q[2] / (g_scale * g_scale); f.beta = p_scale * q[1] / g_scale; f.d = gram; f.ldd = gram_pitch; f.d_stride = side * gram_pitch;
     f.c = poly;
     e = launch_fused(f, s, name);
     if (e != cudaSuccess) break;
     // a X + (.) X, on the last step straight into the caller's matrix
-    const double out = undo * (last ? alpha : 1.0);
+    const double out = last ? alpha : parts_scale(bound);
     f.tri = 0;
     f.m = last ? one : pitch; f.n = last ? two : lines; f.k = side;
     if (gram_of_lines) {
@@ -562,34 +647,16 @@ cudaError_t newton_schulz_half(int dtype, long long one, long long two, double a
       f.a = poly; f.lda = gram_pitch; f.a_stride = side * gram_pitch; f.a_mn = 0;
       f.b = from; f.ldb = pitch; f.b_stride = lines * pitch; f.b_mn = 0;
     }
-    f.alpha = out; f.beta = q[0] * out; f.d = from; f.ldd = pitch; f.d_stride = lines * pitch;
+    f.alpha = out / (p_scale * x_scale); f.beta = out * q[0] / x_scale; f.d = from; f.ldd = pitch; f.d_stride = lines * pitch;
     if (last) {
       f.c_type = dtype; f.c = b; f.ldc = b_ld; f.c_stride = b_stride;
     } else {
       f.c = x[(i + 1) & 1]; f.ldc = pitch; f.c_stride = lines * pitch;
     }
     e = launch_fused(f, s, name);
+    x_scale = out;
   }
   return e;
-}
-
-// Largest singular value that a step can leave, given the largest before it: the polynomial's extreme on [0, s], sampled
-// densely enough (its slope is bounded by the coefficients) and with a margin for rounding.
-double step_bound(double s, const double* q) {
-  double most = 0.0;
-  for (int i = 0; i <= 2000; ++i) {
-    const double x = s * i / 2000.0, y = std::fabs(x * (q[0] + x * x * (q[1] + x * x * q[2])));
-    if (!(y <= most)) most = y;
-  }
-  return 1.02 * most;
-}
-// The power of two that brings a matrix with entries up to `bound` under 2^15, half of half precision's largest number.
-double parts_scale(double bound) {
-  if (!(bound > 0.0)) return 1.0;
-  int e = 0;
-  std::frexp(bound, &e);  // bound < 2^e
-  e = 15 - e;
-  return std::ldexp(1.0, e > 13 ? 13 : e);
 }
 
 // The same iteration in single precision: every matrix is kept as a sum of two halves, hi + lo, about 22 bits, scaled by
@@ -599,14 +666,6 @@ double parts_scale(double bound) {
 cudaError_t newton_schulz_parts(long long one, long long two, double alpha, const void* a, long long a_ld, long long a_stride,
                                 void* b, long long b_ld, long long b_stride, long long batch, int steps,
                                 const double* coefficients, bool per_step, double eps, cudaStream_t s) {
-  double bound = 1.02;  // of a normalised matrix
-  for (int i = 0; i < steps; ++i) {
-    const double* const q = coefficients + (per_step ? 3 * i : 0);
-    const double bracket = std::fabs(q[1]) * bound * bound + std::fabs(q[2]) * bound * bound * bound * bound;
-    if (!(bracket < 4096.0)) return cudaErrorNotSupported;
-    bound = step_bound(bound, q);
-    if (!(bound < 64.0)) return cudaErrorNotSupported;
-  }
   const bool gram_of_lines = one > two;
   const long long pitch = (one + 7) / 8 * 8, lines = (two + 7) / 8 * 8;
   const long long side = gram_of_lines ? lines : pitch;
@@ -621,8 +680,7 @@ cudaError_t newton_schulz_parts(long long one, long long two, double alpha, cons
   void* x[2] = {base, base + x_bytes};
   void* const gram = base + 2 * x_bytes;
   void* const poly = base + 2 * x_bytes + g_bytes;
-  bound = 1.02;
-  double x_scale = parts_scale(bound);
+  double bound = kNormalisedBound, x_scale = parts_scale(bound);
   NormaliseJob norm = {};
   norm.type = 32; norm.x_type = kParts; norm.g = a; norm.one = one; norm.two = two; norm.ld = a_ld; norm.stride = a_stride;
   norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.lines = lines; norm.eps = eps; norm.scale = x_scale;
@@ -674,16 +732,17 @@ cudaError_t newton_schulz_parts(long long one, long long two, double alpha, cons
   }
   if (e != cudaSuccess) return e;
   JoinJob join = {};
-  join.x = x[steps & 1]; join.lines = lines; join.pitch = pitch;
-  join.b = static_cast<float*>(b); join.one = one; join.two = two; join.ld = b_ld; join.stride = b_stride; join.batch = batch;
+  join.type = 32; join.x_type = kParts; join.x = x[steps & 1]; join.lines = lines; join.pitch = pitch;
+  join.b = b; join.one = one; join.two = two; join.ld = b_ld; join.stride = b_stride; join.batch = batch;
   join.scale = static_cast<float>(alpha / x_scale);
   return launch_join(join, s);
 }
 
-// The same on the SGEMM kernels; a product that adds to another matrix adds to a copy of it.
+// The same on the SGEMM kernels, for coefficients whose values halves might not hold; a product that adds to another
+// matrix adds to a copy of it.
 cudaError_t newton_schulz_single(long long one, long long two, double alpha, const void* a, long long a_ld,
                                  long long a_stride, void* b, long long b_ld, long long b_stride, long long batch, int steps,
-                                 const double* coefficients, bool per_step, double eps, cudaStream_t s) {
+                                 const double* coefficients, bool per_step, double eps, cudaStream_t s, int dtype) {
   const bool gram_of_lines = one > two;
   const long long side = gram_of_lines ? two : one;
   const long long pitch = (one + 3) / 4 * 4, gram_pitch = (side + 3) / 4 * 4;
@@ -699,13 +758,12 @@ cudaError_t newton_schulz_single(long long one, long long two, double alpha, con
   void* const gram = base + 2 * x_bytes;
   void* const poly = base + 2 * x_bytes + g_bytes;
   NormaliseJob norm = {};
-  norm.type = 32; norm.x_type = 32; norm.g = a; norm.one = one; norm.two = two; norm.ld = a_ld; norm.stride = a_stride;
+  norm.type = dtype; norm.x_type = 32; norm.g = a; norm.one = one; norm.two = two; norm.ld = a_ld; norm.stride = a_stride;
   norm.batch = batch; norm.x = x[0]; norm.pitch = pitch; norm.lines = two; norm.eps = eps; norm.scale = 1.0;
   norm.sums = reinterpret_cast<double*>(base + 2 * x_bytes + 2 * g_bytes);
   e = launch_normalise(norm, s);
   for (int i = 0; i < steps && e == cudaSuccess; ++i) {
     const double* const q = coefficients + (per_step ? 3 * i : 0);
-    const bool last = i == steps - 1;
     void* const from = x[i & 1];
     GemmDesc g = {};
     g.dtype = 32; g.batch = batch;
@@ -724,7 +782,6 @@ cudaError_t newton_schulz_single(long long one, long long two, double alpha, con
     g.c = poly;
     e = dispatch(g, s);
     if (e != cudaSuccess) break;
-    const double out = last ? alpha : 1.0;
     g.m = one; g.n = two; g.k = side;
     if (gram_of_lines) {
       g.a = from; g.lda = pitch; g.a_stride = two * pitch; g.a_kcontig = 0;
@@ -733,20 +790,17 @@ cudaError_t newton_schulz_single(long long one, long long two, double alpha, con
       g.a = poly; g.lda = gram_pitch; g.a_stride = side * gram_pitch; g.a_kcontig = 1;
       g.b = from; g.ldb = pitch; g.b_stride = two * pitch; g.b_kcontig = 1;
     }
-    g.alpha[0] = out; g.beta[0] = q[0] * out;
-    if (last) {
-      g.c = b; g.ldc = b_ld; g.c_stride = b_stride;
-      for (long long z = 0; z < batch && e == cudaSuccess; ++z)
-        e = cudaMemcpy2DAsync(static_cast<float*>(b) + z * b_stride, static_cast<size_t>(b_ld) * 4,
-                              static_cast<const float*>(from) + z * two * pitch, static_cast<size_t>(pitch) * 4,
-                              static_cast<size_t>(one) * 4, static_cast<size_t>(two), cudaMemcpyDeviceToDevice, s);
-    } else {
-      g.c = x[(i + 1) & 1]; g.ldc = pitch; g.c_stride = two * pitch;
-      e = cudaMemcpyAsync(g.c, from, static_cast<size_t>(batch) * two * pitch * 4, cudaMemcpyDeviceToDevice, s);
-    }
+    g.alpha[0] = 1.0; g.beta[0] = q[0];
+    g.c = x[(i + 1) & 1]; g.ldc = pitch; g.c_stride = two * pitch;
+    e = cudaMemcpyAsync(g.c, from, static_cast<size_t>(batch) * two * pitch * 4, cudaMemcpyDeviceToDevice, s);
     if (e == cudaSuccess) e = dispatch(g, s);
   }
-  return e;
+  if (e != cudaSuccess) return e;
+  JoinJob join = {};
+  join.type = dtype; join.x_type = 32; join.x = x[steps & 1]; join.lines = two; join.pitch = pitch;
+  join.b = b; join.one = one; join.two = two; join.ld = b_ld; join.stride = b_stride; join.batch = batch;
+  join.scale = static_cast<float>(alpha);
+  return launch_join(join, s);
 }
 
 }  // namespace
@@ -762,6 +816,8 @@ extern "C" int b200blas_newton_schulz(int dtype, int layout, size_t m, size_t n,
     if (batch_count < 1 || batch_count > 65535) return kInvalidBatchCount;
     if (m == 0 || n == 0 || !extents_ok(m, n, 0)) return kInvalidDimension;
     if (steps < 1 || steps > 1000 || (coefficient_count != 1 && coefficient_count < steps) || !(epsilon >= 0.0)) return kInvalidDimension;
+    const bool per_step = coefficient_count > 1;
+    const bool halves = bounded(coefficients, per_step, static_cast<int>(steps));
     const int elem = elem_of(dtype);
     const size_t one = layout == kRowMajor ? n : m, two = layout == kRowMajor ? m : n;
     if ((st = check_a(one, two, batch_count, a, a_offset, a_ld, a_stride, elem))) return st;
@@ -770,27 +826,16 @@ extern "C" int b200blas_newton_schulz(int dtype, int layout, size_t m, size_t n,
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
-    const char* name = "newton_schulz_single";
-    const bool per_step = coefficient_count > 1;
-    cudaError_t e;
-    if (dtype == 32) {
-      const auto run = [&](auto* f) {
-        return f(static_cast<long long>(one), static_cast<long long>(two), alpha, at(a, a_offset, elem),
-                 static_cast<long long>(a_ld), static_cast<long long>(a_stride), at(b, b_offset, elem),
-                 static_cast<long long>(b_ld), static_cast<long long>(b_stride), static_cast<long long>(batch_count),
-                 static_cast<int>(steps), coefficients, per_step, epsilon, s);
-      };
-      name = "newton_schulz_parts";
-      e = run(&newton_schulz_parts);
-      if (e == cudaErrorNotSupported) {
-        name = "newton_schulz_single";
-        e = run(&newton_schulz_single);
-      }
-    }
-    else e = newton_schulz_half(dtype, static_cast<long long>(one), static_cast<long long>(two), alpha, at(a, a_offset, elem),
-                             static_cast<long long>(a_ld), static_cast<long long>(a_stride), at(b, b_offset, elem),
-                             static_cast<long long>(b_ld), static_cast<long long>(b_stride),
-                             static_cast<long long>(batch_count), static_cast<int>(steps), coefficients, per_step, epsilon, s, &name);
+    const char* name = halves ? (dtype == 32 ? "newton_schulz_parts" : "none") : "newton_schulz_single";
+    const auto run = [&](auto* f, auto... more) {
+      return f(static_cast<long long>(one), static_cast<long long>(two), alpha, at(a, a_offset, elem), static_cast<long long>(a_ld),
+               static_cast<long long>(a_stride), at(b, b_offset, elem), static_cast<long long>(b_ld),
+               static_cast<long long>(b_stride), static_cast<long long>(batch_count), static_cast<int>(steps), coefficients, per_step,
+               epsilon, s, more...);
+    };
+    const cudaError_t e = !halves       ? run(&newton_schulz_single, dtype)
+                          : dtype == 32 ? run(&newton_schulz_parts)
+                                        : run(&newton_schulz_half, dtype, &name);
     return finish(s, async, e, name);
   });
 }

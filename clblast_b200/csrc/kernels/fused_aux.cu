@@ -220,15 +220,20 @@ __global__ void __launch_bounds__(256) scale_kernel(const NormaliseJob job, int 
   }
 }
 
+template <class T, bool PARTS>
 __global__ void __launch_bounds__(256) join_kernel(const JoinJob job) {
-  const __half* const x = static_cast<const __half*>(job.x) + static_cast<long long>(blockIdx.y) * 2 * job.lines * job.pitch;
-  float* const b = job.b + static_cast<long long>(blockIdx.y) * job.stride;
+  using S = typename std::conditional<PARTS, __half, float>::type;
+  const long long plane = job.lines * job.pitch;
+  const S* const x = static_cast<const S*>(job.x) + static_cast<long long>(blockIdx.y) * (PARTS ? 2 : 1) * plane;
+  T* const b = static_cast<T*>(job.b) + static_cast<long long>(blockIdx.y) * job.stride;
   for (long long line = blockIdx.x; line < job.two; line += gridDim.x) {
-    const __half* const high = x + line * job.pitch;
-    const __half* const low = high + job.lines * job.pitch;
+    const S* const from = x + line * job.pitch;
 #pragma unroll 4
-    for (long long i = threadIdx.x; i < job.one; i += 256)
-      b[line * job.ld + i] = job.scale * (__half2float(high[i]) + __half2float(low[i]));
+    for (long long i = threadIdx.x; i < job.one; i += 256) {
+      float v = to_float(from[i]);
+      if constexpr (PARTS) v += to_float(from[plane + i]);
+      b[line * job.ld + i] = from_float<T>(job.scale * v);
+    }
   }
 }
 
@@ -342,8 +347,12 @@ cudaError_t launch_normalise(const NormaliseJob& job, cudaStream_t stream) {
 cudaError_t launch_join(const JoinJob& job, cudaStream_t stream) {
   if (job.batch > 65535) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(job.two < 4096 ? job.two : 4096), static_cast<unsigned>(job.batch));
-  join_kernel<<<grid, 256, 0, stream>>>(job);
-  return cudaGetLastError();
+  return by_type(job.type, [&](auto* tag) {
+    using T = typename std::remove_pointer<decltype(tag)>::type;
+    if (job.x_type == kParts) join_kernel<T, true><<<grid, 256, 0, stream>>>(job);
+    else join_kernel<T, false><<<grid, 256, 0, stream>>>(job);
+    return cudaGetLastError();
+  });
 }
 
 }  // namespace b200

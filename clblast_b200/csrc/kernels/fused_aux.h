@@ -69,11 +69,13 @@ struct NormaliseJob {
 };
 cudaError_t launch_normalise(const NormaliseJob& job, cudaStream_t stream);
 
-// B = scale * (hi + lo): `batch` matrices from planes 2z and 2z + 1 of x (lines x pitch halves each) to single precision.
+// B = scale * X, `batch` matrices to the caller's type. x_type 32: X in single precision; kParts: planes 2z and 2z + 1 of
+// x (lines x pitch halves each) hold hi and lo, X = hi + lo.
 struct JoinJob {
+  int type, x_type;
   const void* x;
   long long lines, pitch;
-  float* b;
+  void* b;
   long long one, two, ld, stride, batch;
   float scale;
 };

@@ -28,7 +28,8 @@ int context_key(unsigned long long* key);
 cudaError_t kernel_ready(const void* func, int smem_bytes, int* regs = nullptr);
 
 // Status block written by the tensor-core kernels when a bounded wait expires: word 0 = code (1 producer,
-// 2 accumulator-free, 3 operands-ready, 4 accumulator-ready, 5 raw-tile, 6 old-C block), word 1 = block index,
+// 2 accumulator-free, 3 operands-ready, 4 accumulator-ready, 5 raw-tile, 6 old-C block, 7 sums-free and 8 sums-ready of a
+// split tile, 10 last-block and 11 cleared-block of a ragged inner extent), word 1 = block index,
 // word 2 = barrier address. It lives in a page of host memory inside the library image that is registered with the
 // driver as mapped, portable pinned memory, so kernels of every context write it directly and the host reads it
 // without a copy or a stream operation (after synchronising the stream the kernel ran on). Nothing is allocated.

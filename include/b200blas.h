@@ -156,8 +156,9 @@ int b200blas_col2im(int dtype, int kernel_mode, size_t channels, size_t height, 
  *   - `activation`: 161 identity, 162 relu, 163 gelu (z times the normal distribution function), 164 gelu in its tanh
  *     form, 165 silu. act' below is its derivative.
  *   - optional buffers are absent when NULL; D is not read when beta == 0, Z is not read when the activation is the
- *     identity. D may be C itself, a Z that is read may be C too; any other overlap with C is refused
- *     (kInvalidMatrixC). C must not overlap A or B.
+ *     identity. D may be C itself, and so may a Z that is read; DZ may be DY or Z. Otherwise what is written may not
+ *     meet anything that the call reads or writes (kInvalidMatrixC, for a bias gradient kInvalidVectorY), except as
+ *     other columns of the same lines. B of the Newton-Schulz products may overlap A.
  *   - Z and D have C's extents and are reported with C's status codes; a bad bias is kInvalidVectorX (-1019) or
  *     kInsufficientMemoryX (-1008), a bad bias gradient kInvalidVectorY (-1018) or kInsufficientMemoryY (-1007).
  *     Extents above 2^31 - 4097 are kInvalidDimension. Buffers that do not lie on the current device are invalid.
@@ -227,8 +228,9 @@ int b200blas_gemm_grouped_weight(int dtype, int c_dtype, size_t groups, size_t r
 /* Orthogonalises batch_count m x n matrices by Newton-Schulz products: X = A / (|A|_F + epsilon), then `steps` times
  * X <- a X + (b G + c G G) X with G = X X^T (on the shorter side), B = alpha * X. `coefficients` (HOST) holds one triple
  * (a, b, c) for all steps, or, with coefficient_count >= steps, one per step. B may be A. 16-bit types keep X, G and the
- * bracket in half precision between the products; 32 runs on the single-precision kernels throughout.
- * dtype 16, bf16, 32. steps 1 to 1000, at most 65535 matrices. */
+ * bracket in half precision between the products, single precision as sums of two halves (about 22 bits). Coefficients
+ * that let a singular value reach 64, or the bracket 4096, run on the single-precision kernels, which take several
+ * times as long. dtype 16, bf16, 32. steps 1 to 1000, at most 65535 matrices. */
 int b200blas_newton_schulz(int dtype, int layout, size_t m, size_t n, double alpha, const void* a, size_t a_offset,
                            size_t a_ld, size_t a_stride, void* b, size_t b_offset, size_t b_ld, size_t b_stride,
                            size_t batch_count, size_t steps, const double* coefficients, size_t coefficient_count,
