@@ -18,6 +18,8 @@
 #include "fused_host.h"
 #include "host_common.h"
 #include "kernels/fused_aux.h"
+#include "kernels/fused_rows.h"
+#include "kernels/fused_single.h"
 #include "kernels/launchers.h"
 #include "scratch.h"
 
@@ -152,10 +154,36 @@ cudaError_t single_epilogue(int layout, int ta, int tb, size_t m, size_t n, size
                             size_t a_ld, const void* b, size_t b_ld, PointwiseJob job, void* bias_grad,
                             cudaStream_t s, const char** name) {
   const double al[2] = {alpha, 0.0}, zero[2] = {0.0, 0.0};
+  const Operands o = orient(layout, ta, tb, m, n, a, a_ld, b, b_ld);
+  const bool split = single_fits(job.m, job.n, static_cast<long long>(k));
+  SingleJob one = {};
+  one.m = job.m; one.n = job.n; one.k = static_cast<long long>(k); one.alpha = static_cast<float>(alpha);
+  one.a = static_cast<const float*>(o.a); one.lda = static_cast<long long>(o.lda); one.a_mn = o.a_mn;
+  one.b = static_cast<const float*>(o.b); one.ldb = static_cast<long long>(o.ldb); one.b_mn = o.b_mn;
+  one.act = kActIdentityCode;
+  if (bias_grad == nullptr && job.n <= kFewRows && !o.a_mn && !o.b_mn && (reinterpret_cast<uintptr_t>(o.a) & 15) == 0 && o.lda % 4 == 0) {
+    FewRowsJob rows = {};
+    rows.type = rows.c_type = 32;
+    rows.m = static_cast<int>(job.m); rows.n = static_cast<int>(job.n); rows.k = static_cast<int>(k);
+    rows.w = o.a; rows.ldw = one.lda; rows.x = o.b; rows.ldx = one.ldb;
+    rows.alpha = one.alpha; rows.beta = job.beta; rows.bias = job.bias; rows.act = job.act; rows.grad = job.grad;
+    rows.d = job.d; rows.ldd = job.ldd; rows.z = job.z; rows.ldz = job.ldz; rows.c = job.c; rows.ldc = job.ldc;
+    *name = "single_few_rows";
+    return launch_few_rows(rows, s);
+  }
+  if (bias_grad == nullptr && split) {
+    one.bias = static_cast<const float*>(job.bias); one.act = job.act; one.grad = job.grad;
+    one.d = static_cast<const float*>(job.d); one.ldd = job.ldd; one.beta = job.beta;
+    one.z = static_cast<float*>(job.z); one.ldz = job.ldz;
+    one.c = static_cast<float*>(job.c); one.ldc = job.ldc;
+    *name = "single_split";
+    return launch_single(one, s);
+  }
   const Span c = span_of(job.c, job.m, job.n, job.ldc, 4);
   PoolScratch product, partial;
   void* p = job.c;
   size_t ldp = static_cast<size_t>(job.ldc);
+  // a pass over the product must find its own D and Z whole
   const bool reads_c = overlap(c, span_of(job.d, job.m, job.n, job.ldd, 4)) ||
                        (job.grad && overlap(c, span_of(job.z, job.m, job.n, job.ldz, 4)));
   if (reads_c) {
@@ -164,9 +192,16 @@ cudaError_t single_epilogue(int layout, int ta, int tb, size_t m, size_t n, size
     if (e != cudaSuccess) return e;
     p = product.ptr();
   }
-  const int st = gemm_enqueue(32, layout, ta, tb, m, n, k, al, a, 0, a_ld, b, 0, b_ld, zero, p, 0, ldp, s);
-  if (st != kSuccess) return st > 0 ? static_cast<cudaError_t>(st) : cudaErrorInvalidValue;
-  *name = "single_product_pointwise";
+  if (split) {
+    one.c = static_cast<float*>(p); one.ldc = static_cast<long long>(ldp);
+    *name = "single_split_pointwise";
+    const cudaError_t e = launch_single(one, s);
+    if (e != cudaSuccess) return e;
+  } else {
+    const int st = gemm_enqueue(32, layout, ta, tb, m, n, k, al, a, 0, a_ld, b, 0, b_ld, zero, p, 0, ldp, s);
+    if (st != kSuccess) return st > 0 ? static_cast<cudaError_t>(st) : cudaErrorInvalidValue;
+    *name = "single_product_pointwise";
+  }
   const bool plain = job.bias == nullptr && job.d == nullptr && job.z == nullptr && job.act == kActIdentityCode;
   if (plain && bias_grad == nullptr && p == job.c) return cudaSuccess;
   job.p = p;

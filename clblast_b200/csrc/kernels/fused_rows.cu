@@ -3,7 +3,7 @@
 // one vector: 14 us); here every warp reads one row of the matrix, or a part of it, with all its 16-byte loads in flight
 // and the vectors come out of L1.
 //
-// Sums run in fp32: eight per lane and vector, then over the lanes by shuffles, then over the parts in order.
+// Sums run in fp32: one per lane and vector, then over the lanes by shuffles, then over the parts in order.
 #include "fused_rows.h"
 
 #include <cuda_bf16.h>
@@ -23,14 +23,19 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kDeep = 4;  // 16-byte loads of W that a lane has in flight
 
+// Elements of a 16-byte piece.
 template <class T>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[16 / sizeof(T)]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const unsigned short lo = static_cast<unsigned short>(w[i]), hi = static_cast<unsigned short>(w[i] >> 16);
-    f[2 * i] = to_float(*reinterpret_cast<const T*>(&lo));
-    f[2 * i + 1] = to_float(*reinterpret_cast<const T*>(&hi));
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(w[i]);
+    } else {
+      const unsigned short lo = static_cast<unsigned short>(w[i]), hi = static_cast<unsigned short>(w[i] >> 16);
+      f[2 * i] = to_float(*reinterpret_cast<const T*>(&lo));
+      f[2 * i + 1] = to_float(*reinterpret_cast<const T*>(&hi));
+    }
   }
 }
 
@@ -38,6 +43,7 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
 template <class T, class OT, int ROWS, int PARTS, bool VX>
 __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const FewRowsJob job) {
   constexpr bool FAST = sizeof(OT) == 2;
+  constexpr int PV = 16 / sizeof(T);
   __shared__ float sums[kWarps][ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x * (kWarps / PARTS) + warp / PARTS;
@@ -48,25 +54,25 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const FewRowsJob 
   if (row < job.m) {
     const T* const w = static_cast<const T*>(job.w) + static_cast<long long>(row) * job.ldw;
     const T* const x = static_cast<const T*>(job.x);
-    const int vectors = job.k / 8;  // whole 16-byte pieces
+    const int vectors = job.k / PV;  // whole 16-byte pieces
     const int begin = static_cast<int>(static_cast<long long>(vectors) * part / PARTS);
     const int end = static_cast<int>(static_cast<long long>(vectors) * (part + 1) / PARTS);
     auto multiply = [&](const uint4& wv, int i) {
-      float a[8];
-      unpack8<T>(wv, a);
+      float a[PV];
+      unpack<T>(wv, a);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         if (r >= job.n) break;
-        float b[8];
-        const T* const xr = x + static_cast<long long>(r) * job.ldx + 8 * i;
+        float b[PV];
+        const T* const xr = x + static_cast<long long>(r) * job.ldx + PV * i;
         if (VX) {
-          unpack8<T>(__ldg(reinterpret_cast<const uint4*>(xr)), b);
+          unpack<T>(__ldg(reinterpret_cast<const uint4*>(xr)), b);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) b[j] = to_float(xr[j]);
+          for (int j = 0; j < PV; ++j) b[j] = to_float(xr[j]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[r] = fmaf(a[j], b[j], acc[r]);
+        for (int j = 0; j < PV; ++j) acc[r] = fmaf(a[j], b[j], acc[r]);
       }
     };
     int i = begin + lane;
@@ -79,7 +85,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const FewRowsJob 
     }
     for (; i < end; i += 32) multiply(__ldcs(reinterpret_cast<const uint4*>(w) + i), i);
     if (part == PARTS - 1) {  // what is left behind the last whole piece
-      const int j = vectors * 8 + lane;
+      const int j = vectors * PV + lane;
       if (j < job.k) {
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
@@ -123,7 +129,7 @@ template <class T, class OT, int ROWS, int PARTS>
 cudaError_t launch_parts(const FewRowsJob& job, cudaStream_t stream) {
   const int per_block = kWarps / PARTS;
   const unsigned blocks = static_cast<unsigned>((job.m + per_block - 1) / per_block);
-  const bool vx = (reinterpret_cast<uintptr_t>(job.x) & 15) == 0 && (job.n == 1 || job.ldx % 8 == 0);
+  const bool vx = (reinterpret_cast<uintptr_t>(job.x) & 15) == 0 && (job.n == 1 || job.ldx % (16 / static_cast<int>(sizeof(T))) == 0);
   if (vx) few_rows_kernel<T, OT, ROWS, PARTS, true><<<blocks, kWarps * 32, 0, stream>>>(job);
   else few_rows_kernel<T, OT, ROWS, PARTS, false><<<blocks, kWarps * 32, 0, stream>>>(job);
   return cudaGetLastError();
@@ -133,9 +139,10 @@ template <class T, class OT, int ROWS>
 cudaError_t launch_rows(const FewRowsJob& job, cudaStream_t stream) {
   // enough warps to keep every SM's memory pipeline full, each with at least one round of deep loads
   const long long wanted = 148LL * 24;
-  if (job.m >= wanted || job.k < 2 * 256 * kDeep) return launch_parts<T, OT, ROWS, 1>(job, stream);
-  if (2LL * job.m >= wanted || job.k < 4 * 256 * kDeep) return launch_parts<T, OT, ROWS, 2>(job, stream);
-  if (4LL * job.m >= wanted || job.k < 8 * 256 * kDeep) return launch_parts<T, OT, ROWS, 4>(job, stream);
+  const int round = 32 * kDeep * 16 / static_cast<int>(sizeof(T));  // elements of one
+  if (job.m >= wanted || job.k < 2 * round) return launch_parts<T, OT, ROWS, 1>(job, stream);
+  if (2LL * job.m >= wanted || job.k < 4 * round) return launch_parts<T, OT, ROWS, 2>(job, stream);
+  if (4LL * job.m >= wanted || job.k < 8 * round) return launch_parts<T, OT, ROWS, 4>(job, stream);
   return launch_parts<T, OT, ROWS, 8>(job, stream);
 }
 
@@ -157,6 +164,7 @@ cudaError_t launch_few_rows(const FewRowsJob& job, cudaStream_t stream) {
     if (job.c_type == kBFloat16) return launch_types<__nv_bfloat16, __nv_bfloat16>(job, stream);
     if (job.c_type == 32) return launch_types<__nv_bfloat16, float>(job, stream);
   }
+  if (job.type == 32 && job.c_type == 32) return launch_types<float, float>(job, stream);
   return cudaErrorInvalidValue;
 }
 

@@ -9,7 +9,7 @@ namespace b200 {
 // aligned rows. One kernel for up to kFewRows vectors.
 constexpr int kFewRows = 4;
 struct FewRowsJob {
-  int type, c_type;  // operands (16 or bfloat16's code), C and D (the same or 32)
+  int type, c_type;  // operands (16, bfloat16's code or 32), C and D (the same or 32)
   int m, n, k;
   const void* w; long long ldw;
   const void* x; long long ldx;

@@ -145,6 +145,20 @@ def test_sizes(cuda, monkeypatch, rows, n, k, name):
     linear(cuda, monkeypatch, None, name, name, ROW, NO, NO, rows, n, k, act=164, beta=1.0, grad=True)
 
 
+@pytest.mark.parametrize("rows,n,k", [(5, 33, 130), (16, 100, 1025), (17, 65, 515), (32, 520, 2050), (33, 64, 31), (64, 400, 300), (65, 129, 777),
+                                      (130, 130, 2048), (700, 1000, 900), (1030, 257, 2400)])
+@pytest.mark.parametrize("layout,ta,tb", [(ROW, NO, YES), (ROW, NO, NO), (COL, NO, NO), (COL, YES, YES), (ROW, YES, NO)])
+def test_single_precision(cuda, monkeypatch, rows, n, k, layout, ta, tb):
+    """Few vectors, one tile, ragged tiles, an inner extent split over blocks, and products with many tiles."""
+    for pads, offs in (((0, 0, 0, 0, 0), (0, 0, 0, 0, 0)), ((4, 4, 1, 2, 3), (4, 8, 1, 2, 3)), ((1, 3, 0, 0, 0), (0, 5, 0, 0, 0))):
+        linear(cuda, monkeypatch, None, "single", "single", layout, ta, tb, rows, n, k, act=163, beta=1.0, alpha=0.75, pads=pads, offs=offs)
+        linear(cuda, monkeypatch, None, "single", "single", layout, ta, tb, rows, n, k, act=165, beta=-0.5, grad=True, pads=pads, offs=offs)
+        linear(cuda, monkeypatch, None, "single", "single", layout, ta, tb, rows, n, k, act=164, grad=True, pads=pads, offs=offs, bias_grad=False)
+    linear(cuda, monkeypatch, None, "single", "single", layout, ta, tb, rows, n, k, act=165, beta=1.0, inplace="d")
+    linear(cuda, monkeypatch, None, "single", "single", layout, ta, tb, rows, n, k, act=165, beta=1.0, grad=True, inplace="z", bias_grad=False)
+    linear(cuda, monkeypatch, None, "single", "single", layout, ta, tb, rows, n, k, act=165, beta=1.0, grad=True, inplace="z")
+
+
 @pytest.mark.parametrize("act", [161, 162, 163, 164, 165])
 @pytest.mark.parametrize("name,c_name", [("half", "half"), ("bf16", "bf16"), ("half", "single"), ("bf16", "single"), ("single", "single")])
 @pytest.mark.parametrize("bias,keep,beta", [(False, False, 0.0), (True, True, 0.0), (True, False, 1.0), (False, True, -0.25)])

@@ -314,7 +314,7 @@ def test_capture_of_copies_and_single_precision(cuda):
 # ---- few vectors -----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5])
-@pytest.mark.parametrize("dtype,c_dtype", [("float16", "float16"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("dtype,c_dtype", [("float16", "float16"), ("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float32", "float32")])
 @pytest.mark.parametrize("n,k,act,beta,off", [(1000, 4104, 165, 1.0, 0), (8, 520, 163, -0.5, 3), (4104, 64, 164, 0.0, 0), (1, 1, 162, 1.0, 1),
                                               (777, 333, 161, 2.0, 0), (2048, 2048, 162, 1.0, 8)])
 def test_few_vectors(cuda, rows, dtype, c_dtype, n, k, act, beta, off):
