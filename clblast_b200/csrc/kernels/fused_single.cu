@@ -1,21 +1,21 @@
 // Single-precision products of few vectors or of small matrices, with the epilogue in the same kernel, on the CUDA cores.
 //
 // The tensor-core product in single precision works on 128 x 128 tiles over the whole inner extent: with few tiles most
-// SMs have nothing to do, and a pass over the result follows. Here a tile is 64 x 64 or, for up to 32 vectors, 32 x 16 or
-// 32 x 32, and the inner extent is split over up to eight blocks of a cluster. Each keeps a ring of cp.async copies in
-// flight; the partial sums meet through the cluster's shared memory, in a fixed order, and every block finishes its share
-// of the tile.
+// SMs have nothing to do, and a pass over the result follows. Here a tile is 64 x 64 or 32 x 16, and the inner extent is
+// split over up to eight blocks of a cluster. Each keeps a ring of cp.async copies in flight; the partial sums meet through
+// the cluster's shared memory, in a fixed order, and every block finishes its share of the tile.
 //
 // Within a block the operands stay in shared memory as they lie in memory. A thread reads four inner elements at a time:
 // along k as 16-byte pieces of its features' lines (lines are padded by four words, so the eight lines that lanes read at a
 // time fall into different banks), or, where features are contiguous, four features of each of the four. Either way TM + TN
-// 16-byte reads feed 4 * TM * TN multiply-adds. Sums run in fp32, one running sum per element, block and warp.
+// 16-byte reads feed 4 * TM * TN multiply-adds. Shared memory bounds it: 12 reads of a warp, four cycles each, for 128
+// multiply-adds that four schedulers share (25 of the 74 TFLOP/s; tiles of 8 x 8 per thread leave too few warps and are
+// slower). Sums run in fp32, one running sum per element, block and warp.
 #include "fused_single.h"
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
-#include <algorithm>
 #include <cstdint>
 
 #include "activation.cuh"
@@ -26,8 +26,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 128;
 constexpr int kStages = 4;
+constexpr int kEach = 4;
 constexpr int kMaxSplit = 8;  // blocks of a cluster that any launch may have
 
 // TM x TN elements per thread, 8 x 4 threads per warp; WN warps side by side along the vectors, WK warps on different parts
@@ -35,11 +35,10 @@ constexpr int kMaxSplit = 8;  // blocks of a cluster that any launch may have
 template <int TM_, int TN_, int WN_, int WK_, int KT_>
 struct Shape {
   static constexpr int TM = TM_, TN = TN_, WN = WN_, WK = WK_, KT = KT_;
-  static constexpr int BM = 8 * TM, BN = 4 * TN * WN;
-  static_assert(WN * WK * 32 == kThreads && KT % (4 * WK) == 0, "");
+  static constexpr int BM = 8 * TM, BN = 4 * TN * WN, THREADS = 32 * WN * WK;
+  static_assert(KT % (4 * WK) == 0, "");
 };
-using Wide = Shape<8, 4, 4, 1, 32>;     // 64 x 64
-using Narrow = Shape<4, 8, 1, 4, 64>;   // 32 x 32
+using Wide = Shape<8, 4, 4, 2, 32>;     // 64 x 64
 using Slim = Shape<4, 4, 1, 4, 64>;     // 32 x 16
 
 // Words of one operand's stage: `rows` lines of KT, or KT lines of `rows`.
@@ -65,17 +64,17 @@ __device__ __forceinline__ void copy_async(uint32_t to, const void* from, int va
 }
 
 // One operand's stage: rows [r0, r0 + ROWS) of `count`, inner elements [k0, k0 + KT) of those before `end`.
-template <bool MN, int ROWS, int KT, int VEC>
+template <bool MN, int ROWS, int KT, int VEC, int THREADS>
 __device__ __forceinline__ void load_stage(uint32_t to, const float* base, long long ld, long long r0, long long count, long long k0,
                                            long long end) {
   constexpr int LINE = MN ? ROWS : KT, LINES = MN ? KT : ROWS, PITCH = pitch_of<MN>(ROWS, KT);
   constexpr int PIECES = LINE / VEC * LINES;
-  static_assert(PIECES % kThreads == 0, "");
+  static_assert(PIECES % THREADS == 0, "");
   const long long one0 = MN ? r0 : k0, one_end = MN ? count : end;
   const long long two0 = MN ? k0 : r0, two_end = MN ? end : count;
 #pragma unroll
-  for (int i = 0; i < PIECES / kThreads; ++i) {
-    const int p = i * kThreads + static_cast<int>(threadIdx.x);
+  for (int i = 0; i < PIECES / THREADS; ++i) {
+    const int p = i * THREADS + static_cast<int>(threadIdx.x);
     const int line = p / (LINE / VEC), word = p % (LINE / VEC) * VEC;
     const long long one = one0 + word, two = two0 + line;
     long long left = one_end - one;
@@ -112,7 +111,7 @@ __device__ __forceinline__ void read_operand(float (&v)[N][4], const float* stag
 }
 
 template <class S, bool AMN, bool BMN, int VEC>
-__global__ void __launch_bounds__(kThreads) single_kernel(const SingleJob job, const long long k_per_block) {
+__global__ void __launch_bounds__(S::THREADS) single_kernel(const SingleJob job, const long long k_per_block) {
   constexpr int A_WORDS = words_of<AMN>(S::BM, S::KT), B_WORDS = words_of<BMN>(S::BN, S::KT);
   constexpr int A_PITCH = pitch_of<AMN>(S::BM, S::KT), B_PITCH = pitch_of<BMN>(S::BN, S::KT);
   extern __shared__ __align__(16) float ring[];
@@ -129,8 +128,8 @@ __global__ void __launch_bounds__(kThreads) single_kernel(const SingleJob job, c
     if (s < stages) {
       const uint32_t at = ring_at + 4u * static_cast<uint32_t>((s % kStages) * (A_WORDS + B_WORDS));
       const long long k0 = begin + static_cast<long long>(s) * S::KT;
-      load_stage<AMN, S::BM, S::KT, VEC>(at, job.a, job.lda, m0, job.m, k0, end);
-      load_stage<BMN, S::BN, S::KT, VEC>(at + 4u * A_WORDS, job.b, job.ldb, n0, job.n, k0, end);
+      load_stage<AMN, S::BM, S::KT, VEC, S::THREADS>(at, job.a, job.lda, m0, job.m, k0, end);
+      load_stage<BMN, S::BN, S::KT, VEC, S::THREADS>(at + 4u * A_WORDS, job.b, job.ldb, n0, job.n, k0, end);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -179,37 +178,49 @@ __global__ void __launch_bounds__(kThreads) single_kernel(const SingleJob job, c
   cluster.sync();
   constexpr int TILE = S::BM * S::BN;
   const int share = TILE / split;  // split is a power of two up to eight
-  for (int e = rank * share + static_cast<int>(threadIdx.x); e < (rank + 1) * share; e += kThreads) {
-    const long long f = m0 + e % S::BM, v = n0 + e / S::BM;
-    if (f >= job.m || v >= job.n) continue;
-    float part[kMaxSplit];
+  // kEach elements of a thread at a time, so that their reads overlap
+  for (int first = rank * share + static_cast<int>(threadIdx.x); first < (rank + 1) * share; first += kEach * S::THREADS) {
+    float y[kEach], add[kEach], z[kEach], bias[kEach];
+    bool in[kEach];
 #pragma unroll
-    for (int q = 0; q < kMaxSplit; ++q) {
-      part[q] = 0.f;
-      if (q < split) {
+    for (int u = 0; u < kEach; ++u) {
+      const int e = first + u * S::THREADS;
+      const long long f = m0 + e % S::BM, v = n0 + e / S::BM;
+      in[u] = e < (rank + 1) * share && f < job.m && v < job.n;
+      add[u] = in[u] && job.d != nullptr ? job.d[v * job.ldd + f] : 0.f;
+      z[u] = in[u] && job.grad && job.z != nullptr ? job.z[v * job.ldz + f] : 0.f;
+      bias[u] = in[u] && job.bias != nullptr ? job.bias[f] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int e = first + u * S::THREADS;
+      y[u] = 0.f;
+      if (!in[u]) continue;
+#pragma unroll
+      for (int q = 0; q < kMaxSplit; ++q) {
+        if (q >= split) break;
         const float* const other = cluster.map_shared_rank(ring, q);
 #pragma unroll
-        for (int w = 0; w < S::WK; ++w) part[q] += other[w * TILE + e];
+        for (int w = 0; w < S::WK; ++w) y[u] += other[w * TILE + e];
       }
+      y[u] = job.alpha * y[u] + bias[u];
     }
-    float y = part[0];
+    with_act(job.grad && job.z == nullptr ? static_cast<int>(kActIdentity) : job.act, [&](auto tag) {
+      constexpr int ACT = decltype(tag)::value;
 #pragma unroll
-    for (int q = 1; q < kMaxSplit; ++q) y += part[q];
-    y *= job.alpha;
-    const float add = job.d != nullptr ? job.beta * job.d[v * job.ldd + f] : 0.f;
-    if (job.grad) {
-      y += add;
-      if (job.z != nullptr) {
-        const float z = job.z[v * job.ldz + f];
-        with_act(job.act, [&](auto tag) { y *= act_slope<false, decltype(tag)::value>(z); });
+      for (int u = 0; u < kEach; ++u) {
+        const int e = first + u * S::THREADS;
+        const long long f = m0 + e % S::BM, v = n0 + e / S::BM;
+        const float more = job.beta * add[u];
+        if (job.grad) {
+          y[u] = (y[u] + more) * act_slope<false, ACT>(z[u]);
+        } else {
+          if (in[u] && job.z != nullptr) job.z[v * job.ldz + f] = y[u];
+          y[u] = act_value<false, ACT>(y[u]) + more;
+        }
+        if (in[u]) job.c[v * job.ldc + f] = y[u];
       }
-    } else {
-      if (job.bias != nullptr) y += job.bias[f];
-      if (job.z != nullptr) job.z[v * job.ldz + f] = y;
-      with_act(job.act, [&](auto tag) { y = act_value<false, decltype(tag)::value>(y); });
-      y += add;
-    }
-    job.c[v * job.ldc + f] = y;
+    });
   }
   cluster.sync();  // nobody leaves while its sums are being read
 }
@@ -236,7 +247,7 @@ cudaError_t launch_as(const SingleJob& job, cudaStream_t stream) {
   const int split = split_of<S>(job.m, job.n, job.k);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy), static_cast<unsigned>(split));
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3(S::THREADS);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attr = {};
@@ -265,14 +276,25 @@ cudaError_t launch_shape(const SingleJob& job, cudaStream_t stream) {
 
 }  // namespace
 
+// The tensor-core product takes 24 to 31 us for anything up to two waves of its tiles, the kernels here run at 20 to 27
+// TFLOP/s: 0.5e9 operations are where they meet (300 x 1000 x 1000: 29 us against 38; 256 x 1000 x 1000: 29 against 26).
+// With fewer than 128 vectors it does not run at all, and the CUDA-core kernels without a split take 148 to 970 us where
+// these take 85 to 153 (64 x 8192 x 2048 to 16 x 8192 x 8192); with fewer than 128 features its narrow form does, from
+// 2e9 operations on better than this.
 bool single_fits(long long m, long long n, long long k) {
-  return m <= 65535LL * 16 && n <= 65535LL * 16 && 2.0 * m * n * k < 1.2e9;
+  if (m > 65535LL * 16 || n > 65535LL * 16) return false;
+  const double work = 2.0 * m * n * k;
+  return n < 128 || work < (m < 128 ? 2e9 : 5e8);
 }
 
 cudaError_t launch_single(const SingleJob& job, cudaStream_t stream) {
-  if (job.n <= 16) return launch_shape<Slim>(job, stream);
-  if (job.n <= 32) return launch_shape<Narrow>(job, stream);
-  return launch_shape<Wide>(job, stream);
+  // The wide tile reads shared memory less often (100 x 4096 x 4096: 153 us against 174), the slim one wastes less on
+  // ragged edges (33 x 1000 x 4096: 24 us against 40) and makes more blocks of a small product (64 x 400 x 300: 6.0 us
+  // against 12.8).
+  const auto covered = [&](long long bm, long long bn) { return static_cast<double>(ceil_div(job.m, bm) * bm) * (ceil_div(job.n, bn) * bn); };
+  const long long wide_blocks = ceil_div(job.m, Wide::BM) * ceil_div(job.n, Wide::BN) * split_of<Wide>(job.m, job.n, job.k);
+  if (wide_blocks >= 148 && 0.8 * covered(Wide::BM, Wide::BN) < covered(Slim::BM, Slim::BN)) return launch_shape<Wide>(job, stream);
+  return launch_shape<Slim>(job, stream);
 }
 
 }  // namespace b200
