@@ -78,10 +78,10 @@ int resident_teams(int team) {
 // Time in SM cycles by a small model: waves of tiles, each the slower of its inner blocks and its epilogue, against the
 // memory traffic of the whole call, and what nothing hides at both ends. The constants were fitted to 190 problems with
 // every variant timed on each (sizes 1 to 8192, all kinds and types): the choice is within 2 % of the best one in the mean.
-// A stage of the narrow variants holds 128 inner elements, of the wide ones 64. Results in single precision wait for their
+// A stage holds 128 inner elements, of 128 x 256 on single SMs 64. Results in single precision wait for their
 // one accumulator on 256 columns.
 double estimate(const FusedDesc& d, int v, int split, bool vec) {
-  static constexpr double kBlock[kFusedVariants] = {720.0, 755.0, 700.0, 705.0, 730.0, 1000.0};
+  static constexpr double kBlock[kFusedVariants] = {1320.0, 755.0, 700.0, 705.0, 730.0, 1000.0};
   const FusedVariant& t = kFusedTable[v];
   const auto whole = [](double x) { return std::ceil(x); };
   const bool single = d.c_type == 32 || d.parts;
@@ -99,7 +99,7 @@ double estimate(const FusedDesc& d, int v, int split, bool vec) {
   const double block = kBlock[v] * (single && t.bn == 256 ? 1.7 : 1.0);
   const double load = t.stage_bytes / 73.5;
   const double waves = whole(tiles / resident_teams(t.ctas * split));
-  const double main = whole((d.parts ? 3.0 : 1.0) * whole(k / (64.0 * fused_stage_rows(t.bn))) / split) * (block > load ? block : load) + 1800.0;
+  const double main = whole((d.parts ? 3.0 : 1.0) * whole(k / (64.0 * fused_stage_rows(t.ctas, t.bn))) / split) * (block > load ? block : load) + 1800.0;
   // per column of a tile
   const bool reads_z = d.z != nullptr && d.grad, writes_z = d.z != nullptr && !d.grad;
   const bool adds = d.beta != 0.0 && d.d != nullptr;

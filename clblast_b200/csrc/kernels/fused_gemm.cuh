@@ -375,11 +375,11 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                   const FusedParams p) {
   static_assert(sizeof(DT) == sizeof(OT), "D and C share the staging buffers");
   constexpr bool CHUNKED = sizeof(OT) == 4 || MODE == kModeParts;  // sums beyond what the accumulators give
-  constexpr int CHUNK = (MODE == kModeParts ? kChunkParts : kChunkSingle) / (ROW_K * fused_stage_rows(BN));  // stages
+  constexpr int CHUNK = (MODE == kModeParts ? kChunkParts : kChunkSingle) / (ROW_K * fused_stage_rows(CTAS, BN));  // stages
   constexpr int EG = fused_groups(BN);
   constexpr int CB = 16;  // columns per epilogue block
   constexpr int B_ROWS = BN / CTAS;
-  constexpr int SUBS = fused_stage_rows(BN);  // a stage holds SUBS blocks of 64 inner elements, one after the other
+  constexpr int SUBS = fused_stage_rows(CTAS, BN);  // a stage holds SUBS blocks of 64 inner elements, one after the other
   constexpr int BK = ROW_K * SUBS;
   constexpr int A_BYTES = BM * ROW_K * 2;
   constexpr int SUB_BYTES = A_BYTES + B_ROWS * ROW_K * 2;
@@ -573,9 +573,11 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       const int in_row = valid % ROW_K;
       uint8_t* const s = base_ptr + stage * STAGE_BYTES + valid / ROW_K * SUB_BYTES;
       constexpr int TILES = BM / 64 + B_ROWS / 64;
-      for (int i = lane; i < rows * TILES * 8; i += 32) {
-        const int chunk = i & 7, r = (i >> 3) % rows, j = (i >> 3) / rows;
-        *reinterpret_cast<uint4*>(s + j * 8192 + (in_row + r) * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+      // eight lanes to a row, four rows at a time
+      for (int r = lane >> 3; r < rows; r += 4) {
+#pragma unroll
+        for (int j = 0; j < TILES; ++j)
+          *reinterpret_cast<uint4*>(s + j * 8192 + (in_row + r) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
       }
       fence_proxy_async();
       __syncwarp();

@@ -55,9 +55,11 @@ struct FusedParams {
 #else
 #define B200_HD
 #endif
-// Inner elements per operand stage, in swizzle rows of 64. The loops over the stages cost the same whatever a stage holds, and
-// up to 128 columns the MMAs of one swizzle row are shorter than that.
-B200_HD constexpr int fused_stage_rows(int bn) { return bn <= 128 ? 2 : 1; }
+// Inner elements per operand stage, in swizzle rows of 64. The loops over the stages take about 700 cycles whatever a stage
+// holds, more than the MMAs of one swizzle row (8192 x 8192 x 2048 on 256 x 256 pairs: 220 us with one row per stage, 212
+// with two; 32 groups of 512 x 2048 x 2048 into single precision 287 and 236). 128 x 256 on a single SM has no room for
+// more than two stages of two rows.
+B200_HD constexpr int fused_stage_rows(int ctas, int bn) { return ctas == 2 || bn <= 128 ? 2 : 1; }
 
 // Sizes of one kernel variant as the selection sees it.
 struct FusedVariant {
@@ -79,7 +81,7 @@ B200_HD constexpr int fused_staging_bytes(int bn, bool single, bool aux, int spl
 constexpr int kFusedBarBytes = 512;
 constexpr int kFusedVariants = 6;
 constexpr FusedVariant kFusedTable[kFusedVariants] = {
-    {2, 256, 32768}, {1, 256, 49152}, {1, 128, 65536}, {1, 64, 49152}, {1, 32, 40960}, {2, 128, 49152}};
+    {2, 256, 65536}, {1, 256, 49152}, {1, 128, 65536}, {1, 64, 49152}, {1, 32, 40960}, {2, 128, 49152}};
 
 // Enqueues variant `v` with operand type / D type / C type. `grid` counts CTAs, `smem` bytes of dynamic shared memory.
 cudaError_t launch_fused_variant(int v, int type, int d_type, int c_type, const CUtensorMap* maps, const FusedParams& p,
