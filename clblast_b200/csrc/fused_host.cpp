@@ -76,12 +76,12 @@ int resident_teams(int team) {
 }
 
 // Time in SM cycles by a small model: waves of tiles, each the slower of its inner blocks and its epilogue, against the
-// memory traffic of the whole call, and what nothing hides at both ends. The constants were fitted to 190 problems with
-// every variant timed on each (sizes 1 to 8192, all kinds and types): the choice is within 2 % of the best one in the mean.
+// memory traffic of the whole call, and what nothing hides at both ends. The constants were fitted to 727 problems with
+// every variant timed on each (sizes 1 to 8192, all kinds and types): the choice is within 3 % of the best one in the mean.
 // A stage holds 128 inner elements, of 128 x 256 on single SMs 64. Results in single precision wait for their
 // one accumulator on 256 columns.
 double estimate(const FusedDesc& d, int v, int split, bool vec) {
-  static constexpr double kBlock[kFusedVariants] = {1320.0, 755.0, 700.0, 705.0, 730.0, 1000.0};
+  static constexpr double kBlock[kFusedVariants] = {1320.0, 743.0, 700.0, 704.0, 700.0, 1000.0};
   const FusedVariant& t = kFusedTable[v];
   const auto whole = [](double x) { return std::ceil(x); };
   const bool single = d.c_type == 32 || d.parts;
@@ -97,23 +97,23 @@ double estimate(const FusedDesc& d, int v, int split, bool vec) {
   }
   const double tiles = d.tri ? tm * (tm + 1.0) / 2.0 * problems : tm * tn * problems;
   const double block = kBlock[v] * (single && t.bn == 256 ? 1.7 : 1.0);
-  const double load = t.stage_bytes / 73.5;
+  const double load = t.stage_bytes / 71.6;
   const double waves = whole(tiles / resident_teams(t.ctas * split));
-  const double main = whole((d.parts ? 3.0 : 1.0) * whole(k / (64.0 * fused_stage_rows(t.ctas, t.bn))) / split) * (block > load ? block : load) + 1800.0;
+  const double main = whole((d.parts ? 3.0 : 1.0) * whole(k / (64.0 * fused_stage_rows(t.ctas, t.bn))) / split) * (block > load ? block : load) + 2350.0;
   // per column of a tile
   const bool reads_z = d.z != nullptr && d.grad, writes_z = d.z != nullptr && !d.grad;
   const bool adds = d.beta != 0.0 && d.d != nullptr;
-  double column = 12.0 + (d.act != 161 ? 6.0 : 0.0) + (adds ? 4.3 : 0.0) + (d.z != nullptr ? 4.3 : 0.0);
+  double column = 10.1 + (d.act != 161 ? 7.5 : 0.0) + (adds ? 4.3 : 0.0) + (d.z != nullptr ? 4.3 : 0.0);
   if (single) column *= 1.5;
-  if (!vec) column += 5.6 * (1.0 + (writes_z ? 1.0 : 0.0) + (reads_z ? 0.5 : 0.0) + (adds ? 0.5 : 0.0));
+  if (!vec) column += 4.65 * (1.0 + (writes_z ? 1.0 : 0.0) + (reads_z ? 0.5 : 0.0) + (adds ? 0.5 : 0.0));
   double epilogue = column * t.bn;
-  if (split > 1) epilogue = 3.0 * epilogue / split + 5000.0 + 10.0 * t.bn;
+  if (split > 1) epilogue = 3.0 * epilogue / split + 5500.0 + 10.0 * t.bn;
   // each operand read once and C written once
   const double a_planes = d.kind == kFusedRaggedCols ? active : (d.a_stride != 0 ? problems : 1.0);
   const double c_planes = d.kind == kFusedRaggedCols ? 1.0 : static_cast<double>(d.problems);
   const double bytes = 2.0 * d.k * (a_planes * rows + cols * (d.kind == kFusedPlain ? problems : 1.0)) +
                        c_planes * rows * cols * (single ? 4.0 : 2.0);
-  const double work = waves * (main > epilogue ? main : epilogue), memory = bytes / 3600.0;
+  const double work = waves * (main > epilogue ? main : epilogue), memory = bytes / 4136.0;
   return (work > memory ? work : memory) + 6000.0 + epilogue;
 }
 
