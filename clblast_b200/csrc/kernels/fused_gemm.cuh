@@ -7,9 +7,10 @@
 // the epilogue owns one feature (one tensor-memory lane) and walks along the vectors: the bias is one register, the
 // bias gradient a running sum, and a 32-lane store covers consecutive addresses.
 //
-// Warp roles: warp 0 lane 0 issues the TMA loads of the operand ring, warp 1 the MMAs (and clears what a ragged inner
-// extent leaves behind its end), warp 2 builds the group table, warps 4.. drain the accumulators in groups of four warps, each group its own range
-// of the tile's columns. Two accumulators alternate, so a tile is drained under the next one's MMAs.
+// Warp roles: warp 0 issues the TMA loads of the operand ring, warp 1 the MMAs (and clears what a ragged inner extent
+// leaves behind its end), warp 2 builds the group table, warp 3 asks for D and Z of the next tile, warps 4.. drain the
+// accumulators in groups of four warps, each group its own range of the tile's columns. Two accumulators alternate, so a
+// tile is drained under the next one's MMAs.
 //   CTAS == 2: a cluster of two CTAs works on 256 x BN tiles with cta_group::2, each CTA staging half of op(B).
 //   CTAS == 1: tiles of 128 x BN; a cluster of p.split CTAs may share a tile's inner extent. Each CTA then leaves its
 //   fp32 sums in its own shared memory and the CTAs add them up for a range of columns each, in the order of the ranks
@@ -17,7 +18,7 @@
 //
 // The epilogue goes by blocks of 16 columns x 32 rows, each warp by itself. A lane holds one row of a block while memory
 // runs along the rows, so blocks are turned round in 1 to 2 KB of the warp's own shared memory and leave as 16-byte
-// stores, four lanes to a column (C in half precision); D and Z come in the same way, two blocks ahead in registers.
+// stores, four lanes to a column (C in half precision); D and Z come in the same way, one block ahead in registers.
 // Columns and rows that end inside a block are cut off lane by lane. (Staging through TMA with a barrier among the warps
 // per block, the form of the half-precision GEMM kernels, took 115 us for 8192 x 8192 x 512 and could not cut a group's
 // columns.)
@@ -25,7 +26,14 @@
 // Sums for results in single precision: the tensor cores cut off instead of rounding when they add to an accumulator, an
 // error of about 4e-8 of the result per 16 inner elements that all points towards zero. Results in 16 bits do not see it.
 // For the others an accumulator takes a few blocks at most and is then added, rounded, to sums in further columns of
-// tensor memory (which the widest tile has room for only with one accumulator instead of two).
+// tensor memory (which the widest tile has room for only with one accumulator instead of two). The same sums in registers
+// spill: 286 us against 247 for 32 weight gradients of 512 rows, 2048 x 2048 each, on 128 x 128 tiles.
+//
+// What bounds it: products of 10^11 operations and more the board's power (8192 x 8192 x 2048 in bfloat16 with bias, gelu
+// and Z kept 207 us, 1.33 PFLOP/s, tensor pipe busy 70 % of the cycles; a plain library product sustains 1.40); weight
+// gradients in single precision the writes, which nothing hides while an accumulator is being emptied (236 us, 2.8 TB/s);
+// decoding the reads of the weights (48 x 4096 x 8192 16.5 us, 4.1 TB/s, of which 5 us are the start and the meeting of
+// the split tiles).
 //
 // All waits are bounded; on expiry a code is left in the status word and every role leaves its loop.
 #pragma once
