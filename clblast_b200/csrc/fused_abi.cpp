@@ -61,7 +61,11 @@ int check(size_t one, size_t two, size_t planes, const void* buf, size_t offset,
   CUdeviceptr base = 0;
   size_t size = 0;
   const CUdeviceptr at = reinterpret_cast<CUdeviceptr>(buf);
-  if (drv.MemGetAddressRange(&base, &size, at) != CUDA_SUCCESS) return invalid;
+  if (drv.MemGetAddressRange(&base, &size, at) != CUDA_SUCCESS) {
+    // a host thread's first call finds no context: that binds the device's own (backward passes run on such threads)
+    unsigned long long key = 0;
+    if (context_key(&key) != 0 || drv.MemGetAddressRange(&base, &size, at) != CUDA_SUCCESS) return invalid;
+  }
   if (drv.PointerGetAttribute) {
     int owner = -1, current = -2;
     if (drv.PointerGetAttribute(&owner, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, at) == CUDA_SUCCESS &&
@@ -121,9 +125,20 @@ bool beside(const Area& x, const Area& c, bool same_allowed) {
   return gap >= c_line && gap + x_line <= pitch;
 }
 
+// What a first call sets up (the status block, the pool, kernel attributes) would invalidate a capture that this thread is
+// recording in the usual mode; none of it is work on the captured stream.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  const bool on = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+  ~RelaxedCapture() {
+    if (on) (void)cudaThreadExchangeStreamCaptureMode(&mode);
+  }
+};
+
 template <class F>
 int guarded(F&& f) {
   try {
+    RelaxedCapture relaxed;
     return f();
   } catch (...) {
     return kUnexpectedError;

@@ -189,7 +189,8 @@ int b200blas_gemm_epilogue_grad(int dtype, int layout, int a_transpose, int b_tr
 /* DZ = DY * act'(Z) for `rows` contiguous vectors of n elements, and the sums of DZ over the rows: the same for a
  * gradient that no product of this library produced. DZ or bias_grad may be absent; DZ may be DY or Z. With `groups`
  * > 0 there is one bias gradient per group (lines of bias_grad_ld elements) and only the rows of groups are touched
- * (see b200blas_gemm_grouped); group_offsets is NULL exactly when groups == 0. dtype 16, bf16, 32. */
+ * (see b200blas_gemm_grouped), at most 64 * (65535 - groups) of them (kInvalidDimension); group_offsets is NULL exactly
+ * when groups == 0. dtype 16, bf16, 32. */
 int b200blas_activation_grad(int dtype, size_t rows, size_t n, int activation, const void* dy, size_t dy_offset,
                              size_t dy_ld, const void* z, size_t z_offset, size_t z_ld, void* dz, size_t dz_offset,
                              size_t dz_ld, void* bias_grad, size_t bias_grad_offset, size_t groups,

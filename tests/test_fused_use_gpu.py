@@ -311,6 +311,63 @@ def test_capture_of_copies_and_single_precision(cuda):
     healthy()
 
 
+def test_host_threads(cuda):
+    """Several host threads, each with a stream and leaves of its own, at once: results are those of one thread alone."""
+    import threading
+    torch = cuda
+    steps = [make(torch, 100 * i) for i in range(4)]
+    alone = [make(torch, 100 * i) for i in range(4)]
+    for e in alone:
+        e.step(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(e, i):
+        try:
+            stream = torch.cuda.Stream()
+            for j in range(5):
+                e.step(stream if i % 2 else None)  # synchronous calls among them
+            stream.synchronize()
+        except BaseException as error:  # noqa: BLE001
+            failures.append(error)
+
+    threads = [threading.Thread(target=work, args=(e, i)) for i, e in enumerate(steps)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failures, failures
+    for e, want in zip(steps, alone):
+        for p, q in zip(e.results, want.results):
+            assert torch.equal(p, q)
+    healthy()
+
+
+def test_first_calls_of_a_process_captured(cuda):
+    """Nothing has to run before a capture: what the library sets up at first use can be set up while a graph records."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from tests.test_fused_use_gpu import make
+e, ref = make(torch), make(torch)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    e.step(torch.cuda.current_stream())
+graph.replay()
+torch.cuda.synchronize()
+ref.step(torch.cuda.current_stream())
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(e.results, ref.results))
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
 # ---- few vectors -----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5])
@@ -394,6 +451,44 @@ def test_offsets_past_32_bits(cuda):
     for i, (lo, hi) in enumerate(((0, 100), (100, 100), (100, 300))):
         want, mag = R.product(y0[lo:hi].t(), x0[lo:hi], 1.0)
         R.check(wide[i], want, R.stored(want, R.sum_error(hi - lo, dtype) * mag, dtype), "weight gradient")
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_many_vectors(cuda, dtype):
+    """More vectors than a grid has rows of blocks: products, their gradients and the sums over all vectors. Values are
+    small integers, so that sums over four million of them are exact in single precision below 2^24."""
+    torch = cuda
+    dtype = getattr(torch, dtype)
+    rows, n, k = 4_300_000, 8, 16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randint(-1, 2, (rows, k), generator=g, device="cuda").to(dtype)
+    w = torch.randint(-1, 2, (n, k), generator=g, device="cuda").to(dtype)
+    c, sums = torch.zeros(rows, n, device="cuda", dtype=dtype), torch.zeros(n, device="cuda", dtype=dtype)
+    stream = torch.cuda.current_stream()
+    want = x.double() @ w.double().t()
+    total = want.sum(0)
+    assert cb.GemmEpilogue(ROW, NO, YES, rows, n, k, 1.0, x, 0, k, w, 0, k, None, 0, 162, None, 0, n, 0.0, None, 0, n, c, 0, n, stream=stream) == OK
+    assert torch.equal(c.double(), want.clamp(min=0))
+    assert cb.GemmEpilogueGrad(ROW, NO, YES, rows, n, k, 1.0, x, 0, k, w, 0, k, 0.0, None, 0, n, 161, None, 0, n, c, 0, n, sums, 0, stream=stream) == OK
+    assert torch.equal(c.double(), want) and torch.equal(sums, total.to(dtype))
+    sums.zero_()
+    assert cb.ActivationGrad(rows, n, 161, c, 0, n, None, 0, n, None, 0, n, sums, 0, stream=stream) == OK
+    assert torch.equal(sums, total.to(dtype))
+    if dtype == torch.float16:
+        off = torch.tensor([0, 1, 1, 4_000_000, rows], dtype=torch.int64, device="cuda")
+        y = torch.zeros_like(c)
+        wg = torch.stack([w, -w, w, -w])
+        assert cb.GemmGrouped(YES, 4, rows, n, k, 1.0, x, 0, k, wg, 0, k, n * k, off, None, 0, n, 161, None, 0, n, 0.0, None, 0, n, y, 0, n,
+                              stream=stream) == OK
+        want[4_000_000:] *= -1
+        assert torch.equal(y.double(), want)
+        dw = torch.zeros(4, n, k, device="cuda")
+        assert cb.GemmGroupedWeight(4, rows, n, k, 1.0, y, 0, n, x, 0, k, off, 0.0, dw, 0, k, n * k, stream=stream) == OK
+        for i, (lo, hi) in enumerate(((0, 1), (1, 1), (1, 4_000_000), (4_000_000, rows))):
+            exact = y[lo:hi].double().t() @ x[lo:hi].double()
+            bound = R.sum_error(hi - lo, dtype) * (y[lo:hi].double().abs().t() @ x[lo:hi].double().abs())
+            R.check(dw[i], exact, R.stored(exact, bound, torch.float32), "weight gradient")
     healthy()
 
 
