@@ -146,8 +146,11 @@ Choice choose(const FusedDesc& d, bool vec) {
   return best;
 }
 
+// Addresses and strides of a tensor map are multiples of 16 bytes, strides below 2^40.
 bool unaddressable(const void* base, long long ld, long long planes, long long stride) {
-  return (reinterpret_cast<uintptr_t>(base) & 15) != 0 || (ld % 8) != 0 || (planes > 1 && (stride % 8) != 0);
+  constexpr long long kFar = 1LL << 39;
+  return (reinterpret_cast<uintptr_t>(base) & 15) != 0 || (ld % 8) != 0 || ld >= kFar ||
+         (planes > 1 && ((stride % 8) != 0 || stride >= kFar));
 }
 
 }  // namespace

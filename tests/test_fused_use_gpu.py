@@ -492,6 +492,23 @@ def test_many_vectors(cuda, dtype):
     healthy()
 
 
+def test_leading_dimension_of_a_single_line(cuda):
+    """Of a matrix with one line the leading dimension is never walked, however large."""
+    torch = cuda
+    n, k, far = 136, 72, 2 ** 40
+    x, w = randn(torch, 1, (1, k), torch.float16), randn(torch, 2, (n, k), torch.float16, k ** -0.5)
+    z, c, sums = randn(torch, 3, (1, n), torch.float16), torch.zeros(1, n, device="cuda", dtype=torch.float16), torch.zeros(n, device="cuda", dtype=torch.float16)
+    stream = torch.cuda.current_stream()
+    want, tol, total, t_tol = R.backward(x, w.t(), 1.0, 0.0, None, 165, z, torch.float16)
+    for bias_grad in (sums, None):
+        c.zero_()
+        assert cb.GemmEpilogueGrad(ROW, NO, YES, 1, n, k, 1.0, x, 0, far, w, 0, k, 0.0, None, 0, n, 165, z, 0, far, c, 0, far, bias_grad, 0,
+                                   stream=stream) == OK
+        R.check(c, want, tol, "C")
+    R.check(sums, total, t_tol, "bias gradient")
+    healthy()
+
+
 # ---- refusals --------------------------------------------------------------------------------------------------------
 
 def test_refused_on_a_device(cuda):
