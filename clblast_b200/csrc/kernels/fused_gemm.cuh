@@ -30,7 +30,7 @@
 // spill: 286 us against 247 for 32 weight gradients of 512 rows, 2048 x 2048 each, on 128 x 128 tiles.
 //
 // What bounds it: products of 10^11 operations and more the board's power (8192 x 8192 x 2048 in bfloat16 with bias, gelu
-// and Z kept 207 us, 1.33 PFLOP/s, tensor pipe busy 70 % of the cycles; a plain library product sustains 1.40); weight
+// and Z kept 207 us, 1.33 PFLOP/s, tensor pipe busy 77 % of the cycles; a plain library product sustains 1.40); weight
 // gradients in single precision the writes, which nothing hides while an accumulator is being emptied (236 us, 2.8 TB/s);
 // decoding the reads of the weights (48 x 4096 x 8192 16.5 us, 4.1 TB/s, of which 5 us are the start and the meeting of
 // the split tiles).

@@ -509,6 +509,22 @@ def test_leading_dimension_of_a_single_line(cuda):
     healthy()
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("act", [162, 163, 164, 165])
+def test_limits_of_activations(cuda, dtype, act):
+    """At infinities and the type's largest numbers: the value tends to z and 0, the slope to 1 and 0; NaN stays NaN."""
+    torch = cuda
+    dtype = getattr(torch, dtype)
+    most = torch.finfo(dtype).max
+    z = torch.tensor([[float("inf"), most, 1e4, 100.0, float("-inf"), -most, -1e4, -100.0, float("nan"), 0.0]], device="cuda", dtype=dtype)
+    n, stream = z.numel(), torch.cuda.current_stream()
+    one, dy, dz, c = torch.ones(1, 1, device="cuda", dtype=dtype), torch.ones_like(z), torch.zeros_like(z), torch.zeros_like(z)
+    assert cb.ActivationGrad(1, n, act, dy, 0, n, z, 0, n, dz, 0, n, None, 0, stream=stream) == OK
+    assert (dz[0, :4] == 1).all() and (dz[0, 4:8] == 0).all() and torch.isnan(dz[0, 8]) and dz[0, 9] == (0.0 if act == 162 else 0.5)
+    assert cb.GemmEpilogue(ROW, NO, NO, 1, n, 1, 1.0, one, 0, 1, z, 0, n, None, 0, act, None, 0, n, 0.0, None, 0, n, c, 0, n, stream=stream) == OK
+    assert torch.equal(c[0, :4], z[0, :4]) and (c[0, 4:8] == 0).all() and torch.isnan(c[0, 8]) and c[0, 9] == 0
+
+
 # ---- refusals --------------------------------------------------------------------------------------------------------
 
 def test_refused_on_a_device(cuda):
