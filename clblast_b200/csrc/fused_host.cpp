@@ -229,7 +229,7 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   p.raster = t.ctas == 2 ? 8 : 16;
   p.tri = d.tri;
   p.parts = d.parts;
-  p.chained = d.chained;
+  p.chained = d.chained || a_bytes + b_bytes > 0;  // right behind the copies
   p.a_mn = d.a_mn;
   p.b_mn = d.b_mn;
   const unsigned format = d.type == 16 ? 0u : 1u;  // fp32 accumulator; f16 or bf16 operands

@@ -28,6 +28,7 @@ struct PackPair {
 };
 __global__ void __launch_bounds__(kPackThreads) pack_kernel(const PackPair pair) {
   __shared__ __align__(16) unsigned short buf[kPackThreads * kPackVec];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the product behind it may be set up meanwhile
   const int which = blockIdx.x >= pair.first_of_second ? 1 : 0;
   const unsigned block = blockIdx.x - (which ? pair.first_of_second : 0u);
   const PackJob& job = pair.job[which];
@@ -197,6 +198,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormaliseJob job) {
 template <class T, class X, bool PARTS>
 __global__ void __launch_bounds__(256) scale_kernel(const NormaliseJob job, int blocks) {
   __shared__ double factor;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x < 32) {
     double t = 0.0;
     for (int i = threadIdx.x; i < blocks; i += 32) t += job.sums[static_cast<long long>(blockIdx.y) * blocks + i];
