@@ -57,8 +57,22 @@ long long column_tiles(const FusedDesc& d, int bn) {
   return d.kind == kFusedRaggedCols ? whole + d.problems : whole;
 }
 
+// Shared memory that a variant needs besides the operand ring: alignment, staging or the sums of split tiles, barriers and
+// the group table (8 bytes per group; a thousand groups take 8 KB).
+int fixed_smem(const FusedDesc& d, int v, int split) {
+  const bool single = d.c_type == 32 || d.parts;
+  const int table = d.kind != kFusedPlain ? 8 * (static_cast<int>(d.problems) + 1) : 0;
+  return kAlign + fused_staging_bytes(kFusedTable[v].bn, single, d.z != nullptr, split) + kFusedBarBytes + table;
+}
+// Stages of the ring in what is left; the kernel works from two on.
+int ring_stages(const FusedDesc& d, int v, int split) {
+  const int stages = (kMaxSmem - fixed_smem(d, v, split)) / kFusedTable[v].stage_bytes;
+  return stages < 12 ? stages : 12;
+}
+
 bool variant_fits(const FusedDesc& d, int v, int split) {
   const FusedVariant& t = kFusedTable[v];
+  if (ring_stages(d, v, split) < 2) return false;  // 128 x 256 with a split from 192 groups on
   if (t.ctas == 2 && split > 1) return false;
   if (d.b_mn && t.bn / t.ctas < 64) return false;                               // a 128-byte row is 64 columns
   if (d.tri && t.ctas * 128 != t.bn) return false;                               // square tiles meet their mirror image
@@ -268,7 +282,6 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   if (d.kind != kFusedRaggedCols) tiles *= d.problems;
   if (d.tri) tiles = static_cast<long long>(p.tiles_m) * (p.tiles_m + 1) / 2 * d.problems;
   if (tiles > 0x3FFFFFFF) return cudaErrorInvalidValue;
-  const bool single = d.c_type == 32 || d.parts;  // sums beside the accumulators, blocks of four bytes
   const int lines_per_tile = fused_groups(t.bn) * choice.split;
   if (d.bias_grad != nullptr) {
     e = partial.get(static_cast<size_t>(col_tiles) * lines_per_tile * d.m * sizeof(float), stream);
@@ -276,14 +289,8 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
     p.partial = reinterpret_cast<float*>(partial.ptr());
   }
 
-  // shared memory: the ring takes what staging, barriers and the group table leave
-  const int table = d.kind != kFusedPlain ? 8 * (p.problems + 1) : 0;
-  const int fixed = kAlign + fused_staging_bytes(t.bn, single, p.z != nullptr, choice.split) + kFusedBarBytes + table;
-  int stages = (kMaxSmem - fixed) / t.stage_bytes;
-  if (stages > 12) stages = 12;
-  if (stages < 2) return cudaErrorInvalidValue;
-  p.stages = stages;
-  const int smem = fixed + stages * t.stage_bytes;
+  p.stages = ring_stages(d, choice.variant, choice.split);
+  const int smem = fixed_smem(d, choice.variant, choice.split) + p.stages * t.stage_bytes;
 
   const int team = t.ctas * choice.split;
   long long teams = resident_teams(team);
