@@ -61,32 +61,26 @@ cudaError_t kernel_ready(const void* func, int smem_bytes, int* regs) {
   static std::map<std::pair<unsigned long long, const void*>, Entry> table;  // (context, kernel)
   unsigned long long ctx = 0;
   if (context_key(&ctx) != 0) ctx = 0;  // no key: fall through to the runtime calls every time
-  {
-    std::lock_guard<std::mutex> lock(guard);
-    const auto it = table.find({ctx, func});
-    if (ctx != 0 && it != table.end() && it->second.smem >= smem_bytes && (regs == nullptr || it->second.regs > 0)) {
-      if (regs) *regs = it->second.regs;
-      return cudaSuccess;
-    }
-  }
-  Entry e = {smem_bytes, 0};
+  // The lock is held across the runtime calls: of two first calls the one with the smaller size could otherwise set the
+  // attribute last while the table keeps the larger, and every launch with that would fail from then on.
+  std::lock_guard<std::mutex> lock(guard);
+  const auto it = table.find({ctx, func});
+  const Entry known = ctx != 0 && it != table.end() ? it->second : Entry{0, 0};
+  Entry e = {smem_bytes > known.smem ? smem_bytes : known.smem, known.regs};
   if (regs) {
-    cudaFuncAttributes attr;
-    const cudaError_t ga = cudaFuncGetAttributes(&attr, func);
-    if (ga != cudaSuccess) return ga;
-    e.regs = attr.numRegs;
-    *regs = attr.numRegs;
+    if (e.regs == 0) {
+      cudaFuncAttributes attr;
+      const cudaError_t ga = cudaFuncGetAttributes(&attr, func);
+      if (ga != cudaSuccess) return ga;
+      e.regs = attr.numRegs;
+    }
+    *regs = e.regs;
   }
-  if (smem_bytes > 48 * 1024) {
-    const cudaError_t sa = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+  if (e.smem > known.smem && e.smem > 48 * 1024) {
+    const cudaError_t sa = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, e.smem);
     if (sa != cudaSuccess) return sa;
   }
-  if (ctx != 0) {
-    std::lock_guard<std::mutex> lock(guard);
-    Entry& slot = table[{ctx, func}];
-    if (slot.smem < e.smem) slot.smem = e.smem;
-    if (e.regs > 0) slot.regs = e.regs;
-  }
+  if (ctx != 0) table[{ctx, func}] = e;
   return cudaSuccess;
 }
 

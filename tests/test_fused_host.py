@@ -77,3 +77,12 @@ def test_every_call_finds_a_kernel(selection):
             kw.update(c_type=rng.choice([kw["type"], SINGLE]))
         calls.append(call(kind, problems, size(16384), size(65536), size(65536), **kw))
     launched(selection, calls)
+
+
+def test_kernel_attributes_are_never_lowered(tmp_path_factory):
+    """A kernel is launched with sizes that vary from call to call, from several threads: once a size is recorded as set,
+    no other call may set a smaller one."""
+    exe = compiled(tmp_path_factory, "kernel_ready", ROOT / "tests" / "host" / "kernel_ready.cpp", CSRC / "runtime_state.cpp")
+    for _ in range(3):
+        done = subprocess.run([exe], capture_output=True, text=True, check=True, timeout=60)
+        assert done.stdout.split() == ["230000", "230000", "77"]

@@ -16,3 +16,49 @@ def test_groups_beside_the_sums_of_split_tiles(cuda, monkeypatch):
             grouped(cuda, monkeypatch, v, "half", "single", sizes, sum(sizes) + 3, 72, 264, beta=1.0)
             grouped(cuda, monkeypatch, v, "half", "half", sizes, sum(sizes) + 3, 72, 264, grad=True, beta=1.0)
             weight(cuda, monkeypatch, v, "bf16", "single", sizes, sum(sizes) + 3, 72, 40, first=3, poison=True, beta=1.0)
+
+
+def test_first_calls_of_threads_with_different_sizes(cuda):
+    """The first calls of a process, on threads that start together and whose launches of the same kernels need different
+    amounts of shared memory (with and without Z, few and many groups); then every call again."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import threading
+import torch
+import clblast_b200 as cb
+ROW, NO, YES = 101, 111, 112
+rows, n, k = 1024, 264, 128
+half = lambda *shape: torch.randn(*shape, device="cuda").half()
+x, w, wg = half(rows, k), half(n, k), half(1024, n, k)
+z = torch.empty(rows, n, device="cuda", dtype=torch.half)
+calls = []
+for keep in (True, False):
+    calls.append(lambda c, s, keep=keep: cb.GemmEpilogue(ROW, NO, YES, rows, n, k, 1.0, x, 0, k, w, 0, k, None, 0, 161, z if keep else None, 0, n,
+                                                         0.0, None, 0, n, c, 0, n, stream=s))
+for groups in (1024, 2, 300, 40):
+    off = torch.linspace(0, rows, groups + 1, device="cuda").long()
+    calls.append(lambda c, s, groups=groups, off=off: cb.GemmGrouped(YES, groups, rows, n, k, 1.0, x, 0, k, wg, 0, k, n * k, off, None, 0, n, 161,
+                                                                     None, 0, n, 0.0, None, 0, n, c, 0, n, stream=s))
+outs = [torch.empty(rows, n, device="cuda", dtype=torch.half) for _ in calls]
+torch.cuda.synchronize()
+start, states = threading.Barrier(len(calls)), []
+def work(f, c):
+    stream = torch.cuda.Stream()
+    start.wait()
+    states.append(int(f(c, stream)))
+    stream.synchronize()
+threads = [threading.Thread(target=work, args=p) for p in zip(calls, outs)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+for f, c in zip(calls, outs):
+    again = torch.empty_like(c)
+    states.append(int(f(again, torch.cuda.current_stream())))
+    torch.cuda.synchronize()
+    assert torch.equal(c, again)
+assert states == [0] * (2 * len(calls)), states
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
