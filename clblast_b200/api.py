@@ -357,9 +357,10 @@ _OK = StatusCode.kSuccess
 
 def _learn_types():
     import torch
-    _CODE_OF.update({torch.float16: 16, torch.bfloat16: 1016, torch.float32: 32, torch.float64: 64,
-                     torch.complex64: 3232, torch.complex128: 6464})
-    _DTYPE_OF.update({code: dtype for dtype, code in _CODE_OF.items()})
+    codes = {torch.float16: 16, torch.bfloat16: 1016, torch.float32: 32, torch.float64: 64, torch.complex64: 3232,
+             torch.complex128: 6464}
+    _DTYPE_OF.update({code: dtype for dtype, code in codes.items()})
+    _CODE_OF.update(codes)  # last: another thread takes both tables for complete once this one holds something
 
 
 def _types(operand, result, precision, c_precision):
