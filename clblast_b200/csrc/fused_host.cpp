@@ -73,6 +73,8 @@ int ring_stages(const FusedDesc& d, int v, int split) {
 bool variant_fits(const FusedDesc& d, int v, int split) {
   const FusedVariant& t = kFusedTable[v];
   if (ring_stages(d, v, split) < 2) return false;  // 128 x 256 with a split from 192 groups on
+  const int team = t.ctas * split;
+  if (team > 1 && sm_budget() > 0 && team > sm_budget()) return false;  // a tile's CTAs run at once
   if (t.ctas == 2 && split > 1) return false;
   if (d.b_mn && t.bn / t.ctas < 64) return false;                               // a 128-byte row is 64 columns
   if (d.tri && t.ctas * 128 != t.bn) return false;                               // square tiles meet their mirror image

@@ -86,3 +86,24 @@ def test_kernel_attributes_are_never_lowered(tmp_path_factory):
     for _ in range(3):
         done = subprocess.run([exe], capture_output=True, text=True, check=True, timeout=60)
         assert done.stdout.split() == ["230000", "230000", "77"]
+
+
+def test_limit_on_multiprocessors(selection):
+    """No more CTAs than the SMs that the caller leaves, whatever the tiles: pairs and split tiles take several each."""
+    rng = random.Random(1)
+    size = lambda most: max(1, int(most ** rng.random()))
+    calls = []
+    for _ in range(1500):
+        budget = rng.choice([1, 2, 3, 4, 5, 7, 8, 12, 33, 100, 147])
+        rows = 5 + size(8192)
+        calls.append(rng.choice([
+            call(PLAIN, 1, size(8192), rows, size(8192), budget=budget),
+            call(PLAIN, 1, size(8192), rows, size(8192), grad=1, z=1, bias_grad=1, budget=budget),
+            call(COLS, size(64), size(4096), rows, size(4096), budget=budget),
+            call(INNER, size(64), size(4096), size(4096), rows, c_type=SINGLE, a_mn=1, b_mn=1, budget=budget)]))
+    for side in (8, 256, 1024, 4096):
+        calls += [call(PLAIN, 2, side, side, 512, type=HALF, tri=1, parts=parts, budget=budget) for budget in (1, 2, 5) for parts in (0, 1)]
+    for c, row in zip(calls, launched(selection, calls)):
+        assert row[5] <= c[-1] or row[1] == -1, (c, row)
+    for form in ("0", "4,8"):  # asked for by name and too large
+        assert all(row[5] <= c[-1] or row[1] == -1 for c, row in zip(calls, launched(selection, calls, form)))

@@ -1,7 +1,8 @@
 """Fused products at the limits of what their kernels hold, against the same 64-bit forms as their other tests."""
 import pytest
 
-from tests.test_fused_gpu import grouped, weight
+import clblast_b200 as cb
+from tests.test_fused_gpu import NO, ROW, YES, grouped, linear, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +63,17 @@ print("same")
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("budget", [1, 2, 5])
+def test_few_multiprocessors(cuda, monkeypatch, budget):
+    """A limit below what a pair or a split tile takes: tiles of one SM serve the call, one after another."""
+    cb.set_sm_budget(budget)
+    try:
+        for v in (None, "0", "3,8"):
+            linear(cuda, monkeypatch, v, "half", "half", ROW, NO, YES, 70, 264, 200, act=165, beta=0.5)
+            linear(cuda, monkeypatch, v, "bf16", "bf16", ROW, NO, YES, 300, 520, 1000, act=164, grad=True, beta=1.0)
+            grouped(cuda, monkeypatch, v, "bf16", "single", [3, 0, 64, 33, 0, 1, 129], 240, 264, 200, beta=1.0)
+            weight(cuda, monkeypatch, v, "half", "single", [3, 0, 64, 33, 0, 1, 129], 240, 136, 264, beta=1.0)
+    finally:
+        cb.set_sm_budget(0)
