@@ -242,6 +242,9 @@ int check_offsets(const long long* offsets, size_t groups) {
   const int st = check(groups + 1, 1, 1, offsets, 0, groups + 1, 0, 8, kInvalidBatchCount, kInvalidBatchCount, kInvalidBatchCount);
   return st;
 }
+// Every CTA reads the offsets when it starts, at a time when others may be storing results already: were they written, the
+// CTAs of one tile could take different tiles.
+Span offsets_span(const long long* offsets, size_t groups) { return span_of(offsets, groups + 1, 1, groups + 1, 8); }
 
 }  // namespace
 }  // namespace b200
@@ -384,8 +387,11 @@ extern "C" int b200blas_activation_grad(int dtype, size_t rows, size_t n, int ac
     dz = at(dz, dz_offset, elem); bias_grad = at(bias_grad, bias_grad_offset, elem);
     const Area at_dy = {dy, n, rows, dy_ld, elem}, at_z = {z, n, rows, z_ld, elem}, at_dz = {dz, n, rows, dz_ld, elem};
     if (!beside(at_dy, at_dz, true) || !beside(at_z, at_dz, true)) return kInvalidMatrixC;
+    const Span sums = span_of(bias_grad, n, lines, line_ld, elem), offsets = offsets_span(group_offsets, groups);
+    if (overlap(offsets, at_dz.span())) return kInvalidMatrixC;
     for (const Area& in : {at_dy, at_z, at_dz})
-      if (overlap(in.span(), span_of(bias_grad, n, lines, line_ld, elem))) return kInvalidVectorY;
+      if (overlap(in.span(), sums)) return kInvalidVectorY;
+    if (overlap(offsets, sums)) return kInvalidVectorY;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
@@ -493,7 +499,7 @@ extern "C" int b200blas_gemm_grouped(int dtype, int c_dtype, int w_transpose, si
     const Area at_x = {f.b, k, rows, x_ld, elem};
     for (const Area& out : {at_c, at_z})
       if (!beside(at_x, out, false) || overlap(weights_span(g), out.span()) ||
-          overlap(span_of(f.bias, n, groups, bias_ld, elem), out.span()))
+          overlap(span_of(f.bias, n, groups, bias_ld, elem), out.span()) || overlap(offsets_span(group_offsets, groups), out.span()))
         return kInvalidMatrixC;
     if (!beside(at_z, at_c, false) || !beside(at_d, at_c, true) || !beside(at_d, at_z, false)) return kInvalidMatrixC;
     cudaStream_t s;
@@ -533,12 +539,14 @@ extern "C" int b200blas_gemm_grouped_grad(int dtype, int w_transpose, size_t gro
     f.bias_grad = at(bias_grad, bias_grad_offset, elem); f.bias_grad_stride = static_cast<long long>(bias_grad_ld);
     const Area at_c = {f.c, n, rows, c_ld, elem}, at_d = {f.d, n, rows, d_ld, elem}, at_z = {f.z, n, rows, z_ld, elem};
     const Area at_x = {f.b, k, rows, x_ld, elem};
-    if (!beside(at_x, at_c, false) || overlap(weights_span(g), at_c.span()) || !beside(at_z, at_c, true) || !beside(at_d, at_c, true))
+    const Span offsets = offsets_span(group_offsets, groups);
+    if (!beside(at_x, at_c, false) || overlap(weights_span(g), at_c.span()) || !beside(at_z, at_c, true) || !beside(at_d, at_c, true) ||
+        overlap(offsets, at_c.span()))
       return kInvalidMatrixC;
     const Span sums = span_of(f.bias_grad, n, groups, bias_grad_ld, elem);
     for (const Area& in : {at_x, at_c, at_d, at_z})
       if (overlap(in.span(), sums)) return kInvalidVectorY;
-    if (overlap(weights_span(g), sums)) return kInvalidVectorY;
+    if (overlap(weights_span(g), sums) || overlap(offsets, sums)) return kInvalidVectorY;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);
     if (r != 0) return r;
@@ -567,7 +575,8 @@ extern "C" int b200blas_gemm_grouped_weight(int dtype, int c_dtype, size_t group
     if ((st = check_offsets(group_offsets, groups))) return st;
     Span all = span_of(at(c, c_offset, c_elem), n, m, c_ld, c_elem);
     all.last += (groups - 1) * c_stride * c_elem;
-    if (overlap(span_of(at(x, x_offset, elem), m, rows, x_ld, elem), all) || overlap(span_of(at(y, y_offset, elem), n, rows, y_ld, elem), all))
+    if (overlap(span_of(at(x, x_offset, elem), m, rows, x_ld, elem), all) || overlap(span_of(at(y, y_offset, elem), n, rows, y_ld, elem), all) ||
+        overlap(offsets_span(group_offsets, groups), all))
       return kInvalidMatrixC;
     cudaStream_t s;
     const int r = begin_call(stream, async, &s);

@@ -157,8 +157,9 @@ int b200blas_col2im(int dtype, int kernel_mode, size_t channels, size_t height, 
  *     form, 165 silu. act' below is its derivative.
  *   - optional buffers are absent when NULL; D is not read when beta == 0, Z is not read when the activation is the
  *     identity. D may be C itself, and so may a Z that is read; DZ may be DY or Z. Otherwise what is written may not
- *     meet anything that the call reads or writes (kInvalidMatrixC, for a bias gradient kInvalidVectorY), except as
- *     other columns of the same lines. B of the Newton-Schulz products may overlap A.
+ *     meet anything that the call reads or writes, group offsets included (kInvalidMatrixC, for a bias gradient
+ *     kInvalidVectorY), except as other columns of the same lines; weights, biases and offsets of groups may not lie
+ *     between those lines either. B of the Newton-Schulz products may overlap A.
  *   - Z and D have C's extents and are reported with C's status codes; a bad bias is kInvalidVectorX (-1019) or
  *     kInsufficientMemoryX (-1008), a bad bias gradient kInvalidVectorY (-1018) or kInsufficientMemoryY (-1007).
  *     Extents above 2^31 - 4097 are kInvalidDimension. Buffers that do not lie on the current device are invalid.

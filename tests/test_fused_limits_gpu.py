@@ -77,3 +77,55 @@ def test_few_multiprocessors(cuda, monkeypatch, budget):
             weight(cuda, monkeypatch, v, "half", "single", [3, 0, 64, 33, 0, 1, 129], 240, 136, 264, beta=1.0)
     finally:
         cb.set_sm_budget(0)
+
+
+def test_results_that_meet_the_group_offsets_are_refused(cuda):
+    """Nothing is launched, and nothing written; right beside them is allowed."""
+    torch = cuda
+    S = cb.StatusCode
+    rows, n, k, G = 64, 24, 16, 3
+    table = torch.tensor([0, 10, 10, rows], dtype=torch.int64, device="cuda")
+    space = torch.zeros(4096, dtype=torch.int64, device="cuda")
+    half = space.view(torch.float16)  # the same memory
+    x, w, z = (torch.ones(s, device="cuda", dtype=torch.float16) for s in ((rows, k), (G, n, k), (rows, n)))
+    y, stream = torch.ones(rows, n, device="cuda", dtype=torch.float16), torch.cuda.current_stream()
+
+    def grouped_(off, c, c_off=0, zz=None, z_off=0):
+        return cb.GemmGrouped(YES, G, rows, n, k, 1.0, x, 0, k, w, 0, k, n * k, off, None, 0, n, 161, zz, z_off, n, 0.0, None, 0, n, c, c_off, n,
+                              stream=stream)
+
+    def gradient(off, c, c_off=0, sums=None, s_off=0):
+        return cb.GemmGroupedGrad(YES, G, rows, n, k, 1.0, x, 0, k, w, 0, k, n * k, off, 0.0, None, 0, n, 165, z, 0, n, c, c_off, n, sums, s_off, n,
+                                  stream=stream)
+
+    def weight_(off, c, c_off=0):
+        return cb.GemmGroupedWeight(G, rows, k, n, 1.0, x, 0, k, y, 0, n, off, 0.0, c, c_off, n, k * n, stream=stream)
+
+    def activation(off, c, c_off=0, sums=None, s_off=0):
+        return cb.ActivationGrad(rows, n, 165, y, 0, n, z, 0, n, c, c_off, n, sums, s_off, groups=G, group_offsets=off, bias_grad_ld=n,
+                                 stream=stream)
+
+    c = torch.zeros(rows, n, device="cuda", dtype=torch.float16)
+    at = 2048  # where the offsets lie, counted in halves
+    space[at // 4:at // 4 + G + 1] = table
+    before, off = space.clone(), space[at // 4:at // 4 + G + 1]
+    for c_off in (at - rows * n + 1, at, at + 4 * (G + 1) - 1):
+        assert grouped_(off, half, c_off) == S.kInvalidMatrixC
+        assert grouped_(off, c, 0, half, c_off) == S.kInvalidMatrixC
+        assert gradient(off, half, c_off) == S.kInvalidMatrixC
+        assert activation(off, half, c_off) == S.kInvalidMatrixC
+    for s_off in (at - G * n + 1, at, at + 4 * (G + 1) - 1):
+        assert gradient(off, c, 0, half, s_off) == S.kInvalidVectorY
+        assert activation(off, c, 0, half, s_off) == S.kInvalidVectorY
+        assert activation(off, None, 0, half, s_off) == S.kInvalidVectorY
+    for c_off in (at - G * k * n + 1, at, at + 4 * (G + 1) - 1):
+        assert weight_(off, half, c_off) == S.kInvalidMatrixC
+    torch.cuda.synchronize()
+    assert torch.equal(space, before)
+    for c_off in (at - rows * n, at + 4 * (G + 1)):
+        assert grouped_(off, half, c_off) == S.kSuccess
+        assert gradient(off, c, 0, half, c_off) == S.kSuccess
+        torch.cuda.synchronize()
+        assert torch.equal(off, table)
+    code, where = cb.tensor_core_status()
+    assert code == S.kSuccess, where
