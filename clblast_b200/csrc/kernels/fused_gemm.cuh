@@ -57,6 +57,7 @@ using namespace tc;
 
 constexpr int BM = 128;   // rows of op(A) per CTA
 constexpr int ROW_K = 64; // inner elements of a 128-byte swizzle row
+constexpr int CB = 16;    // columns per epilogue block
 // inner elements per accumulator: results in single precision; sums of two halves, whose users (the Newton-Schulz steps)
 // amplify an error that all entries share
 constexpr int kChunkSingle = 256, kChunkParts = 128;
@@ -75,41 +76,34 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A block of 32 rows x COLS (16 or 32) columns of a 16-bit matrix between memory and the lanes. In memory order lane l has
-// the rows 8 (l % 4) .. + 7 of the columns 2 (l / 4) and 2 (l / 4) + 1 of each 16; in row order it has row l of all
-// columns. Between the two the block lies in shared memory as [column pair][row] words of two columns.
-template <class E, int COLS>
+// A block of 32 rows x CB columns of a 16-bit matrix between memory and the lanes. In memory order lane l has the rows
+// 8 (l % 4) .. + 7 of the columns 2 (l / 4) and 2 (l / 4) + 1; in row order it has row l of all columns. Between the two the
+// block lies in shared memory as [column pair][row] words of two columns.
+template <class E>
 struct Block16 {
-  static constexpr int HALVES = COLS / 16;
-  static constexpr int WORDS = COLS * 16;  // shared memory
-  uint4 v[2 * HALVES];
+  static constexpr int WORDS = CB * 16;  // shared memory
+  uint4 v[2];
 
   // base: the block's first element; rows_left (a multiple of 8) and cols_left: how many of its rows and columns exist.
   __device__ __forceinline__ void load(const E* base, long long ld, int rows_left, int cols_left, int lane) {
     const int c0 = 2 * (lane >> 2), r0 = 8 * (lane & 3);
     const bool in = r0 < rows_left;
-    const E* at = base + static_cast<long long>(c0) * ld + r0;
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h, at += 16 * ld) {
-      v[2 * h] = v[2 * h + 1] = make_uint4(0, 0, 0, 0);
-      if (in && c0 + 16 * h < cols_left) v[2 * h] = *reinterpret_cast<const uint4*>(at);
-      if (in && c0 + 16 * h + 1 < cols_left) v[2 * h + 1] = *reinterpret_cast<const uint4*>(at + ld);
-    }
+    const E* const at = base + static_cast<long long>(c0) * ld + r0;
+    v[0] = v[1] = make_uint4(0, 0, 0, 0);
+    if (in && c0 < cols_left) v[0] = *reinterpret_cast<const uint4*>(at);
+    if (in && c0 + 1 < cols_left) v[1] = *reinterpret_cast<const uint4*>(at + ld);
   }
   // memory order -> row order: f[j] is column j of this lane's row. The buffer is free before and after.
-  __device__ __forceinline__ void to_rows(uint32_t* smem, float (&f)[COLS], int lane) const {
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h) {
-      const uint4 a = v[2 * h], b = v[2 * h + 1];
-      uint4* const at = reinterpret_cast<uint4*>(smem + h * 256 + (lane >> 2) * 32 + (lane & 3) * 8);
-      at[0] = make_uint4(__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
-                         __byte_perm(a.y, b.y, 0x7632));
-      at[1] = make_uint4(__byte_perm(a.z, b.z, 0x5410), __byte_perm(a.z, b.z, 0x7632), __byte_perm(a.w, b.w, 0x5410),
-                         __byte_perm(a.w, b.w, 0x7632));
-    }
+  __device__ __forceinline__ void to_rows(uint32_t* smem, float (&f)[CB], int lane) const {
+    const uint4 a = v[0], b = v[1];
+    uint4* const at = reinterpret_cast<uint4*>(smem + (lane >> 2) * 32 + (lane & 3) * 8);
+    at[0] = make_uint4(__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
+                       __byte_perm(a.y, b.y, 0x7632));
+    at[1] = make_uint4(__byte_perm(a.z, b.z, 0x5410), __byte_perm(a.z, b.z, 0x7632), __byte_perm(a.w, b.w, 0x5410),
+                       __byte_perm(a.w, b.w, 0x7632));
     __syncwarp();
 #pragma unroll
-    for (int q = 0; q < COLS / 2; ++q) {
+    for (int q = 0; q < CB / 2; ++q) {
       const uint32_t w = smem[q * 32 + lane];
       const unsigned short lo = static_cast<unsigned short>(w), hi = static_cast<unsigned short>(w >> 16);
       f[2 * q] = to_float(*reinterpret_cast<const E*>(&lo));
@@ -119,70 +113,66 @@ struct Block16 {
   }
   // row order -> memory
   static __device__ __forceinline__ void store(E* base, long long ld, int rows_left, int cols_left, uint32_t* smem,
-                                               const float (&f)[COLS], int lane) {
+                                               const float (&f)[CB], int lane) {
 #pragma unroll
-    for (int q = 0; q < COLS / 2; ++q) smem[q * 32 + lane] = pack2<E>(f[2 * q], f[2 * q + 1]);
+    for (int q = 0; q < CB / 2; ++q) smem[q * 32 + lane] = pack2<E>(f[2 * q], f[2 * q + 1]);
     __syncwarp();
     const int c0 = 2 * (lane >> 2), r0 = 8 * (lane & 3);
     const bool in = r0 < rows_left;
-    E* at = base + static_cast<long long>(c0) * ld + r0;
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h, at += 16 * ld) {
-      const uint4* const from = reinterpret_cast<const uint4*>(smem + h * 256 + (lane >> 2) * 32 + r0);
-      const uint4 w0 = from[0], w1 = from[1];
-      if (in && c0 + 16 * h < cols_left)
-        *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(w0.x, w0.y, 0x5410), __byte_perm(w0.z, w0.w, 0x5410),
-                                                   __byte_perm(w1.x, w1.y, 0x5410), __byte_perm(w1.z, w1.w, 0x5410));
-      if (in && c0 + 16 * h + 1 < cols_left)
-        *reinterpret_cast<uint4*>(at + ld) = make_uint4(__byte_perm(w0.x, w0.y, 0x7632), __byte_perm(w0.z, w0.w, 0x7632),
-                                                        __byte_perm(w1.x, w1.y, 0x7632), __byte_perm(w1.z, w1.w, 0x7632));
-    }
+    E* const at = base + static_cast<long long>(c0) * ld + r0;
+    const uint4* const from = reinterpret_cast<const uint4*>(smem + (lane >> 2) * 32 + r0);
+    const uint4 w0 = from[0], w1 = from[1];
+    if (in && c0 < cols_left)
+      *reinterpret_cast<uint4*>(at) = make_uint4(__byte_perm(w0.x, w0.y, 0x5410), __byte_perm(w0.z, w0.w, 0x5410),
+                                                 __byte_perm(w1.x, w1.y, 0x5410), __byte_perm(w1.z, w1.w, 0x5410));
+    if (in && c0 + 1 < cols_left)
+      *reinterpret_cast<uint4*>(at + ld) = make_uint4(__byte_perm(w0.x, w0.y, 0x7632), __byte_perm(w0.z, w0.w, 0x7632),
+                                                      __byte_perm(w1.x, w1.y, 0x7632), __byte_perm(w1.z, w1.w, 0x7632));
     __syncwarp();
   }
 };
 
 // The same for single precision: in memory order lane l has the rows 4 (l % 8) .. + 3 of the columns l / 8 + 4 h.
-template <int COLS>
 struct Block32 {
-  static constexpr int WORDS = COLS * 32;
-  uint4 v[COLS / 4];
+  static constexpr int WORDS = CB * 32;
+  uint4 v[CB / 4];
 
   __device__ __forceinline__ void load(const float* base, long long ld, int rows_left, int cols_left, int lane) {
     const int r0 = 4 * (lane & 7), c0 = lane >> 3;
     const float* at = base + static_cast<long long>(c0) * ld + r0;
 #pragma unroll
-    for (int h = 0; h < COLS / 4; ++h, at += 4 * ld) {
+    for (int h = 0; h < CB / 4; ++h, at += 4 * ld) {
       v[h] = make_uint4(0, 0, 0, 0);
       if (r0 < rows_left && c0 + 4 * h < cols_left) v[h] = *reinterpret_cast<const uint4*>(at);
     }
   }
-  __device__ __forceinline__ void to_rows(uint32_t* smem, float (&f)[COLS], int lane) const {
+  __device__ __forceinline__ void to_rows(uint32_t* smem, float (&f)[CB], int lane) const {
 #pragma unroll
-    for (int h = 0; h < COLS / 4; ++h) *reinterpret_cast<uint4*>(smem + ((lane >> 3) + 4 * h) * 32 + 4 * (lane & 7)) = v[h];
+    for (int h = 0; h < CB / 4; ++h) *reinterpret_cast<uint4*>(smem + ((lane >> 3) + 4 * h) * 32 + 4 * (lane & 7)) = v[h];
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < COLS; ++j) f[j] = __uint_as_float(smem[j * 32 + lane]);
+    for (int j = 0; j < CB; ++j) f[j] = __uint_as_float(smem[j * 32 + lane]);
     __syncwarp();
   }
   static __device__ __forceinline__ void store(float* base, long long ld, int rows_left, int cols_left, uint32_t* smem,
-                                               const float (&f)[COLS], int lane) {
+                                               const float (&f)[CB], int lane) {
 #pragma unroll
-    for (int j = 0; j < COLS; ++j) smem[j * 32 + lane] = __float_as_uint(f[j]);
+    for (int j = 0; j < CB; ++j) smem[j * 32 + lane] = __float_as_uint(f[j]);
     __syncwarp();
     const int r0 = 4 * (lane & 7), c0 = lane >> 3;
     float* at = base + static_cast<long long>(c0) * ld + r0;
 #pragma unroll
-    for (int h = 0; h < COLS / 4; ++h, at += 4 * ld) {
+    for (int h = 0; h < CB / 4; ++h, at += 4 * ld) {
       const uint4 w = *reinterpret_cast<const uint4*>(smem + (c0 + 4 * h) * 32 + r0);
       if (r0 < rows_left && c0 + 4 * h < cols_left) *reinterpret_cast<uint4*>(at) = w;
     }
     __syncwarp();
   }
 };
-template <class E, int COLS>
-struct BlockOf { using type = Block16<E, COLS>; };
-template <int COLS>
-struct BlockOf<float, COLS> { using type = Block32<COLS>; };
+template <class E>
+struct BlockOf { using type = Block16<E>; };
+template <>
+struct BlockOf<float> { using type = Block32; };
 
 // Starts the load of 16 accumulator columns; the values may be used after tmem_wait.
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
@@ -385,7 +375,6 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   constexpr bool CHUNKED = sizeof(OT) == 4 || MODE == kModeParts;  // sums beyond what the accumulators give
   constexpr int CHUNK = (MODE == kModeParts ? kChunkParts : kChunkSingle) / (ROW_K * fused_stage_rows(CTAS, BN));  // stages
   constexpr int EG = fused_groups(BN);
-  constexpr int CB = 16;  // columns per epilogue block
   constexpr int B_ROWS = BN / CTAS;
   constexpr int SUBS = fused_stage_rows(CTAS, BN);  // a stage holds SUBS blocks of 64 inner elements, one after the other
   constexpr int BK = ROW_K * SUBS;
@@ -466,7 +455,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
 
   // Loads of one inner block into a stage of the ring, by one lane.
-  auto issue_block = [&](const Tile& t, int kb, int stage, uint64_t pol_a, uint64_t pol_b) {
+  auto issue_block = [&](const Tile& t, int kb, int stage, uint64_t policy) {
     const int a_row0 = (t.tm * CTAS + (CTAS == 2 ? static_cast<int>(rank) : 0)) * BM;
     const int b_row0 = t.col0 + (CTAS == 2 ? static_cast<int>(rank) * B_ROWS : 0);
     int az = p.a_batched ? t.z : 0, bz = p.b_batched ? t.z : 0;
@@ -494,9 +483,9 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       bar = full_bar(stage);
       mbar_arrive_expect_tx(bar, STAGE_BYTES);
     }
-    auto load = [&](uint32_t dst, const CUtensorMap* map, int cx, int cy, int cz, uint64_t pol) {
-      if constexpr (CTAS == 2) tma_load_3d_pair_hint(dst, map, bar, cx, cy, cz, pol);
-      else tma_load_3d_hint(dst, map, bar, cx, cy, cz, pol);
+    auto load = [&](uint32_t dst, const CUtensorMap* map, int cx, int cy, int cz) {
+      if constexpr (CTAS == 2) tma_load_3d_pair_hint(dst, map, bar, cx, cy, cz, policy);
+      else tma_load_3d_hint(dst, map, bar, cx, cy, cz, policy);
     };
 #pragma unroll
     for (int sub = 0; sub < SUBS; ++sub) {
@@ -505,15 +494,15 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       const int x = t.k0 + kb * BK + sub * ROW_K;
       if (p.a_mn) {
 #pragma unroll
-        for (int j = 0; j < BM / 64; ++j) load(a_dst + j * 8192, &map_a, a_row0 + j * 64, x, az, pol_a);
+        for (int j = 0; j < BM / 64; ++j) load(a_dst + j * 8192, &map_a, a_row0 + j * 64, x, az);
       } else {
-        load(a_dst, &map_a, x, a_row0, az, pol_a);
+        load(a_dst, &map_a, x, a_row0, az);
       }
       if (p.b_mn) {
 #pragma unroll
-        for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * 8192, &map_b, b_row0 + j * 64, x, bz, pol_b);
+        for (int j = 0; j < B_ROWS / 64; ++j) load(b_dst + j * 8192, &map_b, b_row0 + j * 64, x, bz);
       } else {
-        load(b_dst, &map_b, x, b_row0, bz, pol_b);
+        load(b_dst, &map_b, x, b_row0, bz);
       }
     }
   };
@@ -546,7 +535,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      const uint64_t pol_a = l2_policy(p.hint_a), pol_b = l2_policy(p.hint_b);
+      const uint64_t policy = l2_policy(2);  // operands stay in L2: other tiles read them too
       const int last_tile = uniform(num_tiles);
       for (int tile = first_tile; tile < last_tile && ok; tile += tile_step) {
         Tile t = locate<BN>(p, tile, start, tiles);
@@ -560,7 +549,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = loop_wait(empty_bar(stage), phase ^ 1u, abort_flag, 1u, p.status);
           if (!ok) break;
-          if (elect_one()) issue_block(t, kb, stage, pol_a, pol_b);
+          if (elect_one()) issue_block(t, kb, stage, policy);
           __syncwarp();
           if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
@@ -709,9 +698,9 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
   } else if (warp >= 4) {
     // ---- epilogue ----
-    using BlockC = typename BlockOf<OT, CB>::type;
-    using BlockD = typename BlockOf<DT, CB>::type;
-    using BlockZ = Block16<T, CB>;
+    using BlockC = typename BlockOf<OT>::type;
+    using BlockD = typename BlockOf<DT>::type;
+    using BlockZ = Block16<T>;
     constexpr int BLOCKS = GROUP_COLS / CB;
     const int group = (warp - 4) >> 2;
     const int quad = warp & 3;  // tensor-memory lanes this warp may read
@@ -1178,7 +1167,7 @@ cudaError_t launch_mode(const CUtensorMap* maps, const FusedParams& p, int grid,
 
 template <int CTAS, int BN, class T, class DT, class OT>
 cudaError_t launch_typed(const CUtensorMap* maps, const FusedParams& p, int grid, int smem, cudaStream_t stream) {
-  if constexpr ((BN == 256 && CTAS == 2) || (BN == 128 && CTAS == 1)) {
+  if constexpr (BN == 128 && CTAS == 1) {
     if constexpr (std::is_same<T, __half>::value && std::is_same<OT, __half>::value) {
       if (p.parts) return launch_mode<CTAS, BN, T, DT, OT, kModeParts>(maps, p, grid, smem, stream);
     }

@@ -47,7 +47,6 @@ struct FusedParams {
   int vec;                    // C, D and Z: bases, leading dimensions and strides are multiples of 16 bytes
   int prefetch;               // D and Z have tensor maps and are asked for ahead
   float* partial;             // row sums of C per column tile (bias gradient), or null
-  int hint_a, hint_b;
 };
 
 #ifdef __CUDACC__

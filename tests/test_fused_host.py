@@ -107,3 +107,13 @@ def test_limit_on_multiprocessors(selection):
         assert row[5] <= c[-1] or row[1] == -1, (c, row)
     for form in ("0", "4,8"):  # asked for by name and too large
         assert all(row[5] <= c[-1] or row[1] == -1 for c, row in zip(calls, launched(selection, calls, form)))
+
+
+def test_sums_of_two_halves_have_one_kernel(selection):
+    sides = [(8, 8), (128, 304), (512, 1000), (4096, 4096), (1000, 70000)]  # padded to eights, as the iteration keeps them
+    calls = []
+    for side, long in sides:
+        calls += [call(PLAIN, 3, side, side, long, type=HALF, tri=1, parts=1), call(PLAIN, 3, side, side, side, type=HALF, beta=1.0, tri=1, parts=1),
+                  call(PLAIN, 3, side, long, side, type=HALF, beta=1.0, parts=1), call(PLAIN, 3, long, side, side, type=HALF, beta=1.0, a_mn=1, parts=1)]
+    for form in (None, *FORMS):
+        assert all(row[1:3] == (2, 1) for row in launched(selection, calls, form))
