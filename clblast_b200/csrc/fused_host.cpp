@@ -193,7 +193,7 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   const long long a_planes = d.kind == kFusedRaggedInner || d.a_stride == 0 ? 1 : d.problems * per_problem;
   const long long b_planes = d.kind == kFusedPlain && d.b_stride != 0 ? d.problems * per_problem : 1;
   // Operands that TMA cannot address are copied once to an aligned pitch.
-  PoolScratch copies, partial;
+  PoolScratch copies, partial, sums;
   FusedDesc r = d;
   PackJob jobs[2] = {};
   const auto plan = [&](PackJob& job, const void* base, long long ld, long long stride, bool mn, long long rows,
@@ -298,6 +298,14 @@ cudaError_t launch_fused(const FusedDesc& d, cudaStream_t stream, const char** n
   const int team = t.ctas * choice.split;
   long long teams = resident_teams(team);
   if (tiles < teams) teams = tiles;
+  if (d.c_type != 32 && !d.parts) {
+    const long long stage_k = 64LL * fused_stage_rows(t.ctas, t.bn), in_all = (d.k + stage_k - 1) / stage_k;
+    if ((in_all + choice.split - 1) / choice.split > kChunkHalf / stage_k) {
+      e = sums.get(static_cast<size_t>(teams) * team * 128 * t.bn * sizeof(float), stream);
+      if (e != cudaSuccess) return e;
+      p.sums = reinterpret_cast<float*>(sums.ptr());
+    }
+  }
   e = launch_fused_variant(choice.variant, d.type, d.d_type, d.c_type, maps, p, static_cast<int>(teams) * team, smem, stream);
   static thread_local char label[64];
   if (choice.split > 1) std::snprintf(label, sizeof(label), "%s_split%d", kNames[choice.variant], choice.split);

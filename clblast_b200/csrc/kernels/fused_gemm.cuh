@@ -23,11 +23,14 @@
 // per block, the form of the half-precision GEMM kernels, took 115 us for 8192 x 8192 x 512 and could not cut a group's
 // columns.)
 //
-// Sums for results in single precision: the tensor cores cut off instead of rounding when they add to an accumulator, an
-// error of about 4e-8 of the result per 16 inner elements that all points towards zero. Results in 16 bits do not see it.
-// For the others an accumulator takes a few blocks at most and is then added, rounded, to sums in further columns of
-// tensor memory (which the widest tile has room for only with one accumulator instead of two). The same sums in registers
-// spill: 286 us against 247 for 32 weight gradients of 512 rows, 2048 x 2048 each, on 128 x 128 tiles.
+// Sums: the tensor cores cut off instead of rounding when they add to an accumulator, an error that all points towards zero
+// and grows to 1e-7 of the result per 16 inner elements where all products have one sign. For results in single precision
+// an accumulator therefore takes a few blocks at most and is then added, rounded, to sums in further columns of tensor
+// memory (which the widest tile has room for only with one accumulator instead of two). The same sums in registers spill:
+// 286 us against 247 for 32 weight gradients of 512 rows, 2048 x 2048 each, on 128 x 128 tiles. Results in 16 bits see the
+// error beyond some ten thousand inner elements (half, 131072 products of one sign: 2.6 half steps of rounding, a million:
+// 13): from kChunkHalf on an accumulator is handed over and the sums wait in global memory, one tile's per CTA (2048 x 2048
+// x 65536 in half 394 -> 410 to 418 us, 4096 x 4096 x 32768 in bfloat16 1193 -> 1194 to 1222; shorter extents as before).
 //
 // What bounds it: products of 10^11 operations and more the board's power (8192 x 8192 x 2048 in bfloat16 with bias, gelu
 // and Z kept 207 us, 1.33 PFLOP/s, tensor pipe busy 77 % of the cycles; a plain library product sustains 1.40); weight
@@ -61,6 +64,7 @@ constexpr int CB = 16;    // columns per epilogue block
 // inner elements per accumulator: results in single precision; sums of two halves, whose users (the Newton-Schulz steps)
 // amplify an error that all entries share
 constexpr int kChunkSingle = 256, kChunkParts = 128;
+static_assert(kChunkHalf % 128 == 0, "whole stages");
 
 // Two values rounded to 16 bits in one word (the packed conversion runs on the full-rate pipe, the single one does not).
 template <class E>
@@ -395,6 +399,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   const bool aux = p.z != nullptr;
   const int stages = p.stages;
   const int split = (CTAS == 1 && MODE == kModeGeneral) ? p.split : 1;
+  const int chunk = CHUNKED ? CHUNK : (p.sums != nullptr ? kChunkHalf / BK : 0x7FFFFFFF);  // stages per accumulator
   uint8_t* const staging = base_ptr + stages * STAGE_BYTES;
   uint8_t* const behind = staging + fused_staging_bytes(BN, CHUNKED, aux, split);
   const uint32_t bar_base = smem_u32(behind);
@@ -627,7 +632,7 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         uint32_t d_tmem = tmem + static_cast<uint32_t>(acc * BN);
         int first_kb = kb0;  // first block of the current accumulator
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (CHUNKED && kb - first_kb == CHUNK) {  // hand this accumulator over and go on in the other one
+          if (kb - first_kb == chunk) {  // hand this accumulator over and go on in the other one
             if (elect_one()) commit(acc_full_bar(acc));
             __syncwarp();
             ++local;
@@ -786,6 +791,38 @@ fused_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           }
           release_accumulator(local);
           ++local;
+        }
+        if (!ok) break;
+      } else if (kb1 - kb0 > chunk) {
+        // A long inner extent in 16 bits: all accumulators but the last are added up in global memory, where a thread meets
+        // only what it has written itself; the last takes them in and is used like the only one of a short extent.
+        float* const sums = p.sums + (static_cast<long long>(blockIdx.x) * BN + group * GROUP_COLS) * BM + row_in_cta;
+        const int chunks = (kb1 - kb0 + chunk - 1) / chunk;
+        for (int c = 0; c < chunks; ++c) {
+          ok = wait_accumulator(local);
+          if (!ok) break;
+          tcgen05_fence_after();
+          const bool last = c == chunks - 1;
+#pragma unroll 1
+          for (int cb = 0; cb < BLOCKS; ++cb) {
+            uint32_t r[CB];
+            tmem_ld(accumulator(local) + cb * CB, r);
+            tmem_wait(r);
+            float* const at = sums + cb * CB * BM;
+#pragma unroll
+            for (int j = 0; j < CB; ++j) {
+              const float sum = c > 0 ? at[j * BM] + __uint_as_float(r[j]) : __uint_as_float(r[j]);
+              if (last) r[j] = __float_as_uint(sum);
+              else at[j * BM] = sum;
+            }
+            if (last) tmem_st(accumulator(local) + cb * CB, r);
+          }
+          if (last) {
+            tmem_st_wait();
+          } else {
+            release_accumulator(local);
+            ++local;
+          }
         }
         if (!ok) break;
       }

@@ -19,6 +19,10 @@ enum FusedKind : int {
 // Most groups of a call: the table of the groups' tiles lives in shared memory.
 constexpr int kFusedMaxGroups = 1024;
 
+// Inner elements per accumulator of results in 16 bits. What the tensor cores cut off below it is a fifth of half's rounding
+// at most, of bfloat16's a fortieth.
+constexpr int kChunkHalf = 16384;
+
 // Kernel arguments. C is m x n with m contiguous: rows are the features of a caller's contiguous vectors, columns the
 // vectors (tokens).
 struct FusedParams {
@@ -47,6 +51,7 @@ struct FusedParams {
   int vec;                    // C, D and Z: bases, leading dimensions and strides are multiples of 16 bytes
   int prefetch;               // D and Z have tensor maps and are asked for ahead
   float* partial;             // row sums of C per column tile (bias gradient), or null
+  float* sums;                // one tile per CTA, where a result in 16 bits has more than kChunkHalf inner elements; or null
 };
 
 #ifdef __CUDACC__
