@@ -48,8 +48,9 @@ struct Choice {
   int variant, split;
 };
 
-constexpr const char* kNames[kFusedVariants] = {"fused_pair_256x256x64", "fused_128x256x64", "fused_128x128x64",
-                                                "fused_128x64x64", "fused_128x32x64", "fused_pair_256x128x64"};
+// Rows and columns of a tile; a stage's inner elements are fused_stage_rows() swizzle rows of 64.
+constexpr const char* kNames[kFusedVariants] = {"fused_pair_256x256", "fused_128x256", "fused_128x128",
+                                                "fused_128x64", "fused_128x32", "fused_pair_256x128"};
 
 // Upper bound of the column tiles of a call (exact for the plain kinds).
 long long column_tiles(const FusedDesc& d, int bn) {

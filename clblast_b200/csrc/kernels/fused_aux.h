@@ -55,7 +55,8 @@ cudaError_t launch_sum_partials(const SumJob& job, cudaStream_t stream);
 
 // Newton-Schulz input: X = scale * G / (|G|_F + eps) for `batch` matrices (lines of `one` contiguous elements, `two`
 // lines), X dense with `lines` lines of `pitch` elements (what G does not have is zero), planes lines * pitch apart, in half (x_type 16) or single
-// (32) precision, or (x_type kParts) as a sum of two halves in consecutive planes. `sums` is scratch of norm_scratch_doubles(batch) doubles.
+// (32) precision, or (x_type kParts) as a sum of two halves in consecutive planes. `sums` is scratch of batch * kNormBlocks
+// doubles.
 constexpr int kNormBlocks = 256;  // blocks per matrix
 constexpr int kParts = 1616;
 struct NormaliseJob {

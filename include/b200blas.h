@@ -154,8 +154,8 @@ int b200blas_col2im(int dtype, int kernel_mode, size_t channels, size_t height, 
  *     return kNotImplemented.
  *   - scalars are passed by value in double precision. Sums run in fp32; a stored value is rounded once. The tensor cores
  *     cut off when they add to an accumulator, so one takes 16384 inner elements at most (256 for results in single
- *     precision) and the accumulators are added rounded: up to a fifth of a rounding in half where all products of a sum
- *     have one sign, whatever the inner extent.
+ *     precision) and the accumulators are added rounded. Where all products of a sum have one sign that leaves 1e-4 of it
+ *     (a fifth of half's rounding) or 1e-6 (single), whatever the inner extent.
  *   - `activation`: 161 identity, 162 relu, 163 gelu (z times the normal distribution function), 164 gelu in its tanh
  *     form, 165 silu. act' below is its derivative.
  *   - optional buffers are absent when NULL; D is not read when beta == 0, Z is not read when the activation is the
