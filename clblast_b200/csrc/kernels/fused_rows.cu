@@ -13,6 +13,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "../runtime_state.h"
 #include "activation.cuh"
 #include "fused_gemm.h"
 
@@ -138,7 +139,7 @@ cudaError_t launch_parts(const FewRowsJob& job, cudaStream_t stream) {
 template <class T, class OT, int ROWS>
 cudaError_t launch_rows(const FewRowsJob& job, cudaStream_t stream) {
   // enough warps to keep every SM's memory pipeline full, each with at least one round of deep loads
-  const long long wanted = 148LL * 24;
+  const long long wanted = 24LL * sm_count();
   const int round = 32 * kDeep * 16 / static_cast<int>(sizeof(T));  // elements of one
   if (job.m >= wanted || job.k < 2 * round) return launch_parts<T, OT, ROWS, 1>(job, stream);
   if (2LL * job.m >= wanted || job.k < 4 * round) return launch_parts<T, OT, ROWS, 2>(job, stream);

@@ -18,6 +18,7 @@
 
 #include <cstdint>
 
+#include "../runtime_state.h"
 #include "activation.cuh"
 
 namespace b200 {
@@ -232,7 +233,7 @@ template <class S>
 int split_of(long long m, long long n, long long k) {
   const long long tiles = ceil_div(m, S::BM) * ceil_div(n, S::BN);
   int split = 1;
-  while (split < kMaxSplit && tiles * split < 2 * 148 && k / (2 * split) >= 128) split *= 2;
+  while (split < kMaxSplit && tiles * split < 2 * sm_count() && k / (2 * split) >= 128) split *= 2;
   return split;
 }
 
@@ -293,7 +294,7 @@ cudaError_t launch_single(const SingleJob& job, cudaStream_t stream) {
   // against 12.8).
   const auto covered = [&](long long bm, long long bn) { return static_cast<double>(ceil_div(job.m, bm) * bm) * (ceil_div(job.n, bn) * bn); };
   const long long wide_blocks = ceil_div(job.m, Wide::BM) * ceil_div(job.n, Wide::BN) * split_of<Wide>(job.m, job.n, job.k);
-  if (wide_blocks >= 148 && 0.8 * covered(Wide::BM, Wide::BN) < covered(Slim::BM, Slim::BN)) return launch_shape<Wide>(job, stream);
+  if (wide_blocks >= sm_count() && 0.8 * covered(Wide::BM, Wide::BN) < covered(Slim::BM, Slim::BN)) return launch_shape<Wide>(job, stream);
   return launch_shape<Slim>(job, stream);
 }
 
