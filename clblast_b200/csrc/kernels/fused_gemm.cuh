@@ -32,11 +32,14 @@
 // 13): from kChunkHalf on an accumulator is handed over and the sums wait in global memory, one tile's per CTA (2048 x 2048
 // x 65536 in half 394 -> 410 to 418 us, 4096 x 4096 x 32768 in bfloat16 1193 -> 1194 to 1222; shorter extents as before).
 //
-// What bounds it: products of 10^11 operations and more the board's power (8192 x 8192 x 2048 in bfloat16 with bias, gelu
-// and Z kept 207 us, 1.33 PFLOP/s, tensor pipe busy 77 % of the cycles; a plain library product sustains 1.40); weight
-// gradients in single precision the writes, which nothing hides while an accumulator is being emptied (236 us, 2.8 TB/s);
-// decoding the reads of the weights (48 x 4096 x 8192 16.5 us, 4.1 TB/s, of which 5 us are the start and the meeting of
-// the split tiles).
+// What bounds it: products of 10^11 operations and more first the tensor pipe and, run for seconds, the board's power. 8192 x
+// 8192 x 2048 in bfloat16 with bias, gelu and Z kept takes 208 us in a short run at full clock (1.32 PFLOP/s, tensor pipe
+// busy 77 % of the cycles). Back to back at the power limit it takes 248, where a library product without any epilogue takes
+// 210 and this one without any 218: the epilogue's work and its 268 MB of stores draw on the same power. Groups of rows: their last tiles
+// run over the full width (256 columns round 16384 rows of 32 experts up to 1.2 times as many). Weight gradients in single
+// precision: the MMAs wait while the one accumulator of 256 columns is being emptied (244 us for 32 of 2048 x 2048, 2.8 TB/s).
+// Decoding: the reads of the weights (48 x 4096 x 8192 20.5 us with the weights in memory, 3.4 TB/s; 16.4 with them in L2),
+// of which 5 us are the start and the meeting of the split tiles.
 //
 // All waits are bounded; on expiry a code is left in the status word and every role leaves its loop.
 #pragma once
