@@ -168,9 +168,9 @@ int b200blas_col2im(int dtype, int kernel_mode, size_t channels, size_t height, 
  *     Extents above 2^31 - 4097 are kInvalidDimension. Buffers that do not lie on the current device are invalid.
  *   - any alignment, leading dimension and offset is served. Operands whose base, leading dimension or stride is not a
  *     multiple of 16 bytes are first copied to scratch; outputs that are not are written with narrow stores.
- *   - scratch (those copies, partial bias gradients, Newton-Schulz intermediates) comes from a stream-ordered pool of
- *     the library that keeps up to 1 GB per device until b200blas_clear_cache; a captured call owns its scratch through
- *     its graph. Results do not depend on timing: no atomics are used. */
+ *   - scratch (those copies, partial bias gradients, sums of inner extents above 16384, Newton-Schulz intermediates) comes
+ *     from a stream-ordered pool of the library that keeps up to 1 GB per device until b200blas_clear_cache; a captured
+ *     call owns its scratch through its graph. Results do not depend on timing: no atomics are used. */
 #define B200BLAS_BFLOAT16 1016
 #define B200BLAS_MAX_GROUPS 1024
 
