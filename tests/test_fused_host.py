@@ -49,7 +49,7 @@ def launched(exe, calls, form=None):
 
 def test_many_groups_find_a_kernel(selection):
     """Groups take shared memory from the operand ring: 128 x 256 tiles with a split have room for 191 of them."""
-    launched(selection, [call(COLS, 192, 16, 30720, 4096), call(COLS, 200, 16, 38400, 4096), call(COLS, 200, 384, 40000, 4096),
+    launched(selection, [call(COLS, 192, 16, 30912, 4096), call(COLS, 200, 16, 38400, 4096), call(COLS, 200, 384, 40000, 4096),
                          call(COLS, 256, 384, 131072, 7168)])
     for form, groups in itertools.product(FORMS, (1, 191, 192, 1024)):
         rows = launched(selection, [call(COLS, groups, 384, 40000, 4096, z=1), call(COLS, groups, 384, 40000, 4096, c_type=SINGLE, z=1, beta=1.0),

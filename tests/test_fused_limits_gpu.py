@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 
 def test_groups_beside_the_sums_of_split_tiles(cuda, monkeypatch):
     """192 groups and more leave 128 x 256 tiles with a split no room for two ring stages: other tiles serve the call."""
-    grouped(cuda, monkeypatch, None, "bf16", "bf16", [160] * 192, 30720, 16, 4096)  # takes 128 x 256 tiles with fewer groups
+    grouped(cuda, monkeypatch, None, "bf16", "bf16", [161] * 192, 30912, 16, 4096)  # takes 128 x 256 tiles with fewer groups
     for groups in (191, 192, 1024):
         sizes = [(5 * i) % 9 for i in range(groups)]
         for v in ("1,2", "1,4"):
